@@ -1,11 +1,13 @@
 /*
- * ipl_b200.h - C ABI of the B200 (sm_100a) fused add+RMSNorm and SiLU-and-mul library.
+ * ipl_b200.h - C ABI of the B200 (sm_100a) fused add+RMSNorm and SiLU-and-mul library, and of its
+ * paged KV cache (rotary positions, attention, pages).
  *
  * Plain pointers and sizes only; no torch types cross this boundary. Every entry point is
- * stream-ordered: it validates its arguments on the host, enqueues at most one kernel on
- * `stream` (a cudaStream_t; NULL means the legacy default stream) of the CURRENT device and
- * returns without synchronising. Device pointers must be memory of the current device.
- * Nothing is allocated on the device.
+ * stream-ordered: it validates its arguments on the host, enqueues its kernels (at most one for
+ * the norm, SiLU and rotary calls) on `stream` (a cudaStream_t; NULL means the legacy default
+ * stream) of the CURRENT device and returns without synchronising. Device pointers must be memory
+ * of the current device. Nothing is allocated on the device: calls that need scratch memory take
+ * it as a workspace, which may be reused by later work on the same stream.
  *
  * Element type is bfloat16 (passed as raw 16-bit words); arithmetic is fp32.
  *
@@ -120,6 +122,148 @@ IPL_API ipl_status ipl_silu_and_mul_bf16(void* output, const void* input, int64_
 IPL_API ipl_status ipl_silu_and_mul_packed_bf16(void* output, const void* input, int64_t rows,
                                         int64_t intermediate_size, void* stream);
 
+/*
+ * Rotary position embedding. For pair i of the first rotary_dim elements of every head, at position
+ * p = positions[token]:
+ *
+ *   (a, b) := (a cos - b sin, b cos + a sin),  cos = cos_sin_cache[p][i],
+ *                                              sin = cos_sin_cache[p][rotary_dim / 2 + i]
+ *
+ * with a, b = x[i], x[rotary_dim / 2 + i] (is_neox != 0) or x[2 i], x[2 i + 1]; fp32 arithmetic, one
+ * rounding. Scaling for long contexts is folded into the table. query is [num_tokens, num_heads,
+ * head_size], key [num_tokens, num_kv_heads, head_size], with the given strides in elements (the last
+ * dimension contiguous). A token whose position is outside the table is skipped and bit 3 of the
+ * device fault word set.
+ *
+ * ipl_rotary_embedding_bf16 rotates query and key in place (the members from value on are ignored).
+ * ipl_rotary_embedding_cache_bf16 rotates query in place and writes the rotated key and the value to
+ * slot slot_mapping[token] of the caches (page slot / page_size, row slot % page_size); key itself is
+ * not modified. A negative slot writes nothing (query is still rotated); a token whose slot lies past
+ * the cache is skipped and bit 3 of the fault word set. Slots of one call must differ.
+ *
+ * No counterpart in the reference's C++ sources, which leave the decoder layer between its two norms
+ * to vLLM; the table is laid out as vLLM's cos_sin_cache.
+ */
+typedef struct ipl_rotary_args {
+    const int64_t* positions;
+    const float* cos_sin_cache; /* [max_position, rotary_dim] */
+    void* query;
+    void* key;
+    int64_t num_tokens, num_heads, num_kv_heads, head_size, rotary_dim, max_position;
+    int64_t query_token_stride, query_head_stride, key_token_stride, key_head_stride;
+    int is_neox;
+    const void* value;
+    void* key_cache;
+    void* value_cache;
+    const int64_t* slot_mapping;
+    int64_t value_token_stride, value_head_stride;
+    int64_t num_pages, page_size;
+    int64_t key_cache_page_stride, key_cache_token_stride, key_cache_head_stride;
+    int64_t value_cache_page_stride, value_cache_token_stride, value_cache_head_stride;
+} ipl_rotary_args;
+
+IPL_API ipl_status ipl_rotary_embedding_bf16(const ipl_rotary_args* args, void* stream);
+IPL_API ipl_status ipl_rotary_embedding_cache_bf16(const ipl_rotary_args* args, void* stream);
+
+/*
+ * Attention of new tokens over a paged KV cache. Sequence s owns the tokens query_start_loc[s] to
+ * query_start_loc[s + 1] - 1 of query (none: it is skipped) and has seq_lens[s] tokens in the cache,
+ * the new ones included. New token j of n sits at position P = seq_lens[s] - n + j and sees the keys at
+ * positions t <= P, with window > 0 only those with t > P - window:
+ *
+ *   output = sum_t w_t v_t / sum_t w_t,   w_t = exp(scale q.k_t - max_t scale q.k_t)
+ *
+ * with fp32 scores, statistics and sums, rounded to bf16 once; the weights enter the product with the
+ * values rounded to bf16 (their fp32 sum is the denominator). A token that sees no key gives 0. Query
+ * head h reads key head h / (num_heads / num_kv_heads). Key t lies in page block_tables[s][t /
+ * page_size], row t % page_size; table entries past a sequence's pages are never read, rows past its
+ * length never matter, whatever they hold. Keys at masked positions never matter either; values that
+ * one token of a sequence sees must be finite for its other tokens to be. A page number outside
+ * 0..num_pages-1 contributes nothing and sets bit 3 of the fault word. Rows of query that belong to no
+ * sequence are not written.
+ *
+ * Strides are in elements; the last dimension is contiguous. max_query_len and max_seq_len are upper
+ * bounds of the lengths, known on the host: they choose the kernels and the split of long rows.
+ * Sequences longer than the bounds are computed all the same, more slowly. The workspace
+ * (ipl_paged_attention_workspace bytes, 16-byte aligned) holds the parts of split rows.
+ *
+ * No counterpart in the reference's C++ sources (see the rotary calls).
+ */
+typedef struct ipl_paged_attention_args {
+    void* output;
+    const void* query;
+    const void* key_cache;
+    const void* value_cache;
+    const int32_t* block_tables;    /* [num_seqs, table_width], row stride table_stride */
+    const int32_t* query_start_loc; /* [num_seqs + 1], non-decreasing from 0 */
+    const int32_t* seq_lens;        /* [num_seqs] */
+    int64_t num_tokens, num_seqs, num_heads, num_kv_heads, head_size;
+    int64_t num_pages, page_size, table_width, table_stride;
+    int64_t output_token_stride, output_head_stride, query_token_stride, query_head_stride;
+    int64_t key_cache_page_stride, key_cache_token_stride, key_cache_head_stride;
+    int64_t value_cache_page_stride, value_cache_token_stride, value_cache_head_stride;
+    int64_t max_query_len, max_seq_len;
+    int64_t window; /* 0: none */
+    double scale;
+    void* workspace;
+    size_t workspace_bytes;
+} ipl_paged_attention_args;
+
+IPL_API ipl_status ipl_paged_attention_bf16(const ipl_paged_attention_args* args, void* stream);
+/* Bytes of workspace the call needs (0: none); pointers are only looked at for their alignment. */
+IPL_API ipl_status ipl_paged_attention_workspace(const ipl_paged_attention_args* args, size_t* bytes);
+/* Names of the kernels the call launches, as the other plan queries. */
+IPL_API const char* ipl_paged_attention_plan(const ipl_paged_attention_args* args);
+
+/*
+ * Pages of a KV cache, managed on the device. The pool's state is a block table per row (entry j: the
+ * page of tokens j * page_size and on, -1 where there is none), a length per row and a reference count
+ * per page; a page is free when its count is 0. Claims take the lowest-numbered free pages in order, so
+ * equal states give equal results. The caches (K and V of every layer) are opaque: num_caches bases in
+ * a host array, page i of each at i * page_stride_bytes, page_bytes long (16-byte multiples; bases
+ * 16-byte aligned). token_bytes > 0 says that a page is its tokens one after the other, so that a
+ * partly filled one need only be copied as far as it is filled; 0: pages are copied whole.
+ *
+ * status receives 0, or the number of free pages lacking, or -1 for an entry out of range (a row, a
+ * length, a row given twice, a child that holds tokens); unless it is 0 nothing has changed. The
+ * workspace (ipl_pages_workspace bytes, 4-byte aligned) may be reused by later work on the stream.
+ *
+ * ipl_copy_pages: page pairs[2 i] to page pairs[2 i + 1] in every cache; negative entries are skipped.
+ *   No target may be the source or target of another pair.
+ * ipl_reserve_pages: rows[i] gets pages up to new_lens[i] tokens, and that length if it was shorter.
+ * ipl_fork_sequences: children[i] (empty) becomes a copy of parents[i]: it shares the whole pages and
+ *   gets a page of its own with the tokens of a partly filled last one.
+ * ipl_release_sequences: the pages of rows[i] lose one reference each, the row becomes empty.
+ * ipl_compact_pages: the pages in use past the first `live` numbers move, in order, to the free numbers
+ *   below. The renumbered tables ([num_rows, width] contiguous) and counts are written beside the old
+ *   ones, which stay valid for work in flight: moved pages keep their data until they are claimed.
+ */
+typedef struct ipl_page_pool {
+    int32_t* block_tables;
+    int32_t* seq_lens;
+    int32_t* ref_counts;
+    int64_t num_rows, width, table_stride, num_pages, page_size;
+} ipl_page_pool;
+
+typedef struct ipl_page_caches {
+    void* const* caches;
+    int64_t num_caches, page_stride_bytes, page_bytes, token_bytes;
+} ipl_page_caches;
+
+IPL_API ipl_status ipl_pages_workspace(int64_t num_pages, int64_t count, size_t* bytes);
+IPL_API ipl_status ipl_copy_pages(const ipl_page_caches* caches, int64_t num_pages, const int32_t* pairs,
+                                  int64_t count, void* stream);
+IPL_API ipl_status ipl_reserve_pages(const ipl_page_pool* pool, const int32_t* rows, const int32_t* new_lens,
+                                     int64_t count, void* workspace, size_t workspace_bytes, int32_t* status,
+                                     void* stream);
+IPL_API ipl_status ipl_fork_sequences(const ipl_page_caches* caches, const ipl_page_pool* pool, const int32_t* parents,
+                                      const int32_t* children, int64_t count, void* workspace,
+                                      size_t workspace_bytes, int32_t* status, void* stream);
+IPL_API ipl_status ipl_release_sequences(const ipl_page_pool* pool, const int32_t* rows, int64_t count, void* stream);
+IPL_API ipl_status ipl_compact_pages(const ipl_page_caches* caches, const ipl_page_pool* pool,
+                                     int32_t* new_block_tables, int32_t* new_ref_counts, int32_t* live,
+                                     void* workspace, size_t workspace_bytes, void* stream);
+
 /* Message of the last failing call on this thread ("" if none). Valid until the next call. */
 IPL_API const char* ipl_last_error(void);
 
@@ -132,8 +276,9 @@ IPL_API int ipl_abi_version(void);
 /*
  * Device-side fault word of `device`: bit flags that a kernel sets when one of its bounded
  * waits on a shared-memory barrier runs out (the kernel then stops early and its outputs are
- * incomplete). 0 means no kernel of this library has given up on that device. Reading it
- * synchronises the device. These waits never run out on a healthy GPU.
+ * incomplete), and bit 3, set when a paged-cache kernel skipped a position, slot, page or row
+ * outside its range. 0 means that neither has happened on that device. Reading it synchronises the
+ * device. The waits never run out on a healthy GPU.
  */
 IPL_API ipl_status ipl_device_fault_flags(int device, uint32_t* flags);
 

@@ -1,0 +1,508 @@
+// Host side of the paged-cache entry points of ipl_b200.h: argument checks, kernel selection, launch.
+#pragma once
+
+#include "cache_pages.cuh"
+#include "ipl_host.cuh"
+#include "paged_attention.cuh"
+#include "rotary.cuh"
+
+namespace ipl {
+namespace {
+
+bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+ipl_status launch_status(cudaError_t err, const char* what) {
+    if (err == cudaSuccess) return IPL_SUCCESS;
+    return fail(IPL_ERROR_CUDA, "%s kernel launch failed: %s", what, cudaGetErrorString(err));
+}
+
+// ------------------------------------------------------------------------------------------
+// rotary positions
+
+ipl_status check_rotary_args(const ipl_rotary_args* a, bool append) {
+    if (a == nullptr) return fail(IPL_ERROR_INVALID_VALUE, "args must be non-null");
+    if (a->num_tokens < 0) return fail(IPL_ERROR_INVALID_VALUE, "number of tokens must be non-negative");
+    if (a->num_heads < 1 || a->num_kv_heads < 1 || a->head_size < 1) {
+        return fail(IPL_ERROR_INVALID_VALUE, "number of heads and head size must be positive");
+    }
+    if (a->rotary_dim < 2 || a->rotary_dim % 2 != 0 || a->rotary_dim > a->head_size) {
+        return fail(IPL_ERROR_INVALID_VALUE, "rotary dimension must be even, positive and at most the head size");
+    }
+    if (a->max_position < 1) return fail(IPL_ERROR_INVALID_VALUE, "cos_sin_cache must have at least one position");
+    if (a->num_tokens > INT_MAX) return fail(IPL_ERROR_TOO_LARGE, "number of tokens is too large");
+    if (a->num_heads > 65536 || a->num_kv_heads > 65536 || a->head_size > 4096) {
+        return fail(IPL_ERROR_TOO_LARGE, "number of heads or head size is too large");
+    }
+    if (append) {
+        if (a->page_size < 1 || a->num_pages < 0) {
+            return fail(IPL_ERROR_INVALID_VALUE, "page size must be positive and number of pages non-negative");
+        }
+        if (a->page_size > INT_MAX || a->num_pages > INT_MAX / a->page_size) {
+            return fail(IPL_ERROR_TOO_LARGE, "the cache holds too many slots");
+        }
+    }
+    if (a->num_tokens == 0) return IPL_SUCCESS;
+    if (a->positions == nullptr || a->cos_sin_cache == nullptr || a->query == nullptr || a->key == nullptr) {
+        return fail(IPL_ERROR_INVALID_VALUE, "positions, query, key and cos_sin_cache must be non-null");
+    }
+    if (append && (a->value == nullptr || a->slot_mapping == nullptr ||
+                   (a->num_pages > 0 && (a->key_cache == nullptr || a->value_cache == nullptr)))) {
+        return fail(IPL_ERROR_INVALID_VALUE, "value, key_cache, value_cache and slot_mapping must be non-null");
+    }
+    if (!aligned(a->positions, 8) || !aligned(a->cos_sin_cache, 4) || (append && !aligned(a->slot_mapping, 8))) {
+        return fail(IPL_ERROR_INVALID_VALUE, "positions, slot_mapping and cos_sin_cache must be aligned to their types");
+    }
+    if (!aligned(a->query, 2) || !aligned(a->key, 2) ||
+        (append && !(aligned(a->value, 2) && aligned(a->key_cache, 2) && aligned(a->value_cache, 2)))) {
+        return fail(IPL_ERROR_INVALID_VALUE, "bfloat16 pointers must be 2-byte aligned");
+    }
+    return IPL_SUCCESS;
+}
+
+// Whether every 16-byte chunk of the call is 16-byte aligned and holds whole pairs' halves.
+bool rotary_vectorises(const ipl_rotary_args& a, bool append) {
+    int64_t strides = a.query_token_stride | a.query_head_stride | a.key_token_stride | a.key_head_stride;
+    bool pointers = aligned(a.query, 16) && aligned(a.key, 16) && aligned(a.cos_sin_cache, 16);
+    if (append) {
+        strides |= a.value_token_stride | a.value_head_stride | a.key_cache_page_stride | a.key_cache_token_stride |
+                   a.key_cache_head_stride | a.value_cache_page_stride | a.value_cache_token_stride |
+                   a.value_cache_head_stride | a.head_size;
+        pointers = pointers && aligned(a.value, 16) && aligned(a.key_cache, 16) && aligned(a.value_cache, 16);
+    }
+    return pointers && strides % 8 == 0 && a.rotary_dim % (a.is_neox ? 16 : 8) == 0;
+}
+
+template <bool kAppend>
+ipl_status run_rotary(const ipl_rotary_args* a, cudaStream_t stream) {
+    const ipl_status st = check_rotary_args(a, kAppend);
+    if (st != IPL_SUCCESS || a->num_tokens == 0) return st;
+    const bool vector = rotary_vectorises(*a, kAppend);
+    RotaryParams p = {};
+    p.positions = a->positions;
+    p.cos_sin = a->cos_sin_cache;
+    p.max_position = a->max_position;
+    p.rot = static_cast<int>(a->rotary_dim);
+    p.tokens = static_cast<uint32_t>(a->num_tokens);
+    p.q = static_cast<uint16_t*>(a->query);
+    p.k = static_cast<uint16_t*>(a->key);
+    p.q_token = a->query_token_stride, p.q_head = a->query_head_stride;
+    p.k_token = a->key_token_stride, p.k_head = a->key_head_stride;
+    p.q_heads = static_cast<uint32_t>(a->num_heads);
+    const uint32_t kv_heads = static_cast<uint32_t>(a->num_kv_heads);
+    const int64_t chunks = !vector ? a->rotary_dim / 2 : a->is_neox ? a->rotary_dim / 16 : a->rotary_dim / 8;
+    const int64_t pass = (a->head_size - a->rotary_dim) / (vector ? 8 : 1);
+    const int64_t v_chunks = a->head_size / (vector ? 8 : 1);
+    p.rotated_items = (p.q_heads + kv_heads) * static_cast<uint32_t>(chunks);
+    p.items = p.rotated_items;
+    p.rot_chunks = make_fast_div32(static_cast<uint32_t>(chunks));
+    if (kAppend) {
+        p.v = static_cast<const uint16_t*>(a->value);
+        p.slots = a->slot_mapping;
+        p.num_slots = a->num_pages * a->page_size;
+        p.page_size = make_fast_div32(static_cast<uint32_t>(a->page_size));
+        p.key_cache = static_cast<uint16_t*>(a->key_cache);
+        p.value_cache = static_cast<uint16_t*>(a->value_cache);
+        p.v_token = a->value_token_stride, p.v_head = a->value_head_stride;
+        p.key_page = a->key_cache_page_stride, p.key_token = a->key_cache_token_stride;
+        p.key_head = a->key_cache_head_stride;
+        p.value_page = a->value_cache_page_stride, p.value_token = a->value_cache_token_stride;
+        p.value_head = a->value_cache_head_stride;
+        p.passed_items = kv_heads * static_cast<uint32_t>(pass);
+        p.pass_chunks = make_fast_div32(static_cast<uint32_t>(pass > 0 ? pass : 1));
+        p.v_chunks = make_fast_div32(static_cast<uint32_t>(v_chunks));
+        p.items += p.passed_items + kv_heads * static_cast<uint32_t>(v_chunks);
+    }
+    p.items_div = make_fast_div32(p.items);
+    p.tokens_per_cta = p.items < kRotaryThreads ? kRotaryThreads / p.items : 1;
+    const unsigned grid = (p.tokens + p.tokens_per_cta - 1) / p.tokens_per_cta;
+    cudaError_t err;
+    if (vector) {
+        err = a->is_neox ? launch(rotary_kernel<true, true, kAppend>, grid, kRotaryThreads, 0, stream, p)
+                         : launch(rotary_kernel<true, false, kAppend>, grid, kRotaryThreads, 0, stream, p);
+    } else {
+        err = a->is_neox ? launch(rotary_kernel<false, true, kAppend>, grid, kRotaryThreads, 0, stream, p)
+                         : launch(rotary_kernel<false, false, kAppend>, grid, kRotaryThreads, 0, stream, p);
+    }
+    return launch_status(err, "rotary embedding");
+}
+
+// ------------------------------------------------------------------------------------------
+// attention
+
+ipl_status check_attention_args(const ipl_paged_attention_args* a) {
+    if (a == nullptr) return fail(IPL_ERROR_INVALID_VALUE, "args must be non-null");
+    if (a->num_tokens < 0 || a->num_seqs < 0 || a->num_pages < 0 || a->table_width < 0) {
+        return fail(IPL_ERROR_INVALID_VALUE, "sizes must be non-negative");
+    }
+    if (a->num_heads < 1 || a->num_kv_heads < 1 || a->head_size < 1 || a->page_size < 1) {
+        return fail(IPL_ERROR_INVALID_VALUE, "number of heads, head size and page size must be positive");
+    }
+    if (a->num_heads % a->num_kv_heads != 0) {
+        return fail(IPL_ERROR_INVALID_VALUE, "number of query heads must be a multiple of the number of key heads");
+    }
+    if (a->max_query_len < 0 || a->max_seq_len < 0 || a->window < 0) {
+        return fail(IPL_ERROR_INVALID_VALUE, "max_query_len, max_seq_len and window must be non-negative");
+    }
+    if (!(a->scale > 0.0) || a->scale > 1e30) return fail(IPL_ERROR_INVALID_VALUE, "scale must be positive and finite");
+    if (a->head_size > kAttentionMaxDim) {
+        return fail(IPL_ERROR_TOO_LARGE, "head size must be at most %d", kAttentionMaxDim);
+    }
+    if (a->num_tokens > INT_MAX / 2 || a->num_seqs > INT_MAX / 2 || a->num_heads > 65536 || a->num_pages > INT_MAX ||
+        a->page_size > INT_MAX || a->table_width > INT_MAX || a->max_seq_len > INT_MAX / 2 ||
+        a->num_tokens > INT64_MAX / 65536 / 256 || a->num_tokens * a->num_heads > INT64_C(4) * INT_MAX) {
+        return fail(IPL_ERROR_TOO_LARGE, "a size is too large");
+    }
+    if (a->num_tokens == 0 || a->num_seqs == 0) return IPL_SUCCESS;
+    if (a->output == nullptr || a->query == nullptr || a->block_tables == nullptr || a->query_start_loc == nullptr ||
+        a->seq_lens == nullptr || (a->num_pages > 0 && (a->key_cache == nullptr || a->value_cache == nullptr))) {
+        return fail(IPL_ERROR_INVALID_VALUE,
+                    "output, query, key_cache, value_cache, block_tables, query_start_loc and seq_lens must be non-null");
+    }
+    if (!aligned(a->output, 2) || !aligned(a->query, 2) || !aligned(a->key_cache, 2) || !aligned(a->value_cache, 2)) {
+        return fail(IPL_ERROR_INVALID_VALUE, "bfloat16 pointers must be 2-byte aligned");
+    }
+    if (!aligned(a->block_tables, 4) || !aligned(a->query_start_loc, 4) || !aligned(a->seq_lens, 4)) {
+        return fail(IPL_ERROR_INVALID_VALUE, "int32 pointers must be 4-byte aligned");
+    }
+    return IPL_SUCCESS;
+}
+
+AttentionParams attention_params(const ipl_paged_attention_args& a) {
+    AttentionParams p = {};
+    p.out = static_cast<uint16_t*>(a.output);
+    p.q = static_cast<const uint16_t*>(a.query);
+    p.key_cache = static_cast<const uint16_t*>(a.key_cache);
+    p.value_cache = static_cast<const uint16_t*>(a.value_cache);
+    p.tables = a.block_tables;
+    p.starts = a.query_start_loc;
+    p.lens = a.seq_lens;
+    p.num_tokens = static_cast<int>(a.num_tokens);
+    p.num_seqs = static_cast<int>(a.num_seqs);
+    p.heads = static_cast<int>(a.num_heads);
+    p.kv_heads = static_cast<int>(a.num_kv_heads);
+    p.group = p.heads / p.kv_heads;
+    p.dim = static_cast<int>(a.head_size);
+    p.page_size = static_cast<int>(a.page_size);
+    p.num_pages = static_cast<int>(a.num_pages);
+    p.table_width = static_cast<int>(a.table_width);
+    p.window = a.window > 0 && a.window < INT_MAX ? static_cast<int>(a.window) : INT_MAX;
+    p.table_row = a.table_stride;
+    p.out_token = a.output_token_stride, p.out_head = a.output_head_stride;
+    p.q_token = a.query_token_stride, p.q_head = a.query_head_stride;
+    p.key_page = a.key_cache_page_stride, p.key_token = a.key_cache_token_stride, p.key_head = a.key_cache_head_stride;
+    p.value_page = a.value_cache_page_stride, p.value_token = a.value_cache_token_stride;
+    p.value_head = a.value_cache_head_stride;
+    p.scale_log2 = static_cast<float>(a.scale * 1.4426950408889634);
+    return p;
+}
+
+ipl_status run_attention(const ipl_paged_attention_args* a, cudaStream_t stream) {
+    const ipl_status st = check_attention_args(a);
+    if (st != IPL_SUCCESS || a->num_tokens == 0 || a->num_seqs == 0) return st;
+    const AttentionParams p = attention_params(*a);
+    const int64_t rows = a->num_tokens * a->num_heads;
+    const unsigned grid = static_cast<unsigned>((rows + kAttentionRowWarps - 1) / kAttentionRowWarps);
+    return launch_status(launch(attention_row_kernel, grid, kAttentionRowWarps * kWarpSize, 0, stream, p), "paged attention");
+}
+
+// ------------------------------------------------------------------------------------------
+// pages
+
+ipl_status check_pool(const ipl_page_pool* pool) {
+    if (pool == nullptr) return fail(IPL_ERROR_INVALID_VALUE, "pool must be non-null");
+    if (pool->num_rows < 0 || pool->width < 0 || pool->num_pages < 0 || pool->page_size < 1) {
+        return fail(IPL_ERROR_INVALID_VALUE, "sizes of the pool must be non-negative and its page size positive");
+    }
+    if (pool->num_rows > INT_MAX || pool->width > INT_MAX || pool->num_pages > INT_MAX / 2 || pool->page_size > INT_MAX) {
+        return fail(IPL_ERROR_TOO_LARGE, "a size of the pool is too large");
+    }
+    if ((pool->num_rows > 0 && pool->width > 0 && pool->block_tables == nullptr) ||
+        (pool->num_pages > 0 && pool->ref_counts == nullptr)) {
+        return fail(IPL_ERROR_INVALID_VALUE, "block_tables and ref_counts must be non-null");
+    }
+    if (!aligned(pool->block_tables, 4) || !aligned(pool->seq_lens, 4) || !aligned(pool->ref_counts, 4)) {
+        return fail(IPL_ERROR_INVALID_VALUE, "int32 pointers must be 4-byte aligned");
+    }
+    return IPL_SUCCESS;
+}
+
+ipl_status check_rows(const ipl_page_pool* pool, const void* rows, const void* other, int64_t count) {
+    if (count < 0) return fail(IPL_ERROR_INVALID_VALUE, "number of rows must be non-negative");
+    if (count > INT_MAX / 2) return fail(IPL_ERROR_TOO_LARGE, "number of rows is too large");
+    if (count > 0 && (rows == nullptr || other == nullptr)) {
+        return fail(IPL_ERROR_INVALID_VALUE, "the lists of rows must be non-null");
+    }
+    if (pool->num_rows > 0 && pool->seq_lens == nullptr) {
+        return fail(IPL_ERROR_INVALID_VALUE, "seq_lens must be non-null");
+    }
+    if (!aligned(rows, 4) || !aligned(other, 4)) return fail(IPL_ERROR_INVALID_VALUE, "int32 pointers must be 4-byte aligned");
+    return IPL_SUCCESS;
+}
+
+ipl_status check_caches(const ipl_page_caches* c) {
+    if (c == nullptr) return fail(IPL_ERROR_INVALID_VALUE, "caches must be non-null");
+    if (c->num_caches < 0 || c->page_bytes < 0 || c->token_bytes < 0 || c->page_stride_bytes < c->page_bytes) {
+        return fail(IPL_ERROR_INVALID_VALUE, "sizes of the caches must be non-negative and pages must not overlap");
+    }
+    if (c->num_caches > 65536) return fail(IPL_ERROR_TOO_LARGE, "too many caches");
+    if (c->num_caches > 0 && c->caches == nullptr) return fail(IPL_ERROR_INVALID_VALUE, "caches must be non-null");
+    bool ok = (c->page_bytes | c->token_bytes | c->page_stride_bytes) % 16 == 0;
+    for (int64_t i = 0; i < c->num_caches; ++i) {
+        if (c->caches[i] == nullptr && c->page_bytes > 0) return fail(IPL_ERROR_INVALID_VALUE, "caches must be non-null");
+        ok = ok && aligned(c->caches[i], 16);
+    }
+    if (!ok) return fail(IPL_ERROR_MISALIGNED, "pages must be 16-byte aligned multiples of 16 bytes");
+    return IPL_SUCCESS;
+}
+
+PageState page_state(const ipl_page_pool& pool) {
+    PageState s;
+    s.tables = pool.block_tables;
+    s.table_row = pool.table_stride;
+    s.lens = pool.seq_lens;
+    s.ref_counts = pool.ref_counts;
+    s.num_rows = static_cast<int>(pool.num_rows);
+    s.width = static_cast<int>(pool.width);
+    s.num_pages = static_cast<int>(pool.num_pages);
+    s.page_size = static_cast<int>(pool.page_size);
+    return s;
+}
+
+// The caches from number `from` on, as many as one launch takes.
+int cache_list(const ipl_page_caches& c, int64_t from, CacheList* list) {
+    int n = 0;
+    for (; n < kMaxCachesPerLaunch && from + n < c.num_caches; ++n) list->cache[n] = static_cast<char*>(c.caches[from + n]);
+    return n;
+}
+
+// Workspace of the page calls: first and parent_lens [count], then three lists of num_pages, then one.
+size_t pages_workspace_bytes(int64_t num_pages, int64_t count) {
+    return static_cast<size_t>(2 * count + 3 * num_pages + 1) * sizeof(int32_t);
+}
+
+ipl_status check_workspace(const void* workspace, size_t bytes, int64_t num_pages, int64_t count) {
+    if (workspace == nullptr || !aligned(workspace, 4)) {
+        return fail(IPL_ERROR_INVALID_VALUE, "workspace must be non-null and 4-byte aligned");
+    }
+    if (bytes < pages_workspace_bytes(num_pages, count)) return fail(IPL_ERROR_INVALID_VALUE, "workspace is too small");
+    return IPL_SUCCESS;
+}
+
+ClaimParams claim_params(const ipl_page_pool& pool, const int32_t* parents, const int32_t* rows, const int32_t* new_lens,
+                         int64_t count, void* workspace, int32_t* status) {
+    ClaimParams p = {};
+    p.state = page_state(pool);
+    p.parents = parents;
+    p.rows = rows;
+    p.new_lens = new_lens;
+    p.count = static_cast<int>(count);
+    p.first = static_cast<int32_t*>(workspace);
+    p.parent_lens = p.first + count;
+    p.fresh = p.parent_lens + count;
+    p.status = status;
+    return p;
+}
+
+}  // namespace
+}  // namespace ipl
+
+extern "C" {
+
+ipl_status ipl_rotary_embedding_bf16(const ipl_rotary_args* args, void* stream) {
+    return ipl::run_rotary<false>(args, static_cast<cudaStream_t>(stream));
+}
+
+ipl_status ipl_rotary_embedding_cache_bf16(const ipl_rotary_args* args, void* stream) {
+    return ipl::run_rotary<true>(args, static_cast<cudaStream_t>(stream));
+}
+
+ipl_status ipl_paged_attention_bf16(const ipl_paged_attention_args* args, void* stream) {
+    return ipl::run_attention(args, static_cast<cudaStream_t>(stream));
+}
+
+ipl_status ipl_paged_attention_workspace(const ipl_paged_attention_args* args, size_t* bytes) {
+    using namespace ipl;
+    if (bytes == nullptr) return fail(IPL_ERROR_INVALID_VALUE, "bytes must be non-null");
+    const ipl_status st = check_attention_args(args);
+    if (st == IPL_SUCCESS) *bytes = 0;
+    return st;
+}
+
+const char* ipl_paged_attention_plan(const ipl_paged_attention_args* args) {
+    using namespace ipl;
+    if (check_attention_args(args) != IPL_SUCCESS) return "invalid";
+    return args->num_tokens == 0 || args->num_seqs == 0 ? "none" : "attention_row_kernel";
+}
+
+ipl_status ipl_pages_workspace(int64_t num_pages, int64_t count, size_t* bytes) {
+    using namespace ipl;
+    if (bytes == nullptr || num_pages < 0 || count < 0 || num_pages > INT_MAX || count > INT_MAX) {
+        return fail(IPL_ERROR_INVALID_VALUE, "bytes must be non-null and the sizes non-negative 32-bit numbers");
+    }
+    *bytes = pages_workspace_bytes(num_pages, count);
+    return IPL_SUCCESS;
+}
+
+ipl_status ipl_copy_pages(const ipl_page_caches* caches, int64_t num_pages, const int32_t* pairs, int64_t count,
+                          void* stream) {
+    using namespace ipl;
+    ipl_status st = check_caches(caches);
+    if (st != IPL_SUCCESS) return st;
+    if (num_pages < 0 || count < 0) return fail(IPL_ERROR_INVALID_VALUE, "sizes must be non-negative");
+    if (num_pages > INT_MAX || count > INT_MAX / kMaxCachesPerLaunch) return fail(IPL_ERROR_TOO_LARGE, "a size is too large");
+    if (count == 0 || caches->page_bytes == 0) return IPL_SUCCESS;
+    if (pairs == nullptr || !aligned(pairs, 4)) {
+        return fail(IPL_ERROR_INVALID_VALUE, "pairs must be non-null and 4-byte aligned");
+    }
+    for (int64_t from = 0; from < caches->num_caches; from += kMaxCachesPerLaunch) {
+        CopyPagesParams p = {};
+        p.num_caches = cache_list(*caches, from, &p.caches);
+        p.pairs = pairs;
+        p.num_pages = static_cast<int>(num_pages);
+        p.page_stride = caches->page_stride_bytes;
+        p.page_bytes = caches->page_bytes;
+        const unsigned grid = static_cast<unsigned>(count * p.num_caches);
+        st = launch_status(launch(page_copy_kernel, grid, kPageCopyThreads, 0, static_cast<cudaStream_t>(stream), p), "page copy");
+        if (st != IPL_SUCCESS) return st;
+    }
+    return IPL_SUCCESS;
+}
+
+ipl_status ipl_reserve_pages(const ipl_page_pool* pool, const int32_t* rows, const int32_t* new_lens, int64_t count,
+                             void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+    using namespace ipl;
+    ipl_status st = check_pool(pool);
+    if (st == IPL_SUCCESS) st = check_rows(pool, rows, new_lens, count);
+    if (st == IPL_SUCCESS) st = check_workspace(workspace, workspace_bytes, pool->num_pages, count);
+    if (st != IPL_SUCCESS) return st;
+    if (status == nullptr || !aligned(status, 4)) {
+        return fail(IPL_ERROR_INVALID_VALUE, "status must be non-null and 4-byte aligned");
+    }
+    const ClaimParams p = claim_params(*pool, nullptr, rows, new_lens, count, workspace, status);
+    return launch_status(launch(page_claim_kernel<false>, 1, kPlanThreads, 0, static_cast<cudaStream_t>(stream), p), "page claim");
+}
+
+ipl_status ipl_fork_sequences(const ipl_page_caches* caches, const ipl_page_pool* pool, const int32_t* parents,
+                              const int32_t* children, int64_t count, void* workspace, size_t workspace_bytes,
+                              int32_t* status, void* stream) {
+    using namespace ipl;
+    ipl_status st = check_caches(caches);
+    if (st == IPL_SUCCESS) st = check_pool(pool);
+    if (st == IPL_SUCCESS) st = check_rows(pool, parents, children, count);
+    if (st == IPL_SUCCESS) st = check_workspace(workspace, workspace_bytes, pool->num_pages, count);
+    if (st != IPL_SUCCESS) return st;
+    if (status == nullptr || !aligned(status, 4)) {
+        return fail(IPL_ERROR_INVALID_VALUE, "status must be non-null and 4-byte aligned");
+    }
+    if (count > INT_MAX / kMaxCachesPerLaunch) return fail(IPL_ERROR_TOO_LARGE, "number of rows is too large");
+    if (caches->token_bytes > 0 && caches->token_bytes * pool->page_size != caches->page_bytes) {
+        return fail(IPL_ERROR_INVALID_VALUE, "a page must hold page_size tokens of token_bytes");
+    }
+    const ClaimParams claim = claim_params(*pool, parents, children, nullptr, count, workspace, status);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    st = launch_status(launch(page_claim_kernel<true>, 1, kPlanThreads, 0, s, claim), "page claim");
+    if (st != IPL_SUCCESS || count == 0) return st;
+    int64_t from = 0;
+    do {
+        ForkParams p = {};
+        p.num_caches = cache_list(*caches, from, &p.caches);
+        p.with_tables = from == 0;
+        p.state = claim.state;
+        p.parents = parents;
+        p.children = children;
+        p.first = claim.first;
+        p.parent_lens = claim.parent_lens;
+        p.fresh = claim.fresh;
+        p.status = status;
+        p.page_stride = caches->page_stride_bytes;
+        p.page_bytes = caches->page_bytes;
+        p.token_bytes = caches->token_bytes;
+        if (p.num_caches == 0) {  // tables alone
+            p.num_caches = 1;
+            p.page_bytes = p.token_bytes = 0;
+        }
+        const unsigned grid = static_cast<unsigned>(count * p.num_caches);
+        st = launch_status(launch(page_fork_kernel, grid, kPageCopyThreads, 0, s, p), "page fork");
+        if (st != IPL_SUCCESS) return st;
+        from += kMaxCachesPerLaunch;
+    } while (from < caches->num_caches);
+    return IPL_SUCCESS;
+}
+
+ipl_status ipl_release_sequences(const ipl_page_pool* pool, const int32_t* rows, int64_t count, void* stream) {
+    using namespace ipl;
+    ipl_status st = check_pool(pool);
+    if (st == IPL_SUCCESS) st = check_rows(pool, rows, rows, count);
+    if (st != IPL_SUCCESS || count == 0) return st;
+    return launch_status(launch(page_release_kernel, static_cast<unsigned>(count), kReleaseThreads, 0,
+                                static_cast<cudaStream_t>(stream), page_state(*pool), rows),
+                         "page release");
+}
+
+ipl_status ipl_compact_pages(const ipl_page_caches* caches, const ipl_page_pool* pool, int32_t* new_block_tables,
+                             int32_t* new_ref_counts, int32_t* live, void* workspace, size_t workspace_bytes,
+                             void* stream) {
+    using namespace ipl;
+    ipl_status st = check_caches(caches);
+    if (st == IPL_SUCCESS) st = check_pool(pool);
+    if (st == IPL_SUCCESS) st = check_workspace(workspace, workspace_bytes, pool->num_pages, 0);
+    if (st != IPL_SUCCESS) return st;
+    if ((pool->num_rows > 0 && pool->width > 0 && new_block_tables == nullptr) ||
+        (pool->num_pages > 0 && new_ref_counts == nullptr) || live == nullptr) {
+        return fail(IPL_ERROR_INVALID_VALUE, "new_block_tables, new_ref_counts and live must be non-null");
+    }
+    if (!aligned(new_block_tables, 4) || !aligned(new_ref_counts, 4) || !aligned(live, 4)) {
+        return fail(IPL_ERROR_INVALID_VALUE, "int32 pointers must be 4-byte aligned");
+    }
+    if (pool->num_rows > 0 && pool->num_pages > 0 &&
+        (new_block_tables == pool->block_tables || new_ref_counts == pool->ref_counts)) {
+        return fail(IPL_ERROR_INVALID_VALUE, "the new tables and counts must not alias the old ones");
+    }
+    int device = 0;
+    DeviceInfo* info = nullptr;
+    st = current_device(&device, &info);
+    if (st != IPL_SUCCESS) return st;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    CompactPlanParams plan = {};
+    plan.ref_counts = pool->ref_counts;
+    plan.new_ref_counts = new_ref_counts;
+    plan.num_pages = static_cast<int>(pool->num_pages);
+    plan.live = live;
+    plan.map = static_cast<int32_t*>(workspace);
+    plan.holes = plan.map + pool->num_pages;
+    plan.movers = plan.holes + pool->num_pages;
+    plan.moves = plan.movers + pool->num_pages;
+    st = launch_status(launch(page_compact_plan_kernel, 1, kPlanThreads, 0, s, plan), "page compaction plan");
+    if (st != IPL_SUCCESS) return st;
+    int64_t from = 0;
+    do {
+        CompactMoveParams p = {};
+        p.num_caches = cache_list(*caches, from, &p.caches);
+        p.tables = from == 0 && pool->num_rows > 0 ? pool->block_tables : nullptr;
+        p.new_tables = new_block_tables;
+        p.table_row = pool->table_stride;
+        p.num_rows = static_cast<int>(pool->num_rows);
+        p.width = static_cast<int>(pool->width);
+        p.num_pages = plan.num_pages;
+        p.moves = plan.moves;
+        p.map = plan.map;
+        p.holes = plan.holes;
+        p.movers = plan.movers;
+        p.page_stride = caches->page_stride_bytes;
+        p.page_bytes = caches->page_bytes;
+        // At most half the pages move; the kernel's loop covers what the grid does not.
+        const int64_t most = pool->num_pages / 2 * p.num_caches;
+        const int64_t entries = (pool->num_rows * pool->width + kPageCopyThreads - 1) / kPageCopyThreads;
+        const int64_t cap = static_cast<int64_t>(info->sm_count.load(std::memory_order_relaxed)) * 8;
+        int64_t grid = most > entries ? most : entries;
+        grid = grid < 1 ? 1 : grid > cap ? cap : grid;
+        if (p.num_caches == 0) p.num_caches = 1, p.page_bytes = 0;
+        st = launch_status(launch(page_compact_move_kernel, static_cast<unsigned>(grid), kPageCopyThreads, 0, s, p),
+                           "page compaction");
+        if (st != IPL_SUCCESS) return st;
+        from += kMaxCachesPerLaunch;
+    } while (from < caches->num_caches);
+    return IPL_SUCCESS;
+}
+
+}  // extern "C"

@@ -18,6 +18,7 @@ constexpr int kWarpSize = 32;
 constexpr uint32_t kFaultFullBarrierTimeout = 1u << 0;   // a consumer never saw its stage fill
 constexpr uint32_t kFaultEmptyBarrierTimeout = 1u << 1;  // the producer never saw a stage drain
 constexpr uint32_t kFaultCopyDrainTimeout = 1u << 2;     // a copy the producer issued never landed
+constexpr uint32_t kFaultIndexOutOfRange = 1u << 3;      // a position, slot, page or row index outside its range was skipped
 
 // Bounded waits give up after this long (nanoseconds of %globaltimer). A stage fills within
 // microseconds on a healthy GPU; the bound only exists so that a lost copy ends the kernel

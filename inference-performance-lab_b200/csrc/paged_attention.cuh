@@ -1,0 +1,140 @@
+// Attention of new tokens over a paged KV cache, for sm_100a.
+//
+// Token j of the n new ones of a sequence of L tokens (its own keys and values already in the cache)
+// sits at position P = L - n + j and sees the keys t with max(0, P - window + 1) <= t <= P:
+//
+//   out = sum_t exp(scale q.k_t - m) v_t / sum_t exp(scale q.k_t - m),   m = max_t scale q.k_t
+//
+// in one pass over the keys with a running m and sum (fp32). A token that sees no key gives 0.
+// Query head h reads key head h / (heads / kv_heads). Key t of a sequence lies in page
+// table[t / page_size], row t % page_size.
+#pragma once
+
+#include "ipl_common.cuh"
+
+namespace ipl {
+
+constexpr int kAttentionMaxDim = 256;
+
+struct AttentionParams {
+    uint16_t* out;
+    const uint16_t* q;
+    const uint16_t* key_cache;
+    const uint16_t* value_cache;
+    const int32_t* tables;
+    const int32_t* starts;
+    const int32_t* lens;
+    int num_tokens, num_seqs, heads, kv_heads, group, dim, page_size, num_pages, table_width;
+    int window;  // INT_MAX without one
+    int64_t table_row;
+    int64_t out_token, out_head, q_token, q_head;
+    int64_t key_page, key_token, key_head, value_page, value_token, value_head;
+    float scale_log2;  // scale * log2(e): the exponentials are powers of two
+};
+
+// The sequence that token `token` belongs to: the last s with starts[s] <= token.
+__device__ __forceinline__ int sequence_of_token(const int32_t* starts, int num_seqs, int token) {
+    int lo = 0, hi = num_seqs - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (starts[mid] <= token) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+// A sequence's length as far as its row of the block table reaches.
+__device__ __forceinline__ int table_bounded_length(const AttentionParams& p, int seq) {
+    const int64_t most = static_cast<int64_t>(p.table_width) * p.page_size;
+    const int len = p.lens[seq];
+    if (len > most) {
+        atomicOr(&g_fault_word, kFaultIndexOutOfRange);
+        return static_cast<int>(most);
+    }
+    return len;
+}
+
+__device__ __forceinline__ float warp_max(float value) {
+#pragma unroll
+    for (int offset = kWarpSize / 2; offset > 0; offset >>= 1) {
+        value = fmaxf(value, __shfl_xor_sync(0xffffffffu, value, offset));
+    }
+    return value;
+}
+
+// Any head size up to 256, page size, stride and alignment: a warp for each (token, head), a key a
+// lane for the scores, an element a lane (and every 32nd further) for the sum of values.
+constexpr int kAttentionRowWarps = 4;
+
+__global__ void __launch_bounds__(kAttentionRowWarps * kWarpSize) attention_row_kernel(const AttentionParams p) {
+    __shared__ float q_rows[kAttentionRowWarps][kAttentionMaxDim];
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const int warp = threadIdx.x / kWarpSize, lane = threadIdx.x % kWarpSize;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * kAttentionRowWarps + warp;
+    if (row >= static_cast<int64_t>(p.num_tokens) * p.heads) return;
+    const int token = static_cast<int>(row / p.heads), head = static_cast<int>(row % p.heads);
+    const int seq = sequence_of_token(p.starts, p.num_seqs, token);
+    const int begin = p.starts[seq], end = p.starts[seq + 1];
+    if (token < begin || token >= end) return;  // padding
+    float* q = q_rows[warp];
+    for (int d = lane; d < p.dim; d += kWarpSize) {
+        q[d] = bf16_bits_to_float(p.q[token * p.q_token + head * p.q_head + d]);
+    }
+    __syncwarp();
+    const int len = table_bounded_length(p, seq);
+    const int position = p.lens[seq] - (end - begin) + (token - begin);
+    const int stop = min(position + 1, len);
+    const int first = position >= p.window ? position - p.window + 1 : 0;
+    const int32_t* table = p.tables + seq * p.table_row;
+    const int kv_head = head / p.group;
+
+    constexpr int kSlots = kAttentionMaxDim / kWarpSize;
+    float acc[kSlots] = {};
+    float top = -INFINITY, sum = 0.0f;
+    for (int base = first; base < stop; base += kWarpSize) {
+        const int key = base + lane;
+        int page = -1;
+        float score = -INFINITY;
+        if (key < stop) {
+            page = table[key / p.page_size];
+            if (page < 0 || page >= p.num_pages) {
+                atomicOr(&g_fault_word, kFaultIndexOutOfRange);
+                page = -1;
+            } else {
+                const uint16_t* k = p.key_cache + page * p.key_page + (key % p.page_size) * p.key_token + kv_head * p.key_head;
+                float dot = 0.0f;
+                for (int d = 0; d < p.dim; ++d) dot += q[d] * bf16_bits_to_float(k[d]);
+                score = dot * p.scale_log2;
+            }
+        }
+        const float new_top = fmaxf(top, warp_max(score));
+        if (new_top == -INFINITY) continue;
+        const float weight = exp2f(score - new_top);
+        const float keep = exp2f(top - new_top);
+        sum = sum * keep + warp_sum(weight);
+        top = new_top;
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i) acc[i] *= keep;
+        for (int j = 0; j < kWarpSize; ++j) {
+            const float w = __shfl_sync(0xffffffffu, weight, j);
+            const int from = __shfl_sync(0xffffffffu, page, j);
+            if (from < 0) continue;
+            const int t = base + j;
+            const uint16_t* v = p.value_cache + from * p.value_page + (t % p.page_size) * p.value_token + kv_head * p.value_head;
+#pragma unroll
+            for (int i = 0; i < kSlots; ++i) {
+                const int d = lane + i * kWarpSize;
+                if (d < p.dim) acc[i] += w * bf16_bits_to_float(v[d]);
+            }
+        }
+    }
+    const float inverse = sum > 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) {
+        const int d = lane + i * kWarpSize;
+        if (d < p.dim) p.out[token * p.out_token + head * p.out_head + d] = float_to_bf16_bits(acc[i] * inverse);
+    }
+}
+
+}  // namespace ipl

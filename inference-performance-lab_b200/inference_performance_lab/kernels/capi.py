@@ -18,6 +18,62 @@ IPL_ERROR_MISALIGNED = 2
 IPL_ERROR_TOO_LARGE = 3
 IPL_ERROR_CUDA = 4
 
+
+
+def _fields(pointers: str = "", sizes: str = "") -> list[tuple[str, object]]:
+    return [(n, ctypes.c_void_p) for n in pointers.split()] + [(n, ctypes.c_int64) for n in sizes.split()]
+
+
+class RotaryArgs(ctypes.Structure):
+    """``ipl_rotary_args``."""
+
+    _fields_ = [
+        *_fields(
+            "positions cos_sin_cache query key",
+            "num_tokens num_heads num_kv_heads head_size rotary_dim max_position query_token_stride query_head_stride"
+            " key_token_stride key_head_stride",
+        ),
+        ("is_neox", ctypes.c_int),
+        *_fields(
+            "value key_cache value_cache slot_mapping",
+            "value_token_stride value_head_stride num_pages page_size key_cache_page_stride key_cache_token_stride"
+            " key_cache_head_stride value_cache_page_stride value_cache_token_stride value_cache_head_stride",
+        ),
+    ]
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    """``ipl_paged_attention_args``."""
+
+    _fields_ = [
+        *_fields(
+            "output query key_cache value_cache block_tables query_start_loc seq_lens",
+            "num_tokens num_seqs num_heads num_kv_heads head_size num_pages page_size table_width table_stride"
+            " output_token_stride output_head_stride query_token_stride query_head_stride key_cache_page_stride"
+            " key_cache_token_stride key_cache_head_stride value_cache_page_stride value_cache_token_stride"
+            " value_cache_head_stride max_query_len max_seq_len window",
+        ),
+        ("scale", ctypes.c_double),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class PagePool(ctypes.Structure):
+    """``ipl_page_pool``."""
+
+    _fields_ = _fields("block_tables seq_lens ref_counts", "num_rows width table_stride num_pages page_size")
+
+
+class PageCaches(ctypes.Structure):
+    """``ipl_page_caches``."""
+
+    _fields_ = [
+        ("caches", ctypes.POINTER(ctypes.c_void_p)),
+        *_fields("", "num_caches page_stride_bytes page_bytes token_bytes"),
+    ]
+
+
 # name -> (restype, argtypes): every symbol include/ipl_b200.h declares.
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ipl_fused_add_rms_norm_bf16": (
@@ -65,6 +121,63 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ipl_silu_and_mul_packed_bf16": (
         ctypes.c_int,
         [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p],
+    ),
+    "ipl_rotary_embedding_bf16": (ctypes.c_int, [ctypes.POINTER(RotaryArgs), ctypes.c_void_p]),
+    "ipl_rotary_embedding_cache_bf16": (ctypes.c_int, [ctypes.POINTER(RotaryArgs), ctypes.c_void_p]),
+    "ipl_paged_attention_bf16": (ctypes.c_int, [ctypes.POINTER(PagedAttentionArgs), ctypes.c_void_p]),
+    "ipl_paged_attention_workspace": (
+        ctypes.c_int,
+        [ctypes.POINTER(PagedAttentionArgs), ctypes.POINTER(ctypes.c_size_t)],
+    ),
+    "ipl_paged_attention_plan": (ctypes.c_char_p, [ctypes.POINTER(PagedAttentionArgs)]),
+    "ipl_pages_workspace": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, ctypes.POINTER(ctypes.c_size_t)]),
+    "ipl_copy_pages": (
+        ctypes.c_int,
+        [ctypes.POINTER(PageCaches), ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p],
+    ),
+    "ipl_reserve_pages": (
+        ctypes.c_int,
+        [
+            ctypes.POINTER(PagePool),
+            ctypes.c_void_p,
+            ctypes.c_void_p,
+            ctypes.c_int64,
+            ctypes.c_void_p,
+            ctypes.c_size_t,
+            ctypes.c_void_p,
+            ctypes.c_void_p,
+        ],
+    ),
+    "ipl_fork_sequences": (
+        ctypes.c_int,
+        [
+            ctypes.POINTER(PageCaches),
+            ctypes.POINTER(PagePool),
+            ctypes.c_void_p,
+            ctypes.c_void_p,
+            ctypes.c_int64,
+            ctypes.c_void_p,
+            ctypes.c_size_t,
+            ctypes.c_void_p,
+            ctypes.c_void_p,
+        ],
+    ),
+    "ipl_release_sequences": (
+        ctypes.c_int,
+        [ctypes.POINTER(PagePool), ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p],
+    ),
+    "ipl_compact_pages": (
+        ctypes.c_int,
+        [
+            ctypes.POINTER(PageCaches),
+            ctypes.POINTER(PagePool),
+            ctypes.c_void_p,
+            ctypes.c_void_p,
+            ctypes.c_void_p,
+            ctypes.c_void_p,
+            ctypes.c_size_t,
+            ctypes.c_void_p,
+        ],
     ),
     "ipl_last_error": (ctypes.c_char_p, []),
     "ipl_status_string": (ctypes.c_char_p, [ctypes.c_int]),
@@ -175,6 +288,103 @@ def silu_and_mul_packed(
     _check(
         library().ipl_silu_and_mul_packed_bf16(
             output_ptr, input_ptr, rows, intermediate_size, stream
+        )
+    )
+
+
+def rotary_embedding(args: RotaryArgs, stream: int = 0) -> None:
+    _check(library().ipl_rotary_embedding_bf16(ctypes.byref(args), stream))
+
+
+def rotary_embedding_cache(args: RotaryArgs, stream: int = 0) -> None:
+    _check(library().ipl_rotary_embedding_cache_bf16(ctypes.byref(args), stream))
+
+
+def paged_attention(args: PagedAttentionArgs, stream: int = 0) -> None:
+    _check(library().ipl_paged_attention_bf16(ctypes.byref(args), stream))
+
+
+def paged_attention_workspace(args: PagedAttentionArgs) -> int:
+    size = ctypes.c_size_t(0)
+    _check(library().ipl_paged_attention_workspace(ctypes.byref(args), ctypes.byref(size)))
+    return size.value
+
+
+def paged_attention_plan(args: PagedAttentionArgs) -> str:
+    return library().ipl_paged_attention_plan(ctypes.byref(args)).decode()
+
+
+def pages_workspace(num_pages: int, count: int) -> int:
+    size = ctypes.c_size_t(0)
+    _check(library().ipl_pages_workspace(num_pages, count, ctypes.byref(size)))
+    return size.value
+
+
+def page_caches(
+    bases: list[int], page_stride_bytes: int, page_bytes: int, token_bytes: int
+) -> PageCaches:
+    """The caches of a call; keeps the host array of bases alive."""
+    return PageCaches((ctypes.c_void_p * len(bases))(*bases), len(bases), page_stride_bytes, page_bytes, token_bytes)
+
+
+def copy_pages(caches: PageCaches, num_pages: int, pairs_ptr: int, count: int, stream: int = 0) -> None:
+    _check(library().ipl_copy_pages(ctypes.byref(caches), num_pages, pairs_ptr, count, stream))
+
+
+def reserve_pages(
+    pool: PagePool,
+    rows_ptr: int,
+    new_lens_ptr: int,
+    count: int,
+    workspace_ptr: int,
+    workspace_bytes: int,
+    status_ptr: int,
+    stream: int = 0,
+) -> None:
+    _check(
+        library().ipl_reserve_pages(
+            ctypes.byref(pool), rows_ptr, new_lens_ptr, count, workspace_ptr, workspace_bytes, status_ptr, stream
+        )
+    )
+
+
+def fork_sequences(
+    caches: PageCaches,
+    pool: PagePool,
+    parents_ptr: int,
+    children_ptr: int,
+    count: int,
+    workspace_ptr: int,
+    workspace_bytes: int,
+    status_ptr: int,
+    stream: int = 0,
+) -> None:
+    _check(
+        library().ipl_fork_sequences(
+            ctypes.byref(caches), ctypes.byref(pool), parents_ptr, children_ptr, count, workspace_ptr,
+            workspace_bytes, status_ptr, stream
+        )
+    )
+
+
+def release_sequences(pool: PagePool, rows_ptr: int, count: int, stream: int = 0) -> None:
+    _check(library().ipl_release_sequences(ctypes.byref(pool), rows_ptr, count, stream))
+
+
+def compact_pages(
+    caches: PageCaches,
+    pool: PagePool,
+    new_tables_ptr: int,
+    new_ref_counts_ptr: int,
+    live_ptr: int,
+    workspace_ptr: int,
+    workspace_bytes: int,
+    stream: int = 0,
+) -> None:
+    _check(
+        library().ipl_compact_pages(
+            ctypes.byref(caches), ctypes.byref(pool), new_tables_ptr, new_ref_counts_ptr, live_ptr, workspace_ptr,
+            workspace_bytes, stream
         )
     )
 

@@ -1,7 +1,8 @@
 """Op loader and Python wrappers.
 
 Mirrors ``src/inference_performance_lab/kernels/extension.py`` of the reference (load_extension at
-:12-35, wrappers at :38-71): same function names, arguments, in-place behaviour and errors. The
+:12-35, wrappers at :38-71): same function names, arguments, in-place behaviour and errors; the ops
+of the paged KV cache at the end have no counterpart there. The
 difference is the loader: instead of JIT-compiling with ``torch.utils.cpp_extension.load`` into a
 cache directory, it loads the in-tree library built by ``build.py`` (building it first if it is
 missing or stale and nvcc is present). There is no fallback: if the native library cannot be
@@ -118,3 +119,143 @@ def silu_and_mul_packed(x: torch.Tensor) -> torch.Tensor:
     torch.ops.inference_performance_lab.silu_and_mul_packed(output, x)
 
     return output
+
+
+# ---- paged KV cache (not in the reference library) -----------------------------------------------
+
+
+def rotary_embedding(
+    positions: torch.Tensor,
+    query: torch.Tensor,
+    key: torch.Tensor,
+    cos_sin_cache: torch.Tensor,
+    is_neox: bool = True,
+) -> None:
+    """In place: the first ``R`` elements of every head of ``query`` ``[T, heads, D]`` and ``key``
+    ``[T, kv_heads, D]`` turned by the angles of ``positions`` (int64 ``[T]``).
+
+    ``cos_sin_cache`` is float32 ``[positions, R]`` (:func:`rotary_cos_sin_cache`). Pairs are
+    ``(x[i], x[i + R/2])`` with ``is_neox``, else ``(x[2i], x[2i+1])``. Any strides with a contiguous
+    last dimension.
+    """
+    load_extension()
+
+    torch.ops.inference_performance_lab.rotary_embedding(positions, query, key, cos_sin_cache, is_neox)
+
+
+def rotary_embedding_cache(
+    positions: torch.Tensor,
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    cos_sin_cache: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    slot_mapping: torch.Tensor,
+    is_neox: bool = True,
+) -> None:
+    """Rotates ``query`` in place and writes rotated ``key`` and ``value`` to their slots of the caches
+    ``[pages, page_size, kv_heads, D]``: slot ``s`` (int64, negative: none) is row ``s % page_size`` of
+    page ``s // page_size``. ``key`` itself stays as it is."""
+    load_extension()
+
+    torch.ops.inference_performance_lab.rotary_embedding_cache(
+        positions, query, key, value, cos_sin_cache, key_cache, value_cache, slot_mapping, is_neox
+    )
+
+
+def paged_attention(
+    query: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    block_tables: torch.Tensor,
+    query_start_loc: torch.Tensor,
+    seq_lens: torch.Tensor,
+    max_query_len: int,
+    max_seq_len: int,
+    scale: float,
+    window: int = 0,
+) -> torch.Tensor:
+    """Causal attention of new tokens over a paged cache, into a new ``[T, heads, D]`` tensor.
+
+    Sequence ``s`` owns rows ``query_start_loc[s]:query_start_loc[s + 1]`` of ``query`` and has
+    ``seq_lens[s]`` tokens in the cache, those included; its pages are ``block_tables[s]`` (all int32).
+    ``max_query_len`` and ``max_seq_len`` bound the lengths; ``window`` > 0 limits each token to the last
+    ``window`` keys. A token that sees no key gives 0; rows of no sequence are left unwritten.
+    """
+    load_extension()
+
+    output = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    torch.ops.inference_performance_lab.paged_attention(
+        output, query, key_cache, value_cache, block_tables, query_start_loc, seq_lens, max_query_len, max_seq_len,
+        scale, window
+    )
+
+    return output
+
+
+def copy_pages(caches: list[torch.Tensor], pairs: torch.Tensor) -> None:
+    """Copies page ``pairs[i, 0]`` to page ``pairs[i, 1]`` (int32; negative: skipped) in every cache."""
+    load_extension()
+
+    torch.ops.inference_performance_lab.copy_pages(caches, pairs)
+
+
+def reserve_pages(
+    block_tables: torch.Tensor,
+    seq_lens: torch.Tensor,
+    ref_counts: torch.Tensor,
+    rows: torch.Tensor,
+    new_lens: torch.Tensor,
+    page_size: int,
+) -> torch.Tensor:
+    """Gives ``rows[i]`` pages for ``new_lens[i]`` tokens, in place. Returns an int32 ``[1]`` status on
+    the device: 0, the number of free pages lacking, or -1 for an entry out of range; unless it is 0
+    nothing has changed."""
+    load_extension()
+
+    return torch.ops.inference_performance_lab.reserve_pages(
+        block_tables, seq_lens, ref_counts, rows, new_lens, page_size
+    )
+
+
+def fork_sequences(
+    caches: list[torch.Tensor],
+    block_tables: torch.Tensor,
+    seq_lens: torch.Tensor,
+    ref_counts: torch.Tensor,
+    parents: torch.Tensor,
+    children: torch.Tensor,
+) -> torch.Tensor:
+    """Makes the empty row ``children[i]`` a copy of row ``parents[i]``, in place: whole pages are
+    shared, a partly filled last page is copied in every cache. Returns a status as
+    :func:`reserve_pages` does."""
+    load_extension()
+
+    return torch.ops.inference_performance_lab.fork_sequences(
+        caches, block_tables, seq_lens, ref_counts, parents, children
+    )
+
+
+def release_sequences(
+    block_tables: torch.Tensor, seq_lens: torch.Tensor, ref_counts: torch.Tensor, rows: torch.Tensor
+) -> None:
+    """Empties ``rows``, in place: each of their pages loses one reference."""
+    load_extension()
+
+    torch.ops.inference_performance_lab.release_sequences(block_tables, seq_lens, ref_counts, rows)
+
+
+def compact_pages(
+    caches: list[torch.Tensor], block_tables: torch.Tensor, ref_counts: torch.Tensor
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Moves the pages in use to the lowest numbers. Returns the renumbered tables and counts and the
+    number of pages in use (int32 ``[1]``); the old tables stay valid until moved pages are claimed."""
+    load_extension()
+
+    new_tables = torch.empty(block_tables.shape, dtype=block_tables.dtype, device=block_tables.device)
+    new_counts = torch.empty(ref_counts.shape, dtype=ref_counts.dtype, device=ref_counts.device)
+    live = torch.empty(1, dtype=torch.int32, device=block_tables.device)
+    torch.ops.inference_performance_lab.compact_pages(caches, block_tables, ref_counts, new_tables, new_counts, live)
+
+    return new_tables, new_counts, live

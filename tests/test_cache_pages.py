@@ -1,0 +1,276 @@
+"""Pages of a KV cache: reserving, forking, releasing, copying and compacting against plain Python
+bookkeeping and the pages' own bytes; pools without room, invalid entries, refusals."""
+
+from __future__ import annotations
+
+import random
+
+import pytest
+import torch
+
+from cache_reference import Pool
+from inference_performance_lab.kernels import capi, extension
+from parity import require_cuda
+
+gpu = pytest.mark.gpu
+
+
+class Device:
+    """A pool on the device beside the plain one."""
+
+    def __init__(self, rows, width, pages, page_size, layers=2, kv_heads=2, dim=8, seed=0, hnd=False, dtype=torch.bfloat16):
+        self.page = page_size
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        shape = (2 * layers, pages, kv_heads, page_size, dim) if hnd else (2 * layers, pages, page_size, kv_heads, dim)
+        self.store = torch.randint(0, 127, shape, generator=g, device="cuda").to(dtype)
+        self.view = self.store.transpose(2, 3) if hnd else self.store
+        self.caches = list(self.view.unbind(0))
+        self.tables = torch.full((rows, width), -1, dtype=torch.int32, device="cuda")
+        self.lens = torch.zeros(rows, dtype=torch.int32, device="cuda")
+        self.refs = torch.zeros(pages, dtype=torch.int32, device="cuda")
+        self.pool = Pool(self.tables.tolist(), self.lens.tolist(), self.refs.tolist(), page_size)
+
+    def ints(self, values):
+        return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+    def same(self):
+        assert self.tables.tolist() == self.pool.tables
+        assert self.lens.tolist() == self.pool.lens
+        assert self.refs.tolist() == self.pool.refs
+        assert capi.device_fault_flags(0) == 0
+
+    def reserve(self, rows, lens):
+        status = extension.reserve_pages(self.tables, self.lens, self.refs, self.ints(rows), self.ints(lens), self.page)
+        assert status.tolist() == [self.pool.reserve(rows, lens)]
+        self.same()
+
+    def release(self, rows):
+        extension.release_sequences(self.tables, self.lens, self.refs, self.ints(rows))
+        self.pool.release(rows)
+        self.same()
+
+    def fork(self, parents, children):
+        before = self.view.clone()
+        status = extension.fork_sequences(self.caches, self.tables, self.lens, self.refs, self.ints(parents), self.ints(children))
+        lacking, copies = self.pool.fork(parents, children)
+        assert status.tolist() == [lacking]
+        self.same()
+        for source, target, tokens in copies:
+            assert torch.equal(self.view[:, target, :tokens], before[:, source, :tokens])
+        kept = torch.ones(before.shape[1], dtype=torch.bool, device="cuda")
+        kept[[c[1] for c in copies]] = False
+        assert torch.equal(self.view[:, kept], before[:, kept])
+
+    def compact(self):
+        before = self.view.clone()
+        old = self.tables.clone(), self.refs.clone()
+        tables, refs, live = extension.compact_pages(self.caches, self.tables, self.refs)
+        want_tables, want_refs, want_live, moves = self.pool.compact()
+        assert tables.tolist() == want_tables and refs.tolist() == want_refs and live.tolist() == [want_live]
+        assert torch.equal(self.tables, old[0]) and torch.equal(self.refs, old[1])
+        for source, target in moves:
+            before[:, target] = before[:, source]
+        assert torch.equal(self.view, before)
+        self.tables, self.refs = tables, refs
+        self.pool.tables, self.pool.refs = want_tables, want_refs
+        self.same()
+
+
+@gpu
+@pytest.mark.parametrize("page_size, pages, rows, hnd, dim", [(16, 200, 12, False, 8), (1, 90, 9, False, 8), (48, 64, 20, True, 16),
+                                                              (7, 3000, 40, False, 24), (16, 40, 10, True, 8)])
+def test_random_traffic(page_size, pages, rows, hnd, dim):
+    """A random mix of every call; the pool often has no room."""
+    require_cuda()
+    d = Device(rows, 40, pages, page_size, dim=dim, hnd=hnd, seed=page_size)
+    rng = random.Random(page_size)
+    for _ in range(60):
+        kind = rng.choice(["reserve", "reserve", "fork", "release", "compact"])
+        some = rng.sample(range(rows), rng.randint(0, rows // 2))
+        if kind == "reserve":
+            d.reserve(some, [rng.randint(0, 40 * page_size) if rng.random() < 0.3 else min(40 * page_size, d.pool.lens[r] + rng.randint(0, 30))
+                             for r in some])
+        elif kind == "release":
+            d.release(some)
+        elif kind == "fork":
+            empty = [r for r in range(rows) if d.pool.lens[r] == 0 and not any(p >= 0 for p in d.pool.tables[r])]
+            children = rng.sample(empty, rng.randint(0, len(empty)))
+            held = [r for r in range(rows) if r not in children] or [0]
+            d.fork([rng.choice(held) for _ in children], children)
+        else:
+            d.compact()
+
+
+@gpu
+def test_more_rows_and_pages_than_threads():
+    require_cuda()
+    d = Device(3000, 3, 5000, 4, layers=1, kv_heads=1)
+    d.reserve(list(range(0, 2500)), [(i * 7) % 9 for i in range(2500)])
+    d.release(list(range(0, 2500, 3)))
+    parents = [i for i in range(1, 1500, 3)]
+    d.fork(parents, list(range(2500, 2500 + len(parents))))
+    d.compact()
+    d.reserve(list(range(2999, -1, -1)), [12] * 3000)  # lacks pages: nothing changes
+
+
+@gpu
+def test_many_caches_take_several_launches():
+    require_cuda()
+    d = Device(4, 4, 12, 8, layers=70)
+    d.reserve([0], [19])
+    d.fork([0, 0], [1, 3])
+    d.release([0])
+    d.compact()
+
+
+@gpu
+def test_invalid_entries_change_nothing():
+    require_cuda()
+    d = Device(6, 4, 30, 16)
+    d.reserve([0, 1], [20, 40])
+    for rows, lens in (([6], [1]), ([-1], [1]), ([2], [65]), ([2], [-1]), ([3, 2, 3], [1, 1, 1])):
+        status = extension.reserve_pages(d.tables, d.lens, d.refs, d.ints(rows), d.ints(lens), 16)
+        assert status.tolist() == [-1]
+        d.same()
+    for parents, children in (([0], [6]), ([7], [2]), ([0], [1]), ([0, 1], [2, 2]), ([-1], [2])):
+        status = extension.fork_sequences(d.caches, d.tables, d.lens, d.refs, d.ints(parents), d.ints(children))
+        assert status.tolist() == [-1]
+        d.same()
+    d.fork([0, 3], [3, 4])  # a parent that is itself an empty child
+
+
+@gpu
+def test_a_row_released_twice_and_out_of_range():
+    require_cuda()
+    capi.clear_device_fault_flags(0)
+    d = Device(4, 8, 20, 4)
+    d.reserve([0, 1], [9, 30])
+    extension.release_sequences(d.tables, d.lens, d.refs, d.ints([1, 1, 1]))
+    d.pool.release([1])
+    d.same()
+    extension.release_sequences(d.tables, d.lens, d.refs, d.ints([4, -1]))
+    assert capi.device_fault_flags(0) == 8
+    capi.clear_device_fault_flags(0)
+    d.same()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn, torch.float32])
+def test_copy_pages(dtype):
+    require_cuda()
+    store = torch.arange(3 * 20 * 16 * 2 * 16, device="cuda").remainder(97).float().to(dtype).view(3, 20, 16, 2, 16)
+    expected = store.clone()
+    pairs = [(0, 5), (0, 7), (-1, 3), (4, -1), (19, 2)]
+    extension.copy_pages(list(store.unbind(0)), torch.tensor(pairs, dtype=torch.int32, device="cuda"))
+    for source, target in pairs:
+        if min(source, target) >= 0:
+            expected.view(torch.uint8)[:, target] = expected.view(torch.uint8)[:, source]
+    assert torch.equal(store.view(torch.uint8), expected.view(torch.uint8))
+    assert capi.device_fault_flags(0) == 0
+    extension.copy_pages(list(store.unbind(0)), torch.tensor([(0, 20), (2**30, 0)], dtype=torch.int32, device="cuda"))
+    assert capi.device_fault_flags(0) == 8
+    capi.clear_device_fault_flags(0)
+    assert torch.equal(store.view(torch.uint8), expected.view(torch.uint8))
+    extension.copy_pages(list(store.unbind(0)), torch.empty(0, 2, dtype=torch.int32, device="cuda"))
+
+
+@gpu
+def test_interleaved_caches_and_long_offsets():
+    """Layers interleaved page by page in one buffer of more than 2^32 bytes."""
+    require_cuda()
+    pages, layers = 66000, 4
+    store = torch.empty(pages, layers, 16, 2, 256, dtype=torch.bfloat16, device="cuda")
+    store[-3:].copy_(torch.randn_like(store[-3:]))
+    expected = store[-1].clone()
+    extension.copy_pages(list(store.unbind(1)), torch.tensor([[pages - 1, 1], [pages - 1, pages - 3]], dtype=torch.int32, device="cuda"))
+    assert torch.equal(store[1], expected) and torch.equal(store[-3], expected)
+
+
+@gpu
+def test_graph_replay():
+    require_cuda()
+    d = Device(8, 8, 40, 4)
+    d.reserve([0, 1], [9, 14])
+    parents, children = d.ints([0, 1]), d.ints([2, 3])
+    extension.fork_sequences(d.caches, d.tables, d.lens, d.refs, parents, children)
+    extension.release_sequences(d.tables, d.lens, d.refs, children)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        extension.release_sequences(d.tables, d.lens, d.refs, children)
+        status = extension.fork_sequences(d.caches, d.tables, d.lens, d.refs, parents, children)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert status.tolist() == [0]
+        d.pool.release([2, 3])
+        d.pool.fork([0, 1], [2, 3])
+        d.same()
+
+
+@gpu
+def test_refusals():
+    require_cuda()
+    d = Device(4, 8, 20, 4)
+    rows = d.ints([0])
+    with pytest.raises(RuntimeError, match="rows and new_lens must have the same length"):
+        extension.reserve_pages(d.tables, d.lens, d.refs, rows, d.ints([1, 2]), 4)
+    with pytest.raises(RuntimeError, match="page size positive"):
+        extension.reserve_pages(d.tables, d.lens, d.refs, rows, rows, 0)
+    with pytest.raises(RuntimeError, match="block_tables must be int32"):
+        extension.release_sequences(d.tables.long(), d.lens, d.refs, rows)
+    with pytest.raises(RuntimeError, match="a length for each row"):
+        extension.release_sequences(d.tables, d.lens[:3], d.refs, rows)
+    with pytest.raises(RuntimeError, match="same device"):
+        extension.release_sequences(d.tables, d.lens, d.refs, rows.cpu())
+    with pytest.raises(RuntimeError, match="a count for each page"):
+        extension.fork_sequences(d.caches, d.tables, d.lens, d.refs[:19], rows, rows)
+    with pytest.raises(RuntimeError, match="same type, shape and strides"):
+        extension.fork_sequences([d.caches[0], d.caches[1].float()], d.tables, d.lens, d.refs, rows, rows)
+    with pytest.raises(RuntimeError, match="must not be empty"):
+        extension.compact_pages([], d.tables, d.refs)
+    with pytest.raises(RuntimeError, match="must be contiguous, tokens or heads"):
+        extension.copy_pages([d.caches[0][..., :4]], d.ints([[0, 1]]))
+    with pytest.raises(RuntimeError, match="16-byte"):
+        extension.copy_pages([torch.zeros(4, 1, 3, device="cuda")], d.ints([[0, 1]]))
+    with pytest.raises(RuntimeError, match="pairs must be contiguous int32"):
+        extension.copy_pages(d.caches, d.ints([0, 1]))
+
+
+BASE = 0x7F0000000000
+
+
+def pool(**changes):
+    a = dict(block_tables=BASE, seq_lens=BASE, ref_counts=BASE, num_rows=4, width=8, table_stride=8, num_pages=20, page_size=16)
+    a.update(changes)
+    return capi.PagePool(**a)
+
+
+def caches(stride=4096, size=4096, token=256, bases=(BASE, BASE + 4096)):
+    return capi.page_caches(list(bases), stride, size, token)
+
+
+@pytest.mark.parametrize("call, status, message", [
+    (lambda: capi.reserve_pages(pool(num_rows=-1), BASE, BASE, 1, BASE, 1 << 20, BASE), capi.IPL_ERROR_INVALID_VALUE, "non-negative"),
+    (lambda: capi.reserve_pages(pool(num_pages=2**31), BASE, BASE, 1, BASE, 1 << 20, BASE), capi.IPL_ERROR_TOO_LARGE, "too large"),
+    (lambda: capi.reserve_pages(pool(), 0, BASE, 1, BASE, 1 << 20, BASE), capi.IPL_ERROR_INVALID_VALUE, "non-null"),
+    (lambda: capi.reserve_pages(pool(), BASE, BASE, 1, BASE, 16, BASE), capi.IPL_ERROR_INVALID_VALUE, "workspace is too small"),
+    (lambda: capi.reserve_pages(pool(), BASE, BASE, 1, BASE, 1 << 20, 0), capi.IPL_ERROR_INVALID_VALUE, "status must be non-null"),
+    (lambda: capi.release_sequences(pool(ref_counts=0), BASE, 1), capi.IPL_ERROR_INVALID_VALUE, "non-null"),
+    (lambda: capi.release_sequences(pool(seq_lens=BASE + 2), BASE, 1), capi.IPL_ERROR_INVALID_VALUE, "4-byte aligned"),
+    (lambda: capi.copy_pages(caches(stride=2048), 20, BASE, 1), capi.IPL_ERROR_INVALID_VALUE, "must not overlap"),
+    (lambda: capi.copy_pages(caches(size=4088), 20, BASE, 1), capi.IPL_ERROR_MISALIGNED, "16"),
+    (lambda: capi.copy_pages(caches(bases=(BASE + 8,)), 20, BASE, 1), capi.IPL_ERROR_MISALIGNED, "16"),
+    (lambda: capi.fork_sequences(caches(token=128), pool(), BASE, BASE, 1, BASE, 1 << 20, BASE), capi.IPL_ERROR_INVALID_VALUE,
+     "page_size tokens"),
+    (lambda: capi.compact_pages(caches(), pool(), BASE, BASE + 64, BASE, BASE, 1 << 20), capi.IPL_ERROR_INVALID_VALUE, "must not alias"),
+])
+def test_argument_errors(call, status, message):
+    with pytest.raises(capi.IplError, match=message) as info:
+        call()
+    assert info.value.status == status
+
+
+def test_workspace_and_empty_calls():
+    assert capi.pages_workspace(100, 7) >= 4 * (100 + 14)
+    capi.copy_pages(caches(), 20, 0, 0)
+    capi.release_sequences(pool(), 0, 0)

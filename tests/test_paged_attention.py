@@ -1,0 +1,356 @@
+"""Attention over a paged cache against the formula in 64 bits, where it can go wrong: lengths of zero
+and one, rows that see nothing, windows, pages that end inside a tile, garbage (NaN, infinities) in
+unused pages, rows past a length and table entries past a sequence's pages, odd group and head sizes,
+strides, long offsets, streams and graphs; and its refusals."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from cache_reference import attention, attention_bound
+from inference_performance_lab.kernels import capi, extension
+from parity import require_cuda
+
+gpu = pytest.mark.gpu
+
+
+def make(new, total, heads=28, kv_heads=4, dim=128, page=16, seed=0, spare=3, hnd=False, fill=float("nan"), width=None):
+    """Inputs whose every unused place holds `fill`, and whose unused table entries are no page numbers."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    counts = [-(-t // page) for t in total]
+    pages = sum(counts) + spare
+    shape = (2, pages, kv_heads, page, dim) if hnd else (2, pages, page, kv_heads, dim)
+    store = torch.full(shape, fill, dtype=torch.bfloat16, device="cuda")
+    kc, vc = (store.transpose(2, 3) if hnd else store).unbind(0)
+    width = width or max(counts + [1]) + 2
+    tables = torch.full((len(new), width), 2**30, dtype=torch.int32, device="cuda")
+    order = torch.randperm(pages, generator=g, device="cuda").int()
+    at = 0
+    for s, (c, t) in enumerate(zip(counts, total)):
+        mine = order[at : at + c]
+        at += c
+        tables[s, :c] = mine
+        for j, p in enumerate(mine.tolist()):
+            rows = min(page, t - j * page)
+            for cache in (kc, vc):
+                cache[p, :rows] = torch.randn(rows, kv_heads, dim, generator=g, device="cuda").to(torch.bfloat16)
+    q = (torch.randn(sum(new), heads, dim, generator=g, device="cuda") * 1.5).to(torch.bfloat16)
+    starts = torch.tensor([sum(new[:i]) for i in range(len(new) + 1)], dtype=torch.int32, device="cuda")
+    lens = torch.tensor(total, dtype=torch.int32, device="cuda")
+    return q, kc, vc, tables, starts, lens
+
+
+def call(inputs, new, total, window=0, scale=None):
+    q = inputs[0]
+    scale = scale or q.shape[2] ** -0.5
+    return extension.paged_attention(*inputs, max(new), max(total), scale, window), scale
+
+
+def check(inputs, new, total, window=0, scale=None):
+    got, scale = call(inputs, new, total, window, scale)
+    expected, size = attention(*inputs, scale, window)
+    error = (got.double() - expected).abs()
+    assert (error <= attention_bound(expected, size)).all(), (error - attention_bound(expected, size)).max()
+    assert capi.device_fault_flags(0) == 0
+    return got
+
+
+SINGLE = [
+    # new, total (per sequence), heads, kv_heads, dim, page, window
+    ([1], [1], 28, 4, 128, 16, 0),
+    ([1], [17], 28, 4, 128, 16, 0),
+    ([1] * 5, [1, 16, 300, 2, 129], 28, 4, 128, 16, 0),
+    ([1] * 3, [1027, 0, 513], 28, 4, 128, 16, 0),
+    ([1] * 4, [40, 64, 65, 700], 32, 8, 64, 32, 0),
+    ([1] * 3, [900, 31, 128], 16, 16, 64, 16, 100),
+    ([1] * 2, [260, 77], 16, 1, 96, 48, 0),
+    ([1] * 2, [260, 77], 40, 8, 80, 128, 33),
+    ([1], [5000], 4, 4, 128, 64, 1),
+    ([1, 1], [333, 90], 64, 1, 128, 16, 0),
+    ([1, 1], [70, 9], 6, 3, 256, 16, 0),
+    ([1, 1], [70, 9], 4, 2, 20, 7, 12),
+    ([1] * 3, [4097, 4096, 4095], 8, 1, 128, 256, 0),
+]
+CHUNKS = [
+    ([2], [2], 28, 4, 128, 16, 0),
+    ([17, 1, 0, 64], [40, 300, 12, 64], 28, 4, 128, 16, 0),
+    ([129], [129], 4, 4, 128, 16, 0),
+    ([200, 3], [1000, 600], 28, 4, 128, 64, 0),
+    ([300], [301], 32, 8, 64, 32, 70),
+    ([130, 40], [700, 41], 16, 1, 96, 48, 0),
+    ([50], [50], 40, 8, 80, 128, 7),
+    ([511, 64], [511, 900], 8, 2, 128, 128, 256),
+    ([9, 30], [70, 30], 6, 3, 256, 16, 0),
+    ([9, 30], [70, 30], 4, 2, 20, 7, 12),
+    ([37], [2300], 12, 2, 64, 16, 1000),
+    ([260], [260], 16, 16, 8, 16, 0),
+    ([5, 4, 3], [200, 190, 4], 28, 4, 128, 16, 0),
+    ([1, 150, 1, 33], [2000, 150, 3, 1500], 28, 4, 128, 16, 0),
+    ([90], [5000], 3, 1, 128, 32, 0),
+]
+
+
+@gpu
+@pytest.mark.parametrize("new, total, heads, kv_heads, dim, page, window", SINGLE + CHUNKS)
+def test_against_the_formula(new, total, heads, kv_heads, dim, page, window):
+    require_cuda()
+    inputs = make(new, total, heads, kv_heads, dim, page, seed=len(new) + dim)
+    check(inputs, new, total, window)
+
+
+@gpu
+@pytest.mark.parametrize("fill", [float("inf"), float("-inf"), 3e38])
+def test_unused_places_hold_infinities(fill):
+    require_cuda()
+    for new, total in (([1, 1], [37, 5]), ([20, 150], [37, 333])):
+        check(make(new, total, fill=fill), new, total)
+
+
+@gpu
+def test_rows_that_see_nothing_are_zero():
+    """More new tokens than the cache holds: the first ones sit before position 0."""
+    require_cuda()
+    for new, total in (([4], [2]), ([150], [20]), ([1], [0]), ([140], [0]), ([3, 1], [1, 5])):
+        got = check(make(new, total), new, total)
+        assert (got[: new[0] - total[0]] == 0).all()
+
+
+@gpu
+def test_heads_before_tokens_and_views():
+    """A cache with heads before tokens, q a view of a projection, output of another layout."""
+    require_cuda()
+    for new, total in (([1] * 4, [65, 2, 130, 700]), ([70, 200], [100, 500])):
+        q, kc, vc, tables, starts, lens = make(new, total, hnd=True)
+        wide = torch.randn(q.shape[0], 36, 128, device="cuda").to(torch.bfloat16)
+        wide[:, 3:31] = q
+        q = wide[:, 3:31]
+        check((q, kc, vc, tables, starts, lens), new, total)
+        out = torch.zeros(28, q.shape[0], 128, device="cuda", dtype=torch.bfloat16).transpose(0, 1)
+        torch.ops.inference_performance_lab.paged_attention(out, q, kc, vc, tables, starts, lens, max(new), max(total), 0.1, 0)
+        expected, size = attention(q, kc, vc, tables, starts, lens, 0.1)
+        assert ((out.double() - expected).abs() <= attention_bound(expected, size)).all()
+
+
+@gpu
+@pytest.mark.parametrize("offset", [1, 4])
+def test_pointers_off_16_bytes(offset):
+    require_cuda()
+    for new, total in (([1, 1], [65, 200]), ([70], [100])):
+        q, kc, vc, tables, starts, lens = make(new, total, heads=8, kv_heads=2, dim=64)
+
+        def moved(t):
+            flat = torch.empty(t.numel() + offset, dtype=t.dtype, device="cuda")[offset:]
+            return flat.copy_(t.reshape(-1)).view(t.shape)
+
+        check((moved(q), kc, vc, tables, starts, lens), new, total)
+        check((q, moved(kc), moved(vc), tables, starts, lens), new, total)
+
+
+@gpu
+def test_peaked_and_shifted_scores():
+    """Scores that grow along the keys by far more than an exponent's range, large equal offsets, and a
+    single key that takes all the weight."""
+    require_cuda()
+    new, total = [1, 140], [900, 900]
+    q, kc, vc, tables, starts, lens = make(new, total, heads=8, kv_heads=2)
+    q.fill_(1.0)
+    for s in range(2):
+        for j, p in enumerate(tables[s, : -(-900 // 16)].tolist()):
+            rows = min(16, 900 - j * 16)
+            position = (torch.arange(rows, device="cuda") + j * 16).to(torch.bfloat16)
+            kc[p, :rows] = (position / 64.0)[:, None, None]
+    check((q, kc, vc, tables, starts, lens), new, total, scale=1.0)  # rises by 2 a key
+    for s in range(2):
+        for j, p in enumerate(tables[s, : -(-900 // 16)].tolist()):
+            rows = min(16, 900 - j * 16)
+            position = (torch.arange(rows, device="cuda") + j * 16).to(torch.bfloat16)
+            kc[p, :rows] = (-position / 64.0 - 100.0)[:, None, None]
+    check((q, kc, vc, tables, starts, lens), new, total, scale=1.0)  # falls from -12800
+
+
+@gpu
+def test_keys_at_masked_positions_never_matter():
+    """NaN and infinite keys ahead of a token leave it as it is."""
+    require_cuda()
+    new, total = [40], [100]
+    inputs = make(new, total)
+    q, kc, vc, tables, starts, lens = inputs
+    expected = check(inputs, new, total)
+    for bad in (float("nan"), float("inf"), float("-inf")):
+        page, row = int(tables[0, 6]), 3  # position 99, seen by the last token alone
+        kc[page, row] = bad
+        got, _ = call(inputs, new, total)
+        assert torch.equal(got[:39], expected[:39])
+
+
+@gpu
+def test_pages_outside_the_cache_contribute_nothing():
+    require_cuda()
+    capi.clear_device_fault_flags(0)
+    new, total = [1, 20], [40, 40]
+    q, kc, vc, tables, starts, lens = make(new, total, heads=4, kv_heads=2, dim=64)
+    reference = [t.clone() for t in (kc, vc)]
+    tables[:, 1] = torch.tensor([-5, 2**31 - 1], dtype=torch.int32, device="cuda")
+    got, scale = call((q, kc, vc, tables, starts, lens), new, total)
+    assert capi.device_fault_flags(0) == 8
+    capi.clear_device_fault_flags(0)
+    # The formula without positions 16 to 31.
+    for s in range(2):
+        pages = tables[s, [0, 2]].long()
+        keys = torch.cat([reference[0][pages[0]], reference[0][pages[1], :8]]).double()
+        values = torch.cat([reference[1][pages[0]], reference[1][pages[1], :8]]).double()
+        position = torch.cat([torch.arange(16), torch.arange(32, 40)]).cuda()
+        for t in range(int(starts[s]), int(starts[s + 1])):
+            at = 40 - new[s] + t - int(starts[s])
+            for h in range(4):
+                logits = (keys[:, h // 2] @ q[t, h].double()) * scale
+                w = torch.softmax(logits.masked_fill(position > at, -torch.inf), 0)
+                want, size = w @ values[:, h // 2], w @ values[:, h // 2].abs()
+                assert ((got[t, h].double() - want).abs() <= attention_bound(want, size)).all()
+
+
+@gpu
+def test_lengths_past_the_bounds_given():
+    """max_query_len and max_seq_len only choose kernels: longer sequences come out right."""
+    require_cuda()
+    new, total = [1, 60, 1], [700, 500, 90]
+    inputs = make(new, total)
+    expected, size = attention(*inputs, 0.125)
+    for most_new, most in ((1, 1), (1, 700), (60, 32), (2, 2), (4096, 100000)):
+        got = extension.paged_attention(*inputs, most_new, most, 0.125)
+        assert ((got.double() - expected).abs() <= attention_bound(expected, size)).all(), (most_new, most)
+
+
+@gpu
+def test_padding_rows_are_not_written():
+    require_cuda()
+    for new, total in (([1, 1], [33, 40]), ([30, 20], [33, 400])):
+        q, kc, vc, tables, starts, lens = make(new, total)
+        padded = torch.cat([q, q.new_full((9, 28, 128), float("nan"))])
+        out = torch.full_like(padded, 7.0)
+        torch.ops.inference_performance_lab.paged_attention(out, padded, kc, vc, tables, starts, lens, max(new), max(total), 0.1, 0)
+        expected, size = attention(q, kc, vc, tables, starts, lens, 0.1)
+        assert ((out[:-9].double() - expected).abs() <= attention_bound(expected, size)).all()
+        assert (out[-9:] == 7.0).all()
+
+
+@gpu
+def test_offsets_past_32_bits():
+    """A cache of more than 2^31 elements, a sequence in its last pages."""
+    require_cuda()
+    page, kv_heads, dim = 16, 4, 128
+    pages = 2**31 // (page * kv_heads * dim) + 40
+    kc = torch.empty(pages, page, kv_heads, dim, dtype=torch.bfloat16, device="cuda")
+    vc = torch.empty_like(kc)
+    kc[-40:].normal_()
+    vc[-40:].normal_()
+    tables = torch.arange(pages - 40, pages, dtype=torch.int32, device="cuda").flip(0)[None].contiguous()
+    lens = torch.tensor([639], dtype=torch.int32, device="cuda")
+    for n in (1, 100):
+        q = torch.randn(n, 28, dim, device="cuda").to(torch.bfloat16)
+        starts = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+        check((q, kc, vc, tables, starts, lens), [n], [639])
+
+
+@gpu
+def test_repeatable_on_other_streams_and_in_graphs():
+    require_cuda()
+    for new, total in (([1] * 3, [5000, 31, 700]), ([1, 90], [3000, 2000])):
+        inputs = make(new, total)
+        expected = check(inputs, new, total)
+        torch.cuda.synchronize()
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            again = [call(inputs, new, total)[0] for _ in range(3)]
+        stream.synchronize()
+        assert all(torch.equal(a, expected) for a in again)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured, _ = call(inputs, new, total)
+        inputs[0].neg_()
+        graph.replay()
+        torch.cuda.synchronize()
+        negated = captured.clone()
+        assert torch.equal(negated, call(inputs, new, total)[0])
+        inputs[0].neg_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(captured, expected)
+
+
+@gpu
+def test_nothing_to_do():
+    require_cuda()
+    q, kc, vc, tables, starts, lens = make([1], [5])
+    assert extension.paged_attention(q[:0], kc, vc, tables, starts * 0, lens, 0, 5, 0.1).shape == (0, 28, 128)
+    none = extension.paged_attention(q, kc, vc, tables[:0], starts[:1], lens[:0], 0, 0, 0.1)
+    assert none.shape == q.shape
+
+
+@gpu
+def test_refusals():
+    require_cuda()
+    q, kc, vc, tables, starts, lens = make([1, 2], [5, 9], heads=4, kv_heads=2, dim=64)
+
+    def refused(message, **changes):
+        a = dict(query=q, key_cache=kc, value_cache=vc, block_tables=tables, query_start_loc=starts, seq_lens=lens,
+                 max_query_len=2, max_seq_len=9, scale=0.1, window=0)
+        a.update(changes)
+        with pytest.raises(RuntimeError, match=message):
+            extension.paged_attention(**a)
+
+    refused("query must be bfloat16", query=q.half())
+    refused("key_cache must be bfloat16", key_cache=kc.float())
+    refused("identical shapes", value_cache=vc[1:])
+    refused("same head size", query=q[..., :32])
+    refused("multiple of the number of key heads", query=q[:, :3])
+    refused("same sequences", seq_lens=lens[:1])
+    refused("same sequences", query_start_loc=starts[:2])
+    refused("block_tables must be int32", block_tables=tables.long())
+    refused("seq_lens must be contiguous int32", seq_lens=lens.long())
+    refused("same device", seq_lens=lens.cpu())
+    refused("scale must be positive", scale=0.0)
+    refused("scale must be positive", scale=float("nan"))
+    refused("non-negative", window=-1)
+    refused("non-negative", max_query_len=-1)
+
+
+def attention_args(**changes):
+    base = 0x7F0000000000
+    a = dict(output=base, query=base, key_cache=base, value_cache=base, block_tables=base, query_start_loc=base, seq_lens=base,
+             num_tokens=4, num_seqs=4, num_heads=28, num_kv_heads=4, head_size=128, num_pages=100, page_size=16, table_width=64,
+             table_stride=64, output_token_stride=3584, output_head_stride=128, query_token_stride=3584,
+             query_head_stride=128, key_cache_page_stride=8192, key_cache_token_stride=512, key_cache_head_stride=128,
+             value_cache_page_stride=8192, value_cache_token_stride=512, value_cache_head_stride=128, max_query_len=1,
+             max_seq_len=1024, window=0, scale=0.088, workspace=0, workspace_bytes=0)
+    a.update(changes)
+    return capi.PagedAttentionArgs(**a)
+
+
+@pytest.mark.parametrize("changes, status, message", [
+    (dict(num_tokens=-1), capi.IPL_ERROR_INVALID_VALUE, "non-negative"),
+    (dict(num_heads=0), capi.IPL_ERROR_INVALID_VALUE, "must be positive"),
+    (dict(page_size=0), capi.IPL_ERROR_INVALID_VALUE, "must be positive"),
+    (dict(num_heads=30), capi.IPL_ERROR_INVALID_VALUE, "multiple of the number of key heads"),
+    (dict(window=-1), capi.IPL_ERROR_INVALID_VALUE, "non-negative"),
+    (dict(scale=-1.0), capi.IPL_ERROR_INVALID_VALUE, "scale must be positive"),
+    (dict(head_size=264), capi.IPL_ERROR_TOO_LARGE, "at most 256"),
+    (dict(num_tokens=2**31), capi.IPL_ERROR_TOO_LARGE, "too large"),
+    (dict(key_cache=0), capi.IPL_ERROR_INVALID_VALUE, "non-null"),
+    (dict(query=3), capi.IPL_ERROR_INVALID_VALUE, "2-byte aligned"),
+    (dict(seq_lens=2), capi.IPL_ERROR_INVALID_VALUE, "4-byte aligned"),
+])
+def test_argument_errors(changes, status, message):
+    with pytest.raises(capi.IplError, match=message) as info:
+        capi.paged_attention(attention_args(**changes))
+    assert info.value.status == status
+    assert capi.paged_attention_plan(attention_args(**changes)) == "invalid"
+    with pytest.raises(capi.IplError, match=message):
+        capi.paged_attention_workspace(attention_args(**changes))
+
+
+def test_no_tokens_needs_no_device():
+    capi.paged_attention(attention_args(num_tokens=0))
+    assert capi.paged_attention_plan(attention_args(num_tokens=0)) == "none"
+    assert capi.paged_attention_workspace(attention_args(num_tokens=0)) == 0
