@@ -221,8 +221,7 @@ IPL_API const char* ipl_paged_attention_plan(const ipl_paged_attention_args* arg
  * per page; a page is free when its count is 0. Claims take the lowest-numbered free pages in order, so
  * equal states give equal results. The caches (K and V of every layer) are opaque: num_caches bases in
  * a host array, page i of each at i * page_stride_bytes, page_bytes long (16-byte multiples; bases
- * 16-byte aligned). token_bytes > 0 says that a page is its tokens one after the other, so that a
- * partly filled one need only be copied as far as it is filled; 0: pages are copied whole.
+ * 16-byte aligned).
  *
  * status receives 0, or the number of free pages lacking, or -1 for an entry out of range (a row, a
  * length, a row given twice, a child that holds tokens); unless it is 0 nothing has changed. The
@@ -232,7 +231,7 @@ IPL_API const char* ipl_paged_attention_plan(const ipl_paged_attention_args* arg
  *   No target may be the source or target of another pair.
  * ipl_reserve_pages: rows[i] gets pages up to new_lens[i] tokens, and that length if it was shorter.
  * ipl_fork_sequences: children[i] (empty) becomes a copy of parents[i]: it shares the whole pages and
- *   gets a page of its own with the tokens of a partly filled last one.
+ *   gets a page of its own with a copy of a partly filled last one.
  * ipl_release_sequences: the pages of rows[i] lose one reference each, the row becomes empty.
  * ipl_compact_pages: the pages in use past the first `live` numbers move, in order, to the free numbers
  *   below. The renumbered tables ([num_rows, width] contiguous) and counts are written beside the old
@@ -247,7 +246,7 @@ typedef struct ipl_page_pool {
 
 typedef struct ipl_page_caches {
     void* const* caches;
-    int64_t num_caches, page_stride_bytes, page_bytes, token_bytes;
+    int64_t num_caches, page_stride_bytes, page_bytes;
 } ipl_page_caches;
 
 IPL_API ipl_status ipl_pages_workspace(int64_t num_pages, int64_t count, size_t* bytes);

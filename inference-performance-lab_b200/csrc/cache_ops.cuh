@@ -241,12 +241,12 @@ ipl_status check_rows(const ipl_page_pool* pool, const void* rows, const void* o
 
 ipl_status check_caches(const ipl_page_caches* c) {
     if (c == nullptr) return fail(IPL_ERROR_INVALID_VALUE, "caches must be non-null");
-    if (c->num_caches < 0 || c->page_bytes < 0 || c->token_bytes < 0 || c->page_stride_bytes < c->page_bytes) {
+    if (c->num_caches < 0 || c->page_bytes < 0 || c->page_stride_bytes < c->page_bytes) {
         return fail(IPL_ERROR_INVALID_VALUE, "sizes of the caches must be non-negative and pages must not overlap");
     }
     if (c->num_caches > 65536) return fail(IPL_ERROR_TOO_LARGE, "too many caches");
     if (c->num_caches > 0 && c->caches == nullptr) return fail(IPL_ERROR_INVALID_VALUE, "caches must be non-null");
-    bool ok = (c->page_bytes | c->token_bytes | c->page_stride_bytes) % 16 == 0;
+    bool ok = (c->page_bytes | c->page_stride_bytes) % 16 == 0;
     for (int64_t i = 0; i < c->num_caches; ++i) {
         if (c->caches[i] == nullptr && c->page_bytes > 0) return fail(IPL_ERROR_INVALID_VALUE, "caches must be non-null");
         ok = ok && aligned(c->caches[i], 16);
@@ -395,9 +395,6 @@ ipl_status ipl_fork_sequences(const ipl_page_caches* caches, const ipl_page_pool
         return fail(IPL_ERROR_INVALID_VALUE, "status must be non-null and 4-byte aligned");
     }
     if (count > INT_MAX / kMaxCachesPerLaunch) return fail(IPL_ERROR_TOO_LARGE, "number of rows is too large");
-    if (caches->token_bytes > 0 && caches->token_bytes * pool->page_size != caches->page_bytes) {
-        return fail(IPL_ERROR_INVALID_VALUE, "a page must hold page_size tokens of token_bytes");
-    }
     const ClaimParams claim = claim_params(*pool, parents, children, nullptr, count, workspace, status);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     st = launch_status(launch(page_claim_kernel<true>, 1, kPlanThreads, 0, s, claim), "page claim");
@@ -416,10 +413,9 @@ ipl_status ipl_fork_sequences(const ipl_page_caches* caches, const ipl_page_pool
         p.status = status;
         p.page_stride = caches->page_stride_bytes;
         p.page_bytes = caches->page_bytes;
-        p.token_bytes = caches->token_bytes;
         if (p.num_caches == 0) {  // tables alone
             p.num_caches = 1;
-            p.page_bytes = p.token_bytes = 0;
+            p.page_bytes = 0;
         }
         const unsigned grid = static_cast<unsigned>(count * p.num_caches);
         st = launch_status(launch(page_fork_kernel, grid, kPageCopyThreads, 0, s, p), "page fork");

@@ -219,11 +219,10 @@ struct ForkParams {
     const int32_t* fresh;
     const int32_t* status;
     int64_t page_stride, page_bytes;
-    int64_t token_bytes;  // of a page whose tokens lie one after the other; 0: copy whole pages
 };
 
 // A CTA for each child and cache: the child takes the parent's whole pages (one more reference each)
-// and a copy of the tokens in its partly filled one.
+// and a copy of its partly filled one.
 __global__ void __launch_bounds__(kPageCopyThreads) page_fork_kernel(const __grid_constant__ ForkParams p) {
     grid_dependency_wait();
     grid_launch_dependents();
@@ -250,7 +249,7 @@ __global__ void __launch_bounds__(kPageCopyThreads) page_fork_kernel(const __gri
         if (threadIdx.x == 0) atomicOr(&g_fault_word, kFaultIndexOutOfRange);
         return;
     }
-    copy_page(p.caches.cache[cache], p.page_stride, last, fresh, p.token_bytes != 0 ? used * p.token_bytes : p.page_bytes);
+    copy_page(p.caches.cache[cache], p.page_stride, last, fresh, p.page_bytes);
 }
 
 // ---- releasing ---------------------------------------------------------------------------------

@@ -306,7 +306,7 @@ struct Caches {
         for (int64_t d = 2; d < c.dim(); ++d) token *= c.size(d);
         args.page_bytes = page_size * token * element;
         args.page_stride_bytes = num_pages > 1 ? c.stride(0) * element : args.page_bytes;
-        bool tokens_follow = page_size == 1 || c.stride(1) == token;
+        const bool tokens_follow = page_size == 1 || c.stride(1) == token;
         bool dense = true;
         int64_t expect = 1;
         for (int64_t d = c.dim() - 1; d >= 2; --d) {
@@ -318,7 +318,6 @@ struct Caches {
                                   (c.size(2) == 1 || c.stride(2) == c.size(3) * page_size);
         STD_TORCH_CHECK(token == 0 || num_pages == 0 || (dense && tokens_follow) || heads_follow,
                         "the pages of a cache must be contiguous, tokens or heads one after the other");
-        args.token_bytes = dense && tokens_follow && token * element % 16 == 0 ? token * element : 0;
     }
 };
 

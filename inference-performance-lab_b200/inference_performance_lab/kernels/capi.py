@@ -70,7 +70,7 @@ class PageCaches(ctypes.Structure):
 
     _fields_ = [
         ("caches", ctypes.POINTER(ctypes.c_void_p)),
-        *_fields("", "num_caches page_stride_bytes page_bytes token_bytes"),
+        *_fields("", "num_caches page_stride_bytes page_bytes"),
     ]
 
 
@@ -320,11 +320,9 @@ def pages_workspace(num_pages: int, count: int) -> int:
     return size.value
 
 
-def page_caches(
-    bases: list[int], page_stride_bytes: int, page_bytes: int, token_bytes: int
-) -> PageCaches:
+def page_caches(bases: list[int], page_stride_bytes: int, page_bytes: int) -> PageCaches:
     """The caches of a call; keeps the host array of bases alive."""
-    return PageCaches((ctypes.c_void_p * len(bases))(*bases), len(bases), page_stride_bytes, page_bytes, token_bytes)
+    return PageCaches((ctypes.c_void_p * len(bases))(*bases), len(bases), page_stride_bytes, page_bytes)
 
 
 def copy_pages(caches: PageCaches, num_pages: int, pairs_ptr: int, count: int, stream: int = 0) -> None:

@@ -103,7 +103,7 @@ class Pool:
         return 0
 
     def fork(self, parents, children):
-        """(pages lacking, [(source, target, tokens)]); nothing changes unless 0 are lacking."""
+        """(pages lacking, [(source, target)]); nothing changes unless 0 are lacking."""
         lens = [self.lens[p] for p in parents]
         free = self._free()
         need = sum(n % self.page != 0 for n in lens)
@@ -119,7 +119,7 @@ class Pool:
                 page = free.pop(0)
                 self.tables[child][whole] = page
                 self.refs[page] = 1
-                copies.append((self.tables[parent][whole], page, n % self.page))
+                copies.append((self.tables[parent][whole], page))
             self.lens[child] = n
         return 0, copies
 

@@ -55,8 +55,8 @@ class Device:
         lacking, copies = self.pool.fork(parents, children)
         assert status.tolist() == [lacking]
         self.same()
-        for source, target, tokens in copies:
-            assert torch.equal(self.view[:, target, :tokens], before[:, source, :tokens])
+        for source, target in copies:
+            assert torch.equal(self.view[:, target], before[:, source])
         kept = torch.ones(before.shape[1], dtype=torch.bool, device="cuda")
         kept[[c[1] for c in copies]] = False
         assert torch.equal(self.view[:, kept], before[:, kept])
@@ -245,8 +245,8 @@ def pool(**changes):
     return capi.PagePool(**a)
 
 
-def caches(stride=4096, size=4096, token=256, bases=(BASE, BASE + 4096)):
-    return capi.page_caches(list(bases), stride, size, token)
+def caches(stride=4096, size=4096, bases=(BASE, BASE + 4096)):
+    return capi.page_caches(list(bases), stride, size)
 
 
 @pytest.mark.parametrize("call, status, message", [
@@ -260,8 +260,7 @@ def caches(stride=4096, size=4096, token=256, bases=(BASE, BASE + 4096)):
     (lambda: capi.copy_pages(caches(stride=2048), 20, BASE, 1), capi.IPL_ERROR_INVALID_VALUE, "must not overlap"),
     (lambda: capi.copy_pages(caches(size=4088), 20, BASE, 1), capi.IPL_ERROR_MISALIGNED, "16"),
     (lambda: capi.copy_pages(caches(bases=(BASE + 8,)), 20, BASE, 1), capi.IPL_ERROR_MISALIGNED, "16"),
-    (lambda: capi.fork_sequences(caches(token=128), pool(), BASE, BASE, 1, BASE, 1 << 20, BASE), capi.IPL_ERROR_INVALID_VALUE,
-     "page_size tokens"),
+    (lambda: capi.fork_sequences(caches(), pool(), BASE, 0, 1, BASE, 1 << 20, BASE), capi.IPL_ERROR_INVALID_VALUE, "non-null"),
     (lambda: capi.compact_pages(caches(), pool(), BASE, BASE + 64, BASE, BASE, 1 << 20), capi.IPL_ERROR_INVALID_VALUE, "must not alias"),
 ])
 def test_argument_errors(call, status, message):
