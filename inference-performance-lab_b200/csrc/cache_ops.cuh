@@ -196,13 +196,95 @@ AttentionParams attention_params(const ipl_paged_attention_args& a) {
     return p;
 }
 
+// Which kernels a call runs, a pure function of its sizes, strides, alignment and the SM count.
+struct AttentionPlan {
+    bool vector = false;  // the short kernel; else a warp per row
+    int dim = 0;          // head size padded to 64 or 128
+    int tiles = 0;        // short kernel: column tiles of 8 rows
+    int splits = 1, split_len = 0;
+    size_t workspace = 0;
+};
+
+// 16-byte chunks of every row, and 16 keys of a block in one page.
+bool attention_vectorises(const ipl_paged_attention_args& a) {
+    const int64_t strides = a.output_token_stride | a.output_head_stride | a.query_token_stride | a.query_head_stride |
+                            a.key_cache_page_stride | a.key_cache_token_stride | a.key_cache_head_stride |
+                            a.value_cache_page_stride | a.value_cache_token_stride | a.value_cache_head_stride;
+    return a.head_size % 8 == 0 && a.head_size <= 128 && a.page_size % kAttentionBlock == 0 && strides % 8 == 0 &&
+           aligned(a.output, 16) && aligned(a.query, 16) && aligned(a.key_cache, 16) && aligned(a.value_cache, 16);
+}
+
+int64_t round_up(int64_t value, int64_t multiple) { return (value + multiple - 1) / multiple * multiple; }
+
+AttentionPlan plan_attention(const ipl_paged_attention_args& a, int sm_count) {
+    AttentionPlan plan;
+    if (!attention_vectorises(a)) return plan;
+    plan.vector = true;
+    plan.dim = a.head_size <= 64 ? 64 : 128;
+    const int64_t group = a.num_heads / a.num_kv_heads;
+    plan.tiles = a.max_query_len * group <= 8 ? 1 : 2;
+    // Keys a CTA takes: about a quarter of what fills the GPU once, so that ragged lengths even out,
+    // but a block for each of its warps at the least.
+    int64_t keys = a.max_seq_len > 1 ? a.max_seq_len : 1;
+    if (a.window > 0 && a.window + a.max_query_len < keys) keys = a.window + a.max_query_len;
+    const int64_t pairs = a.num_seqs * a.num_kv_heads;
+    const int64_t resident = static_cast<int64_t>(sm_count) * (plan.tiles == 1 ? 3 : 2);
+    constexpr int64_t kLeast = kShortWarps * kAttentionBlock;
+    int64_t len = round_up(pairs * keys / (resident * 4) + 1, kLeast);
+    int64_t splits = (keys + len - 1) / len;
+    if (splits > 256) {
+        len = round_up((keys + 255) / 256, kLeast);
+        splits = (keys + len - 1) / len;
+    }
+    plan.split_len = static_cast<int>(len);
+    plan.splits = static_cast<int>(splits);
+    if (splits > 1) {
+        const size_t rows = static_cast<size_t>(splits) * a.num_tokens * a.num_heads;
+        plan.workspace = rows * (plan.dim * sizeof(float) + sizeof(float2));
+    }
+    return plan;
+}
+
+template <int kDim>
+ipl_status launch_attention(const AttentionPlan& plan, const AttentionParams& p, cudaStream_t stream) {
+    const int64_t grid = static_cast<int64_t>(p.num_seqs) * p.kv_heads * plan.splits;
+    if (grid > INT_MAX) return fail(IPL_ERROR_TOO_LARGE, "too many sequences and heads");
+    constexpr unsigned kThreads = kShortWarps * kWarpSize;
+    const unsigned ctas = static_cast<unsigned>(grid);
+    ipl_status st = launch_status(plan.tiles == 1 ? launch(attention_short_kernel<kDim, 1>, ctas, kThreads, 0, stream, p)
+                                                  : launch(attention_short_kernel<kDim, 2>, ctas, kThreads, 0, stream, p),
+                                  "paged attention");
+    if (st != IPL_SUCCESS || plan.splits == 1) return st;
+    const int64_t rows = static_cast<int64_t>(p.num_tokens) * p.heads;
+    return launch_status(launch(attention_join_kernel<kDim>, static_cast<unsigned>((rows + kJoinWarps - 1) / kJoinWarps),
+                                kJoinWarps * kWarpSize, 0, stream, p),
+                         "paged attention");
+}
+
 ipl_status run_attention(const ipl_paged_attention_args* a, cudaStream_t stream) {
-    const ipl_status st = check_attention_args(a);
+    ipl_status st = check_attention_args(a);
     if (st != IPL_SUCCESS || a->num_tokens == 0 || a->num_seqs == 0) return st;
-    const AttentionParams p = attention_params(*a);
-    const int64_t rows = a->num_tokens * a->num_heads;
-    const unsigned grid = static_cast<unsigned>((rows + kAttentionRowWarps - 1) / kAttentionRowWarps);
-    return launch_status(launch(attention_row_kernel, grid, kAttentionRowWarps * kWarpSize, 0, stream, p), "paged attention");
+    int device = 0;
+    DeviceInfo* info = nullptr;
+    st = current_device(&device, &info);
+    if (st != IPL_SUCCESS) return st;
+    const AttentionPlan plan = plan_attention(*a, info->sm_count.load(std::memory_order_relaxed));
+    AttentionParams p = attention_params(*a);
+    if (!plan.vector) {
+        const int64_t rows = a->num_tokens * a->num_heads;
+        const unsigned grid = static_cast<unsigned>((rows + kAttentionRowWarps - 1) / kAttentionRowWarps);
+        return launch_status(launch(attention_row_kernel, grid, kAttentionRowWarps * kWarpSize, 0, stream, p), "paged attention");
+    }
+    if (a->workspace_bytes < plan.workspace) return fail(IPL_ERROR_INVALID_VALUE, "workspace is too small");
+    if (plan.workspace > 0 && (a->workspace == nullptr || !aligned(a->workspace, 16))) {
+        return fail(IPL_ERROR_INVALID_VALUE, "workspace must be non-null and 16-byte aligned");
+    }
+    p.short_rows = INT_MAX;
+    p.splits = plan.splits;
+    p.split_len = plan.split_len;
+    p.part_sums = static_cast<float*>(a->workspace);
+    p.part_stats = reinterpret_cast<float2*>(p.part_sums + static_cast<size_t>(plan.splits) * a->num_tokens * a->num_heads * plan.dim);
+    return plan.dim == 64 ? launch_attention<64>(plan, p, stream) : launch_attention<128>(plan, p, stream);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -324,14 +406,24 @@ ipl_status ipl_paged_attention_workspace(const ipl_paged_attention_args* args, s
     using namespace ipl;
     if (bytes == nullptr) return fail(IPL_ERROR_INVALID_VALUE, "bytes must be non-null");
     const ipl_status st = check_attention_args(args);
-    if (st == IPL_SUCCESS) *bytes = 0;
-    return st;
+    if (st != IPL_SUCCESS) return st;
+    int sms = 0, smem = 0;
+    plan_limits(&sms, &smem);
+    *bytes = args->num_tokens == 0 || args->num_seqs == 0 ? 0 : plan_attention(*args, sms).workspace;
+    return IPL_SUCCESS;
 }
 
 const char* ipl_paged_attention_plan(const ipl_paged_attention_args* args) {
     using namespace ipl;
     if (check_attention_args(args) != IPL_SUCCESS) return "invalid";
-    return args->num_tokens == 0 || args->num_seqs == 0 ? "none" : "attention_row_kernel";
+    if (args->num_tokens == 0 || args->num_seqs == 0) return "none";
+    int sms = 0, smem = 0;
+    plan_limits(&sms, &smem);
+    const AttentionPlan plan = plan_attention(*args, sms);
+    if (!plan.vector) return "attention_row_kernel";
+    if (plan.splits == 1) return plan.tiles == 1 ? "attention_short_kernel<1>" : "attention_short_kernel<2>";
+    return plan.tiles == 1 ? "attention_short_kernel<1> + attention_join_kernel"
+                           : "attention_short_kernel<2> + attention_join_kernel";
 }
 
 ipl_status ipl_pages_workspace(int64_t num_pages, int64_t count, size_t* bytes) {
