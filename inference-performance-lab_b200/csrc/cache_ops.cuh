@@ -4,6 +4,7 @@
 #include "cache_pages.cuh"
 #include "ipl_host.cuh"
 #include "paged_attention.cuh"
+#include "paged_attention_tile.cuh"
 #include "rotary.cuh"
 
 namespace ipl {
@@ -196,11 +197,52 @@ AttentionParams attention_params(const ipl_paged_attention_args& a) {
     return p;
 }
 
+// cuTensorMapEncodeTiled, from the driver the runtime has loaded (the library links no libcuda).
+using EncodeTensorMap = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                     const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                     CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTensorMap encode_tensor_map() {
+    static const EncodeTensorMap encode = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess) {
+            (void)cudaGetLastError();
+            f = nullptr;
+        }
+        return reinterpret_cast<EncodeTensorMap>(f);
+    }();
+    return encode;
+}
+
+// Map of bf16 elements, boxes of 64 elements in 128-byte swizzled rows; places outside read as 0.
+// strides in elements, of the dimensions after the first.
+ipl_status make_tensor_map(CUtensorMap* map, const void* base, int rank, const int64_t* sizes, const int64_t* strides,
+                           const int* box) {
+    const EncodeTensorMap encode = encode_tensor_map();
+    if (encode == nullptr) return fail(IPL_ERROR_CUDA, "the CUDA driver has no cuTensorMapEncodeTiled");
+    cuuint64_t dims[4], bytes[3];
+    cuuint32_t boxes[4], steps[4];
+    for (int i = 0; i < rank; ++i) {
+        dims[i] = static_cast<cuuint64_t>(sizes[i]);
+        boxes[i] = static_cast<cuuint32_t>(box[i]);
+        steps[i] = 1;
+        if (i > 0) bytes[i - 1] = static_cast<cuuint64_t>(strides[i - 1]) * 2;
+    }
+    const CUresult err = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<cuuint32_t>(rank), const_cast<void*>(base),
+                                dims, bytes, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (err != CUDA_SUCCESS) return fail(IPL_ERROR_CUDA, "cuTensorMapEncodeTiled failed: error %d", static_cast<int>(err));
+    return IPL_SUCCESS;
+}
+
 // Which kernels a call runs, a pure function of its sizes, strides, alignment and the SM count.
 struct AttentionPlan {
     bool vector = false;  // the short kernel; else a warp per row
     int dim = 0;          // head size padded to 64 or 128
-    int tiles = 0;        // short kernel: column tiles of 8 rows
+    int tiles = 0;        // short kernel: column tiles of 8 rows; 0: not launched
+    bool tile = false;    // the tile kernel takes the sequences of more than short_rows rows
+    int short_rows = 0;
     int splits = 1, split_len = 0;
     size_t workspace = 0;
 };
@@ -222,7 +264,24 @@ AttentionPlan plan_attention(const ipl_paged_attention_args& a, int sm_count) {
     plan.vector = true;
     plan.dim = a.head_size <= 64 ? 64 : 128;
     const int64_t group = a.num_heads / a.num_kv_heads;
-    plan.tiles = a.max_query_len * group <= 8 ? 1 : 2;
+    const int64_t rows = a.max_query_len * group;
+    plan.tiles = rows <= 8 ? 1 : 2;
+    plan.short_rows = INT_MAX;
+    // TMA takes strides of up to 2^40 bytes and no zero ones.
+    const int64_t strides[] = {a.query_token_stride, a.query_head_stride, a.key_cache_page_stride, a.key_cache_token_stride,
+                               a.key_cache_head_stride, a.value_cache_page_stride, a.value_cache_token_stride, a.value_cache_head_stride};
+    bool mappable = a.num_pages > 0;
+    for (const int64_t s : strides) mappable = mappable && s > 0 && s < (INT64_C(1) << 38);
+    if (rows > 16 && group <= kTileRows && mappable) {
+        plan.tile = true;
+        plan.tiles = group <= 8 ? 1 : 2;
+        plan.short_rows = plan.tiles * 8;
+        // Sequences of one length have no short one among them.
+        if (group > 16 || a.num_tokens == a.max_query_len * a.num_seqs) {
+            plan.tiles = 0;
+            plan.short_rows = 0;
+        }
+    }
     // Keys a CTA takes: about a quarter of what fills the GPU once, so that ragged lengths even out,
     // but a block for each of its warps at the least.
     int64_t keys = a.max_seq_len > 1 ? a.max_seq_len : 1;
@@ -238,7 +297,8 @@ AttentionPlan plan_attention(const ipl_paged_attention_args& a, int sm_count) {
     }
     plan.split_len = static_cast<int>(len);
     plan.splits = static_cast<int>(splits);
-    if (splits > 1) {
+    if (plan.tiles == 0) plan.splits = 1;
+    if (plan.splits > 1) {
         const size_t rows = static_cast<size_t>(splits) * a.num_tokens * a.num_heads;
         plan.workspace = rows * (plan.dim * sizeof(float) + sizeof(float2));
     }
@@ -246,19 +306,62 @@ AttentionPlan plan_attention(const ipl_paged_attention_args& a, int sm_count) {
 }
 
 template <int kDim>
-ipl_status launch_attention(const AttentionPlan& plan, const AttentionParams& p, cudaStream_t stream) {
+ipl_status launch_short(const AttentionPlan& plan, const AttentionParams& p, cudaStream_t stream) {
     const int64_t grid = static_cast<int64_t>(p.num_seqs) * p.kv_heads * plan.splits;
     if (grid > INT_MAX) return fail(IPL_ERROR_TOO_LARGE, "too many sequences and heads");
     constexpr unsigned kThreads = kShortWarps * kWarpSize;
     const unsigned ctas = static_cast<unsigned>(grid);
-    ipl_status st = launch_status(plan.tiles == 1 ? launch(attention_short_kernel<kDim, 1>, ctas, kThreads, 0, stream, p)
-                                                  : launch(attention_short_kernel<kDim, 2>, ctas, kThreads, 0, stream, p),
-                                  "paged attention");
+    const ipl_status st = launch_status(plan.tiles == 1 ? launch(attention_short_kernel<kDim, 1>, ctas, kThreads, 0, stream, p)
+                                                        : launch(attention_short_kernel<kDim, 2>, ctas, kThreads, 0, stream, p),
+                                        "paged attention");
     if (st != IPL_SUCCESS || plan.splits == 1) return st;
     const int64_t rows = static_cast<int64_t>(p.num_tokens) * p.heads;
     return launch_status(launch(attention_join_kernel<kDim>, static_cast<unsigned>((rows + kJoinWarps - 1) / kJoinWarps),
                                 kJoinWarps * kWarpSize, 0, stream, p),
                          "paged attention");
+}
+
+template <int kDim>
+ipl_status launch_tile(const ipl_paged_attention_args& a, const AttentionParams& p, DeviceInfo* info, cudaStream_t stream) {
+    using Layout = TileLayout<kDim>;
+    const uint32_t bit = 1u << (kDim == 64 ? 30 : 31);
+    if (!(info->smem_configured.load(std::memory_order_acquire) & bit)) {
+        const cudaError_t err = cudaFuncSetAttribute(attention_tile_kernel<kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                     static_cast<int>(Layout::kDynamic));
+        if (err != cudaSuccess) return fail(IPL_ERROR_CUDA, "paged attention kernel setup failed: %s", cudaGetErrorString(err));
+        info->smem_configured.fetch_or(bit, std::memory_order_acq_rel);
+    }
+    TileParams t;
+    t.a = p;
+    t.tile_tokens = kTileRows / p.group;
+    t.box_keys = kAttentionBlock;
+    while (t.box_keys < kTileKeys && p.page_size % (2 * t.box_keys) == 0) t.box_keys *= 2;
+    t.pairs = p.num_tokens / (2 * t.tile_tokens) + p.num_seqs;
+    const int64_t grid = static_cast<int64_t>(t.pairs) * p.kv_heads;
+    if (grid > INT_MAX) return fail(IPL_ERROR_TOO_LARGE, "too many tokens and heads");
+    CUtensorMap q, k, v;
+    const int64_t q_sizes[3] = {p.dim, p.heads, p.num_tokens}, q_strides[2] = {p.q_head, p.q_token};
+    const int q_box[3] = {64, p.group, t.tile_tokens};
+    ipl_status st = make_tensor_map(&q, a.query, 3, q_sizes, q_strides, q_box);
+    const int64_t sizes[4] = {p.dim, p.kv_heads, p.page_size, p.num_pages};
+    const int box[4] = {64, 1, t.box_keys, 1};
+    const int64_t k_strides[3] = {p.key_head, p.key_token, p.key_page};
+    const int64_t v_strides[3] = {p.value_head, p.value_token, p.value_page};
+    if (st == IPL_SUCCESS) st = make_tensor_map(&k, a.key_cache, 4, sizes, k_strides, box);
+    if (st == IPL_SUCCESS) st = make_tensor_map(&v, a.value_cache, 4, sizes, v_strides, box);
+    if (st != IPL_SUCCESS) return st;
+    return launch_status(launch(attention_tile_kernel<kDim>, static_cast<unsigned>(grid), kTileThreads, Layout::kDynamic, stream,
+                                t, q, k, v),
+                         "paged attention");
+}
+
+template <int kDim>
+ipl_status launch_attention(const ipl_paged_attention_args& a, const AttentionPlan& plan, const AttentionParams& p,
+                            DeviceInfo* info, cudaStream_t stream) {
+    ipl_status st = IPL_SUCCESS;
+    if (plan.tile) st = launch_tile<kDim>(a, p, info, stream);
+    if (st == IPL_SUCCESS && plan.tiles > 0) st = launch_short<kDim>(plan, p, stream);
+    return st;
 }
 
 ipl_status run_attention(const ipl_paged_attention_args* a, cudaStream_t stream) {
@@ -279,12 +382,12 @@ ipl_status run_attention(const ipl_paged_attention_args* a, cudaStream_t stream)
     if (plan.workspace > 0 && (a->workspace == nullptr || !aligned(a->workspace, 16))) {
         return fail(IPL_ERROR_INVALID_VALUE, "workspace must be non-null and 16-byte aligned");
     }
-    p.short_rows = INT_MAX;
+    p.short_rows = plan.short_rows;
     p.splits = plan.splits;
     p.split_len = plan.split_len;
     p.part_sums = static_cast<float*>(a->workspace);
     p.part_stats = reinterpret_cast<float2*>(p.part_sums + static_cast<size_t>(plan.splits) * a->num_tokens * a->num_heads * plan.dim);
-    return plan.dim == 64 ? launch_attention<64>(plan, p, stream) : launch_attention<128>(plan, p, stream);
+    return plan.dim == 64 ? launch_attention<64>(*a, plan, p, info, stream) : launch_attention<128>(*a, plan, p, info, stream);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -421,9 +524,13 @@ const char* ipl_paged_attention_plan(const ipl_paged_attention_args* args) {
     plan_limits(&sms, &smem);
     const AttentionPlan plan = plan_attention(*args, sms);
     if (!plan.vector) return "attention_row_kernel";
-    if (plan.splits == 1) return plan.tiles == 1 ? "attention_short_kernel<1>" : "attention_short_kernel<2>";
-    return plan.tiles == 1 ? "attention_short_kernel<1> + attention_join_kernel"
-                           : "attention_short_kernel<2> + attention_join_kernel";
+    static const char* const kNames[2][5] = {
+        {"attention_short_kernel<1>", "attention_short_kernel<2>", "attention_short_kernel<1> + attention_join_kernel",
+         "attention_short_kernel<2> + attention_join_kernel", "invalid"},
+        {"attention_tile_kernel + attention_short_kernel<1>", "attention_tile_kernel + attention_short_kernel<2>",
+         "attention_tile_kernel + attention_short_kernel<1> + attention_join_kernel",
+         "attention_tile_kernel + attention_short_kernel<2> + attention_join_kernel", "attention_tile_kernel"}};
+    return kNames[plan.tile ? 1 : 0][plan.tiles == 0 ? 4 : plan.tiles - 1 + (plan.splits > 1 ? 2 : 0)];
 }
 
 ipl_status ipl_pages_workspace(int64_t num_pages, int64_t count, size_t* bytes) {
