@@ -26,6 +26,7 @@ constexpr int kTileThreads = 384;  // three warpgroups, among which the register
 // Registers a thread: launched with 65536 / 384 rounded down to 168 (64512 in all), of which the two
 // softmax warpgroups take 208 and the third keeps 88 (64512 again).
 constexpr int kSoftmaxRegisters = 208, kOtherRegisters = 88;
+constexpr int kTilePolynomial = 0;  // of 16 pairs of weights, by the polynomial
 constexpr int kTileBoxes = kTileKeys / kAttentionBlock;  // boxes of at least 16 keys a tile
 
 struct TileParams {
@@ -49,6 +50,54 @@ struct TileLayout {
     static constexpr uint32_t kBytes = kItemBase + 128;
     static constexpr uint32_t kDynamic = kBytes + 1024;  // room to align to 1024
 };
+
+// Powers of two of a pair. The special-function units give 16 a cycle and SM, as many as the products of a
+// step have scores for each of their cycles, so a part of the pairs is computed on the FMA pipes:
+// 2^x = 2^n 2^r, n = x rounded (by adding 1.5 2^23, which leaves n in the low bits), r in [-1/2, 1/2],
+// with the polynomial of degree 3 of least relative error for 2^r (7.5e-5 by the Remez exchange, a fiftieth
+// of the rounding of a weight to bf16). x is held above -126, so a vanishing weight is 2^-126, not 0.
+__device__ __forceinline__ F32x2 exp2_pair_units(F32x2 x) {
+    float a, b;
+    f32x2_split(x, a, b);
+    return f32x2_make(exp2_approx(a), exp2_approx(b));
+}
+__device__ __forceinline__ F32x2 exp2_pair_polynomial(F32x2 x) {
+    float a, b;
+    f32x2_split(x, a, b);
+    x = f32x2_make(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
+    const F32x2 magic = f32x2_make(12582912.0f, 12582912.0f), minus = f32x2_make(-12582912.0f, -12582912.0f);
+    const F32x2 n = f32x2_add(x, magic);
+    const F32x2 r = f32x2_fma(f32x2_add(n, minus), f32x2_make(-1.0f, -1.0f), x);
+    F32x2 y = f32x2_fma(r, f32x2_make(0.05517166852951050f, 0.05517166852951050f), f32x2_make(0.2426111251115799f, 0.2426111251115799f));
+    y = f32x2_fma(y, r, f32x2_make(0.6932609677314758f, 0.6932609677314758f));
+    y = f32x2_fma(y, r, f32x2_make(0.9999280571937561f, 0.9999280571937561f));
+    float na, nb;
+    f32x2_split(n, na, nb);
+    f32x2_split(y, a, b);
+    return f32x2_make(__uint_as_float(__float_as_uint(a) + (__float_as_uint(na) << 23)),
+                      __uint_as_float(__float_as_uint(b) + (__float_as_uint(nb) << 23)));
+}
+
+// The largest of three, NaN if one is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+    return m;
+}
+
+// Weights of 32 scores: 2^(score scale - shift), rounded to bf16 pairs; their unrounded sum is added up.
+// kPolynomial: of every 16 pairs, this many by the polynomial.
+template <int kPolynomial>
+__device__ __forceinline__ void tile_weights(const float (&s)[32], F32x2 scale, F32x2 minus_shift, uint32_t (&w)[16], F32x2 (&sums)[2]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const F32x2 x = f32x2_fma(f32x2_make(s[2 * i], s[2 * i + 1]), scale, minus_shift);
+        const bool polynomial = (i + 1) * kPolynomial / 16 > i * kPolynomial / 16;
+        const F32x2 y = polynomial ? exp2_pair_polynomial(x) : exp2_pair_units(x);
+        sums[i & 1] = f32x2_add(sums[i & 1], y);
+        w[i] = f32x2_to_bf16x2(y);
+    }
+}
 
 // Tensor memory columns.
 constexpr uint32_t kTmemScores = 0;     // tile t at 128 t
@@ -108,7 +157,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     const uint32_t smem = (smem_addr(dynamic_smem) + 1023u) & ~1023u;
     const uint32_t bars = smem + L::kBarrierBase;
     const uint32_t stage_full = bars, stage_empty = bars + 8 * L::kStages;
-    const uint32_t q_full = bars + 16 * L::kStages, s_full = q_full + 16, p_ready = s_full + 16, o_full = p_ready + 16,
+    const uint32_t q_full = bars + 16 * L::kStages, s_full = q_full + 16, p_ready = s_full + 16, o_full = p_ready + 32,
                    drain = o_full + 16;
     const uint32_t tmem_slot = drain + 8;
     volatile int* const abort = reinterpret_cast<volatile int*>(dynamic_smem + (tmem_slot + 4 - smem_addr(dynamic_smem)));
@@ -125,7 +174,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
         for (int t = 0; t < 2; ++t) {
             mbar_init(q_full + 8 * t, 1);
             mbar_init(s_full + 8 * t, 1);
-            mbar_init(p_ready + 8 * t, 4);
+            mbar_init(p_ready + 16 * t, 4);
+            mbar_init(p_ready + 16 * t + 8, 4);
             mbar_init(o_full + 8 * t, 1);
         }
         mbar_init(drain, 1);
@@ -210,60 +260,83 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             for (int t = 0; t < item.tiles && item.steps > 0; ++t) mbar_wait_timed(q_full + 8 * t, 0, kFaultCopyDrainTimeout);
         }
       } else if (work && warp == 8) {
-        if (lane == 0 && item.steps > 0) {
-            // Issuer.
-            constexpr uint32_t kScores = mma_descriptor(kTileRows, kTileKeys, false);
-            constexpr uint32_t kOutput = mma_descriptor(kTileRows, kDim, true);
-            const auto scores = [&](int t, int stage) {
-                const uint32_t q = smem + t * L::kTileBytes, k = smem + L::kStageBase + stage * L::kTileBytes;
+        // Issuer: the whole warp walks, one elected lane issues.
+        const int steps = __shfl_sync(0xffffffffu, item.steps, 0), tiles = __shfl_sync(0xffffffffu, item.tiles, 0);
+        constexpr uint32_t kScores = mma_descriptor(kTileRows, kTileKeys, false);
+        constexpr uint32_t kOutput = mma_descriptor(kTileRows, kDim, true);
+        constexpr uint32_t kHigh = smem_descriptor_high(1024);
+        const uint32_t q_low = smem_descriptor_low(smem, 16);
+        const uint32_t k_low = smem_descriptor_low(smem + L::kStageBase, 16);
+        const uint32_t v_low = smem_descriptor_low(smem + L::kStageBase, L::kHalfBytes);
+        bool ok = true;
+        const auto wait = [&](uint32_t bar, uint32_t parity) {
+            ok = ok && mbar_wait_bounded(bar, parity, abort, kFaultFullBarrierTimeout);
+            ok = __all_sync(0xffffffffu, ok);
+            tcgen05_fence_after();
+            return ok;
+        };
+        const auto scores = [&](int t, int stage) {
+            const uint32_t q = q_low + t * (L::kTileBytes >> 4), k = k_low + stage * (L::kTileBytes >> 4);
+            if (elect_lane()) {
 #pragma unroll
                 for (int i = 0; i < kDim / 16; ++i) {
-                    const uint32_t at = (i / 4) * L::kHalfBytes + (i % 4) * 32u;
-                    mma_smem(tmem + kTmemScores + 128 * t, smem_descriptor(q + at, 16, 1024), smem_descriptor(k + at, 16, 1024),
-                             kScores, i > 0);
+                    const uint32_t at = (i / 4) * (L::kHalfBytes >> 4) + (i % 4) * 2u;
+                    mma_smem(tmem + kTmemScores + 128 * t, smem_descriptor(q + at, kHigh), smem_descriptor(k + at, kHigh), kScores,
+                             i > 0);
                 }
                 mma_commit(s_full + 8 * t);
-            };
-            bool ok = true;
-            const auto wait = [&](uint32_t bar, uint32_t parity) {
-                ok = ok && mbar_wait_bounded(bar, parity, abort, kFaultFullBarrierTimeout);
-                tcgen05_fence_after();
-                return ok;
-            };
-            if (wait(stage_full, 0)) {
-                for (int t = 0; t < item.tiles; ++t) {
-                    if (!wait(q_full + 8 * t, 0)) break;
-                    scores(t, 0);
-                }
-                if (ok && item.steps > 1) mma_commit(stage_empty);
             }
-            for (int step = 0; step < item.steps && ok; ++step) {
-                const bool more = step + 1 < item.steps;
-                const int v_load = 2 * step + 1, k_load = v_load + 1;
-                const int v_stage = v_load % L::kStages, k_stage = k_load % L::kStages;
-                if (!wait(stage_full + 8 * v_stage, (v_load / L::kStages) & 1)) break;
-                if (more && !wait(stage_full + 8 * k_stage, (k_load / L::kStages) & 1)) break;
-                for (int t = 0; t < item.tiles; ++t) {
-                    if (!wait(p_ready + 8 * t, step & 1)) break;
-                    const uint32_t v = smem + L::kStageBase + v_stage * L::kTileBytes;
+            __syncwarp();
+        };
+        const auto output = [&](int t, int stage, int half, bool first) {
+            const uint32_t v = v_low + stage * (L::kTileBytes >> 4);
+            if (elect_lane()) {
 #pragma unroll
-                    for (int i = 0; i < kTileKeys / 16; ++i) {
-                        mma_tmem(tmem + kTmemOutput + 128 * t, tmem + kTmemScores + 128 * t + 8 * i,
-                                 smem_descriptor(v + i * 2048u, L::kHalfBytes, 1024), kOutput, step > 0 || i > 0);
-                    }
-                    if (more) scores(t, k_stage);
-                    else mma_commit(o_full + 8 * t);
-                }
-                // None after the last step's: an arrival must not outlive the CTA.
-                if (more) {
-                    mma_commit(stage_empty + 8 * v_stage);
-                    mma_commit(stage_empty + 8 * k_stage);
+                for (int j = 0; j < kTileKeys / 32; ++j) {
+                    const int i = half * (kTileKeys / 32) + j;
+                    mma_tmem(tmem + kTmemOutput + 128 * t, tmem + kTmemScores + 128 * t + 8 * i,
+                             smem_descriptor(v + i * (2048u >> 4), kHigh), kOutput, !first || j > 0);
                 }
             }
-            if (*abort) {
-                mma_commit(drain);
-                mbar_wait_timed(drain, 0, kFaultCopyDrainTimeout);
+            __syncwarp();
+        };
+        const auto commit = [&](uint32_t bar) {
+            if (elect_lane()) mma_commit(bar);
+            __syncwarp();
+        };
+        if (steps > 0 && wait(stage_full, 0)) {
+            for (int t = 0; t < tiles; ++t) {
+                if (!wait(q_full + 8 * t, 0)) break;
+                scores(t, 0);
             }
+            if (ok && steps > 1) commit(stage_empty);
+        }
+        int v_stage = 1, v_phase = 0;
+        for (int step = 0; step < steps && ok; ++step) {
+            const bool more = step + 1 < steps;
+            int k_stage = v_stage + 1, k_phase = v_phase;
+            if (k_stage == L::kStages) k_stage = 0, k_phase ^= 1;
+            if (!wait(stage_full + 8 * v_stage, v_phase)) break;
+            if (more && !wait(stage_full + 8 * k_stage, k_phase)) break;
+            for (int t = 0; t < tiles; ++t) {
+                if (!wait(p_ready + 16 * t, step & 1)) break;
+                output(t, v_stage, 0, step == 0);
+                if (!wait(p_ready + 16 * t + 8, step & 1)) break;
+                output(t, v_stage, 1, false);
+                if (more) scores(t, k_stage);
+                else commit(o_full + 8 * t);
+            }
+            // None after the last step's: an arrival must not outlive the CTA.
+            if (ok && more) {
+                commit(stage_empty + 8 * v_stage);
+                commit(stage_empty + 8 * k_stage);
+            }
+            v_stage = k_stage + 1, v_phase = k_phase;
+            if (v_stage == L::kStages) v_stage = 0, v_phase ^= 1;
+        }
+        if (*abort) {
+            commit(drain);
+            mbar_wait_timed(drain, 0, kFaultCopyDrainTimeout);
         }
       }
     } else {
@@ -296,7 +369,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 const uint32_t mask = block_masks[step % 8];
                 const bool partial = begin > 0 || end < kTileKeys || mask != (1u << kTileBoxes) - 1u;
                 tmem_wait_loads();
-                if (__any_sync(0xffffffffu, partial)) {
+                const bool any_partial = __any_sync(0xffffffffu, partial);
+                if (any_partial) {
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
 #pragma unroll
@@ -309,13 +383,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 float m4[4];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    m4[c] = fmaxf(s[c][0], s[c][1]);
+                    m4[c] = s[c][0];
 #pragma unroll
-                    for (int i = 2; i < 32; i += 2) m4[c] = fmaxf(m4[c], fmaxf(s[c][i], s[c][i + 1]));
+                    for (int i = 1; i < 31; i += 2) m4[c] = max3(m4[c], s[c][i], s[c][i + 1]);
+                    m4[c] = max3(m4[c], s[c][31], s[c][31]);
                 }
-                const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.scale_log2;
-                // Move the reference point when it is left behind by more than 2^8.
-                const bool move = m > top + 8.0f;
+                const float m = max3(max3(m4[0], m4[1], m4[2]), m4[3], m4[3]) * a.scale_log2;
+                // Move the reference point when it is left behind by more than 2^8, and to NaN if a score is.
+                const bool move = real && !(m <= top + 8.0f);
                 if (__any_sync(0xffffffffu, move)) {
                     const float keep = move ? exp2_approx(top - m) : 1.0f;
                     if (move) {
@@ -335,21 +410,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     }
                 }
                 const float shift = top == -INFINITY ? 0.0f : top;
-                float sums[2] = {0.0f, 0.0f};
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t w[16];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float x = exp2_approx(fmaf(s[c][2 * i], a.scale_log2, -shift));
-                        const float y = exp2_approx(fmaf(s[c][2 * i + 1], a.scale_log2, -shift));
-                        sums[0] += x;
-                        sums[1] += y;
-                        w[i] = pack_bf16x2(x, y);
-                    }
-                    tmem_store_16(s_tmem + 16 * c, w);
-                }
-                sum += sums[0] + sums[1];
                 if (t == 0 && (key0 < item.first || key0 + kTileKeys > item.len || mask != (1u << kTileBoxes) - 1u)) {
                     // Value rows that no token sees may hold anything, NaN included: they become zeros before
                     // the product, which would carry a NaN into every row.
@@ -368,10 +428,26 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     }
                     fence_async_shared();
                 }
-                tmem_wait_stores();
-                tcgen05_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_ready + 8 * t);
+                const F32x2 scale = f32x2_make(a.scale_log2, a.scale_log2), minus_shift = f32x2_make(-shift, -shift);
+                F32x2 sums[2] = {0ull, 0ull};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t w[16];
+                    if (any_partial) tile_weights<0>(s[c], scale, minus_shift, w, sums);
+                    else tile_weights<kTilePolynomial>(s[c], scale, minus_shift, w, sums);
+                    tmem_store_16(s_tmem + 16 * c, w);
+                    if (c & 1) {
+                        // Half of the weights are there: their product can begin.
+                        tmem_wait_stores();
+                        tcgen05_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(p_ready + 16 * t + 8 * (c >> 1));
+                    }
+                }
+                float parts[4];
+                f32x2_split(sums[0], parts[0], parts[1]);
+                f32x2_split(sums[1], parts[2], parts[3]);
+                sum += (parts[0] + parts[1]) + (parts[2] + parts[3]);
             }
             if (ok && item.steps > 0) {
                 ok = mbar_wait_bounded(o_full + 8 * t, 0, abort, kFaultFullBarrierTimeout);

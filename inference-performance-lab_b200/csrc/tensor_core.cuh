@@ -91,9 +91,21 @@ __device__ __forceinline__ void warpgroup_leave_registers() {
 // address, leading and stride offsets in 16-byte units, version 1 at bit 46, swizzle mode 2 at bit 61.
 // * operand along rows (K-major): `stride` = 1024, the next 8 rows; the leading offset is unused;
 // * operand across rows (MN-major): `leading` = bytes to the next 64 elements of a row, `stride` = 1024.
-__device__ __forceinline__ uint64_t smem_descriptor(uint32_t address, uint32_t leading, uint32_t stride) {
-    return static_cast<uint64_t>((address & 0x3ffffu) >> 4) | static_cast<uint64_t>(leading >> 4) << 16 |
-           static_cast<uint64_t>(stride >> 4) << 32 | uint64_t{1} << 46 | uint64_t{2} << 61;
+// The address field takes sums in 16-byte units, so a descriptor moves by adding to its low word.
+__device__ __forceinline__ uint32_t smem_descriptor_low(uint32_t address, uint32_t leading) {
+    return ((address & 0x3ffffu) >> 4) | (leading >> 4) << 16;
+}
+constexpr uint32_t smem_descriptor_high(uint32_t stride) { return (stride >> 4) | 1u << 14 | 2u << 29; }
+__device__ __forceinline__ uint64_t smem_descriptor(uint32_t low, uint32_t high) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(low), "r"(high));
+    return d;
+}
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_lane() {
+    uint32_t elected;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
+    return elected != 0;
 }
 // kind::f16 instruction descriptor: fp32 accumulator, bf16 operands, A K-major, B K-major or MN-major.
 constexpr uint32_t mma_descriptor(int m, int n, bool b_mn_major) {

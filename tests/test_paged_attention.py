@@ -182,6 +182,8 @@ def test_keys_at_masked_positions_never_matter():
         kc[page, row] = bad
         got, _ = call(inputs, new, total)
         assert torch.equal(got[:39], expected[:39])
+        if bad != bad:
+            assert got[39].isnan().all()
 
 
 @gpu
