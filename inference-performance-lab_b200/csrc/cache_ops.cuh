@@ -10,6 +10,8 @@
 namespace ipl {
 namespace {
 
+int64_t round_up(int64_t value, int64_t multiple) { return (value + multiple - 1) / multiple * multiple; }
+
 bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 ipl_status launch_status(cudaError_t err, const char* what) {
@@ -243,6 +245,8 @@ struct AttentionPlan {
     int tiles = 0;        // short kernel: column tiles of 8 rows; 0: not launched
     bool tile = false;    // the tile kernel takes the sequences of more than short_rows rows
     int short_rows = 0;
+    int tile_ctas = 0;
+    size_t tile_workspace = 0;  // at the beginning of the workspace; the short kernel's parts follow
     int splits = 1, split_len = 0;
     size_t workspace = 0;
 };
@@ -255,8 +259,6 @@ bool attention_vectorises(const ipl_paged_attention_args& a) {
     return a.head_size % 8 == 0 && a.head_size <= 128 && a.page_size % kAttentionBlock == 0 && strides % 8 == 0 &&
            aligned(a.output, 16) && aligned(a.query, 16) && aligned(a.key_cache, 16) && aligned(a.value_cache, 16);
 }
-
-int64_t round_up(int64_t value, int64_t multiple) { return (value + multiple - 1) / multiple * multiple; }
 
 AttentionPlan plan_attention(const ipl_paged_attention_args& a, int sm_count) {
     AttentionPlan plan;
@@ -298,9 +300,15 @@ AttentionPlan plan_attention(const ipl_paged_attention_args& a, int sm_count) {
     plan.split_len = static_cast<int>(len);
     plan.splits = static_cast<int>(splits);
     if (plan.tiles == 0) plan.splits = 1;
+    if (plan.tile) {
+        plan.tile_ctas = sm_count;
+        const size_t slots = 2 * static_cast<size_t>(sm_count), rows = slots * 2 * kTileRows;
+        plan.tile_workspace = rows * (plan.dim * sizeof(float) + sizeof(float2)) + round_up(slots * sizeof(TilePart), 16);
+        plan.workspace = plan.tile_workspace;
+    }
     if (plan.splits > 1) {
         const size_t rows = static_cast<size_t>(splits) * a.num_tokens * a.num_heads;
-        plan.workspace = rows * (plan.dim * sizeof(float) + sizeof(float2));
+        plan.workspace += rows * (plan.dim * sizeof(float) + sizeof(float2));
     }
     return plan;
 }
@@ -322,7 +330,8 @@ ipl_status launch_short(const AttentionPlan& plan, const AttentionParams& p, cud
 }
 
 template <int kDim>
-ipl_status launch_tile(const ipl_paged_attention_args& a, const AttentionParams& p, DeviceInfo* info, cudaStream_t stream) {
+ipl_status launch_tile(const ipl_paged_attention_args& a, const AttentionPlan& plan, const AttentionParams& p,
+                       DeviceInfo* info, cudaStream_t stream) {
     using Layout = TileLayout<kDim>;
     const uint32_t bit = 1u << (kDim == 64 ? 30 : 31);
     if (!(info->smem_configured.load(std::memory_order_acquire) & bit)) {
@@ -336,9 +345,11 @@ ipl_status launch_tile(const ipl_paged_attention_args& a, const AttentionParams&
     t.tile_tokens = kTileRows / p.group;
     t.box_keys = kAttentionBlock;
     while (t.box_keys < kTileKeys && p.page_size % (2 * t.box_keys) == 0) t.box_keys *= 2;
-    t.pairs = p.num_tokens / (2 * t.tile_tokens) + p.num_seqs;
-    const int64_t grid = static_cast<int64_t>(t.pairs) * p.kv_heads;
-    if (grid > INT_MAX) return fail(IPL_ERROR_TOO_LARGE, "too many tokens and heads");
+    t.units = p.num_tokens / (2 * t.tile_tokens) + p.num_seqs;
+    const size_t rows = static_cast<size_t>(plan.tile_ctas) * 2 * 2 * kTileRows;
+    t.part_sums = static_cast<float*>(a.workspace);
+    t.part_stats = reinterpret_cast<float2*>(t.part_sums + rows * kDim);
+    t.parts = reinterpret_cast<TilePart*>(t.part_stats + rows);
     CUtensorMap q, k, v;
     const int64_t q_sizes[3] = {p.dim, p.heads, p.num_tokens}, q_strides[2] = {p.q_head, p.q_token};
     const int q_box[3] = {64, p.group, t.tile_tokens};
@@ -350,8 +361,12 @@ ipl_status launch_tile(const ipl_paged_attention_args& a, const AttentionParams&
     if (st == IPL_SUCCESS) st = make_tensor_map(&k, a.key_cache, 4, sizes, k_strides, box);
     if (st == IPL_SUCCESS) st = make_tensor_map(&v, a.value_cache, 4, sizes, v_strides, box);
     if (st != IPL_SUCCESS) return st;
-    return launch_status(launch(attention_tile_kernel<kDim>, static_cast<unsigned>(grid), kTileThreads, Layout::kDynamic, stream,
-                                t, q, k, v),
+    const unsigned ctas = static_cast<unsigned>(plan.tile_ctas);
+    st = launch_status(launch(attention_tile_kernel<kDim>, ctas, kTileThreads, Layout::kDynamic, stream, t, q, k, v),
+                       "paged attention");
+    if (st != IPL_SUCCESS) return st;
+    return launch_status(launch_2d(attention_tile_join_kernel<kDim>, ctas, 2 * kTileRows / kTileJoinWarps,
+                                   kTileJoinWarps * kWarpSize, stream, t),
                          "paged attention");
 }
 
@@ -359,7 +374,7 @@ template <int kDim>
 ipl_status launch_attention(const ipl_paged_attention_args& a, const AttentionPlan& plan, const AttentionParams& p,
                             DeviceInfo* info, cudaStream_t stream) {
     ipl_status st = IPL_SUCCESS;
-    if (plan.tile) st = launch_tile<kDim>(a, p, info, stream);
+    if (plan.tile) st = launch_tile<kDim>(a, plan, p, info, stream);
     if (st == IPL_SUCCESS && plan.tiles > 0) st = launch_short<kDim>(plan, p, stream);
     return st;
 }
@@ -385,7 +400,7 @@ ipl_status run_attention(const ipl_paged_attention_args* a, cudaStream_t stream)
     p.short_rows = plan.short_rows;
     p.splits = plan.splits;
     p.split_len = plan.split_len;
-    p.part_sums = static_cast<float*>(a->workspace);
+    p.part_sums = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + plan.tile_workspace);
     p.part_stats = reinterpret_cast<float2*>(p.part_sums + static_cast<size_t>(plan.splits) * a->num_tokens * a->num_heads * plan.dim);
     return plan.dim == 64 ? launch_attention<64>(*a, plan, p, info, stream) : launch_attention<128>(*a, plan, p, info, stream);
 }
@@ -527,9 +542,11 @@ const char* ipl_paged_attention_plan(const ipl_paged_attention_args* args) {
     static const char* const kNames[2][5] = {
         {"attention_short_kernel<1>", "attention_short_kernel<2>", "attention_short_kernel<1> + attention_join_kernel",
          "attention_short_kernel<2> + attention_join_kernel", "invalid"},
-        {"attention_tile_kernel + attention_short_kernel<1>", "attention_tile_kernel + attention_short_kernel<2>",
-         "attention_tile_kernel + attention_short_kernel<1> + attention_join_kernel",
-         "attention_tile_kernel + attention_short_kernel<2> + attention_join_kernel", "attention_tile_kernel"}};
+        {"attention_tile_kernel + attention_tile_join_kernel + attention_short_kernel<1>",
+         "attention_tile_kernel + attention_tile_join_kernel + attention_short_kernel<2>",
+         "attention_tile_kernel + attention_tile_join_kernel + attention_short_kernel<1> + attention_join_kernel",
+         "attention_tile_kernel + attention_tile_join_kernel + attention_short_kernel<2> + attention_join_kernel",
+         "attention_tile_kernel + attention_tile_join_kernel"}};
     return kNames[plan.tile ? 1 : 0][plan.tiles == 0 ? 4 : plan.tiles - 1 + (plan.splits > 1 ? 2 : 0)];
 }
 

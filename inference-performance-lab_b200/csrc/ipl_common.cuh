@@ -240,6 +240,34 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
     return done != 0;
 }
 
+// The same without a suspension time of our own: the waits of the tensor-core pipeline are short, and a
+// thread suspended for long wakes late.
+__device__ __forceinline__ bool mbar_poll(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+// mbar_wait_bounded by mbar_poll.
+__device__ __forceinline__ bool mbar_poll_bounded(uint32_t bar, uint32_t parity, volatile int* abort, uint32_t fault_bit) {
+    if (mbar_poll(bar, parity)) return true;
+    const uint64_t start = global_timer_ns();
+    for (;;) {
+        if (mbar_poll(bar, parity)) return true;
+        if (*abort) return false;
+        if (global_timer_ns() - start > kWaitLimitNs) {
+            atomicOr(&g_fault_word, fault_bit);
+            *abort = 1;
+            return false;
+        }
+    }
+}
+
 // Waits for the phase with the given parity to complete. Returns false (after recording
 // `fault_bit` in the device fault word) if it has not completed within kWaitLimitNs, or as soon
 // as *abort becomes nonzero (another warp of the CTA gave up).

@@ -81,6 +81,20 @@ void plan_limits(int* sm_count, int* smem_limit) {
 }
 
 template <typename Kernel, typename... Args>
+cudaError_t launch_2d(Kernel kernel, unsigned grid_x, unsigned grid_y, unsigned block, cudaStream_t stream, Args... args) {
+    cudaLaunchAttribute attribute[1];
+    attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(grid_x, grid_y);
+    config.blockDim = dim3(block);
+    config.stream = stream;
+    config.attrs = attribute;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
+template <typename Kernel, typename... Args>
 cudaError_t launch(Kernel kernel, unsigned grid, unsigned block, size_t smem, cudaStream_t stream,
                    Args... args) {
     // Programmatic stream serialisation: the kernel may be scheduled while the previous kernel

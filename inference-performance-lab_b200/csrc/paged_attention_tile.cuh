@@ -7,8 +7,13 @@
 //   S_t = Q_t K^T (tensor memory)  ->  P_t = exp2(scale S_t - m) (registers)  ->  O_t += P_t V
 // with the scores of one tile in the softmax while the tensor core works on the other. Roles:
 //   warps 0-3, 4-7   softmax of tile 0 and 1, a row a thread (a lane of tensor memory): no shuffles;
-//   warp 8           one thread issues the products;
-//   warp 9           loads K and V page by page (TMA) into a ring of shared-memory stages.
+//   warp 8           issues the products;
+//   warp 9           loads Q, and K and V page by page (TMA), into a ring of shared-memory stages;
+//   warp 10          hands out the work.
+// A CTA on every SM takes an equal share of the steps of all pairs of tiles and key heads, laid end to end;
+// a pair that a share's border cuts leaves parts in the workspace, which attention_tile_join_kernel adds.
+// Against a CTA for each pair, that evens out the last wave (57 pairs x 4 heads on 148 SMs are 1.54 waves)
+// and hides each pair's first loads behind the pair before.
 // P overwrites the first half of its S; the products are issued in the order P_t V (step j), Q_t K^T (step
 // j + 1), which the tensor core keeps, so nothing is overwritten early. The running maximum is only moved
 // when it has grown by more than 2^8, which then rescales O in tensor memory: the result is the same, as
@@ -26,14 +31,31 @@ constexpr int kTileThreads = 384;  // three warpgroups, among which the register
 // Registers a thread: launched with 65536 / 384 rounded down to 168 (64512 in all), of which the two
 // softmax warpgroups take 208 and the third keeps 88 (64512 again).
 constexpr int kSoftmaxRegisters = 208, kOtherRegisters = 88;
+constexpr int kTileHeadKeys = 96;   // weights of a step handed over first, so that their product begins early
 constexpr int kTilePolynomial = 0;  // of 16 pairs of weights, by the polynomial
 constexpr int kTileBoxes = kTileKeys / kAttentionBlock;  // boxes of at least 16 keys a tile
+constexpr uint32_t kAllBlocks = (1u << kTileBoxes) - 1u;
+
+constexpr int kTilePairCost = 1;  // of a pair beside its steps (first scores, output), in steps
+constexpr int kTileItems = 4;     // ring of work items
 
 struct TileParams {
     AttentionParams a;
     int tile_tokens;  // tokens a tile: 128 / group
     int box_keys;     // keys a TMA box: the largest power of two up to 128 that divides the page size
-    int pairs;        // upper bound of the tile pairs of all sequences
+    int units;        // upper bound of the tile pairs of all sequences
+    // Parts of pairs that several CTAs share. CTA c leaves at most two: in slot 2 c the last steps (or a middle
+    // stretch) of a pair that the CTA before began, in slot 2 c + 1 the first steps of one that it leaves to
+    // the next. A slot holds [256 rows][padded dim] sums and [256] (maximum, sum of weights).
+    float* part_sums;
+    float2* part_stats;
+    struct TilePart* parts;
+};
+
+// What is in a slot: nothing (tiles 0), or rows of a pair.
+struct TilePart {
+    int tiles, token, tokens, kv_head;  // first token, number of tokens of the pair
+    int last;                           // the pair's last steps
 };
 
 // Shared memory: the two Q tiles, the stages, the barriers. A tile of kDim 128 is two halves of 64
@@ -46,8 +68,8 @@ struct TileLayout {
     static constexpr int kStages = kDim == 128 ? 5 : 8;
     static constexpr uint32_t kStageBase = 2 * kTileBytes;
     static constexpr uint32_t kBarrierBase = kStageBase + kStages * kTileBytes;
-    static constexpr uint32_t kItemBase = kBarrierBase + 384;
-    static constexpr uint32_t kBytes = kItemBase + 128;
+    static constexpr uint32_t kItemBase = kBarrierBase + 512;
+    static constexpr uint32_t kBytes = kItemBase + kTileItems * 96;
     static constexpr uint32_t kDynamic = kBytes + 1024;  // room to align to 1024
 };
 
@@ -103,48 +125,52 @@ __device__ __forceinline__ void tile_weights(const float (&s)[32], F32x2 scale, 
 constexpr uint32_t kTmemScores = 0;     // tile t at 128 t
 constexpr uint32_t kTmemOutput = 256;   // tile t at 256 + 128 t
 
-// What a CTA works on; in shared memory, read where it is used, so that it takes no registers.
+// A stretch of steps of a pair. In shared memory, read where it is used, so that it takes no registers.
 struct TileItem {
-    int work;  // 0: nothing
-    int seq, begin, new_tokens, true_len, len, first;
+    int work;  // 0: no more
+    int seq, first, len;  // keys [first, len) of the sequence may be read
     int kv_head;
-    int token0;     // of the pair, in the sequence
-    int tiles;      // 1 or 2
-    int key0;       // of step 0, a multiple of 128
+    int token, tokens;  // first token of the pair (row of query), number of tokens
+    int position;       // of the first token
+    int tiles;          // 1 or 2
+    int key0;           // of the first step, a multiple of 128
     int steps;
+    int slot;           // for parts; -1: the whole pair
+    // Running counts before this item, for the phases of the barriers: stage loads, and for each tile steps
+    // and items with steps.
+    int loads, tile_steps[2], tile_items[2];
+};
+static_assert(sizeof(TileItem) <= 96, "fits its place in shared memory");
+
+// A pair of tiles as its sequence defines it.
+struct TilePair {
+    int seq, token, tokens, position, first, len, key0, steps;
 };
 
-__device__ __forceinline__ TileItem tile_item(const TileParams& p) {
-    TileItem item = {};
+// Pair number u: sequence s starts at number starts[s] / (tokens a pair) + s, which leaves it room for its own
+// rounded up. Returns false for a number that no pair has.
+__device__ __forceinline__ bool tile_pair(const TileParams& p, int u, TilePair& pair) {
     const AttentionParams& a = p.a;
-    const uint32_t unit = blockIdx.x / a.kv_heads;
-    item.kv_head = blockIdx.x - unit * a.kv_heads;
-    // Pair numbers are laid out so that sequence s starts at starts[s] / (tokens a pair) + s, which leaves it
-    // room for its own rounded up. The last pairs, which see the most keys, come first.
     const int pair_tokens = 2 * p.tile_tokens;
-    const int u = p.pairs - 1 - static_cast<int>(unit);
     int lo = 0, hi = a.num_seqs - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (a.starts[mid] / pair_tokens + mid <= u) lo = mid;
         else hi = mid - 1;
     }
-    item.seq = lo;
-    item.begin = a.starts[lo];
-    item.new_tokens = min(a.starts[lo + 1], a.num_tokens) - item.begin;
-    item.token0 = (u - (item.begin / pair_tokens + lo)) * pair_tokens;
-    if (item.begin < 0 || item.token0 < 0 || item.token0 >= item.new_tokens || item.new_tokens * a.group <= a.short_rows) return item;
-    item.tiles = item.token0 + p.tile_tokens < item.new_tokens ? 2 : 1;
-    item.true_len = a.lens[lo];
-    item.len = table_bounded_length(a, lo);
-    const int from = item.true_len - item.new_tokens + item.token0;  // position of the pair's first token
-    const int last = item.true_len - item.new_tokens + min(item.token0 + pair_tokens, item.new_tokens) - 1;
-    item.first = from >= a.window ? from - a.window + 1 : 0;
-    const int stop = min(last + 1, item.len);
-    item.key0 = item.first / kTileKeys * kTileKeys;
-    item.steps = stop > item.key0 ? (stop - item.key0 + kTileKeys - 1) / kTileKeys : 0;
-    item.work = 1;
-    return item;
+    const int begin = a.starts[lo], new_tokens = min(a.starts[lo + 1], a.num_tokens) - begin;
+    const int token0 = (u - (begin / pair_tokens + lo)) * pair_tokens;
+    if (u >= p.units || begin < 0 || token0 < 0 || token0 >= new_tokens || new_tokens * a.group <= a.short_rows) return false;
+    pair.seq = lo;
+    pair.token = begin + token0;
+    pair.tokens = min(pair_tokens, new_tokens - token0);
+    pair.position = a.lens[lo] - new_tokens + token0;
+    pair.len = table_bounded_length(a, lo);
+    pair.first = pair.position >= a.window ? pair.position - a.window + 1 : 0;
+    const int stop = min(pair.position + pair.tokens, pair.len);
+    pair.key0 = pair.first / kTileKeys * kTileKeys;
+    pair.steps = stop > pair.key0 ? (stop - pair.key0 + kTileKeys - 1) / kTileKeys : 0;
+    return true;
 }
 
 template <int kDim>
@@ -157,12 +183,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     const uint32_t smem = (smem_addr(dynamic_smem) + 1023u) & ~1023u;
     const uint32_t bars = smem + L::kBarrierBase;
     const uint32_t stage_full = bars, stage_empty = bars + 8 * L::kStages;
-    const uint32_t q_full = bars + 16 * L::kStages, s_full = q_full + 16, p_ready = s_full + 16, o_full = p_ready + 32,
-                   drain = o_full + 16;
-    const uint32_t tmem_slot = drain + 8;
-    volatile int* const abort = reinterpret_cast<volatile int*>(dynamic_smem + (tmem_slot + 4 - smem_addr(dynamic_smem)));
-    // Blocks of 16 keys of step j whose page is in the cache, at j % 8: the ring is shorter than that.
-    volatile uint32_t* const block_masks = reinterpret_cast<volatile uint32_t*>(dynamic_smem + (tmem_slot + 8 - smem_addr(dynamic_smem)));
+    const uint32_t q_full = bars + 16 * L::kStages, q_empty = q_full + 16, s_full = q_empty + 8, p_ready = s_full + 16;
+    const uint32_t o_full = p_ready + 32, item_full = o_full + 16, item_empty = item_full + 8 * kTileItems;
+    const uint32_t drain = item_empty + 8 * kTileItems, tmem_slot = drain + 8;
+    const auto at = [&](uint32_t address) { return dynamic_smem + (address - smem_addr(dynamic_smem)); };
+    volatile int* const abort = reinterpret_cast<volatile int*>(at(tmem_slot + 4));
+    // Blocks of 16 keys of a step whose page is in the cache, at its number % 8: the ring is shorter than that.
+    volatile uint32_t* const block_masks = reinterpret_cast<volatile uint32_t*>(at(tmem_slot + 8));
+    volatile TileItem* const items = reinterpret_cast<volatile TileItem*>(at(smem + L::kItemBase));
 
     const int warp = threadIdx.x / kWarpSize, lane = threadIdx.x % kWarpSize;
     const AttentionParams& a = p.a;
@@ -178,6 +206,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             mbar_init(p_ready + 16 * t + 8, 4);
             mbar_init(o_full + 8 * t, 1);
         }
+        for (int i = 0; i < kTileItems; ++i) {
+            mbar_init(item_full + 8 * i, 1);
+            mbar_init(item_empty + 8 * i, 10);
+        }
+        mbar_init(q_empty, 1);
         mbar_init(drain, 1);
         *abort = 0;
         fence_mbar_init();
@@ -190,78 +223,193 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     if (warp == 8) tmem_alloc(tmem_slot);
     grid_dependency_wait();
     grid_launch_dependents();
-    TileItem* const shared_item = reinterpret_cast<TileItem*>(dynamic_smem + (smem + L::kItemBase - smem_addr(dynamic_smem)));
-    if (threadIdx.x == 0) *shared_item = tile_item(p);
+
+    // This CTA's share of the steps: of the pairs of one key head in their order, then of the next head. The
+    // items' memory serves the sums. Pair u weighs its steps and kTilePairCost.
+    int* const scratch = reinterpret_cast<int*>(at(smem + L::kItemBase));
+    const auto weight = [&](int u) {
+        TilePair pair;
+        return u < p.units && tile_pair(p, u, pair) ? pair.steps + kTilePairCost : 0;
+    };
+    int sum = 0;
+    for (int u = threadIdx.x; u < p.units; u += kTileThreads) sum += weight(u);
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    if (lane == 0) scratch[warp] = sum;
+    __syncthreads();
+    int head_weight = 0;
+    for (int w = 0; w < kTileThreads / kWarpSize; ++w) head_weight += scratch[w];
+    const int64_t all_weight = static_cast<int64_t>(head_weight) * a.kv_heads;
+    const int64_t share_begin = all_weight * blockIdx.x / gridDim.x, share_end = all_weight * (blockIdx.x + 1) / gridDim.x;
+    const int begin_head = head_weight > 0 ? static_cast<int>(share_begin / head_weight) : 0;
+    const int begin_weight = static_cast<int>(share_begin - static_cast<int64_t>(begin_head) * head_weight);
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
-    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(dynamic_smem + (tmem_slot - smem_addr(dynamic_smem)));
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(at(tmem_slot));
 
-    const volatile TileItem& item = *shared_item;
-    const bool work = item.work != 0;
     if (warp >= 8) {
       warpgroup_leave_registers<kOtherRegisters>();
-      if (work && warp == 9) {
-        // Producer. Lane l loads box l % boxes, half l / boxes of a stage.
-        const int boxes = kTileKeys / p.box_keys;
-        const uint32_t box_bytes = static_cast<uint32_t>(p.box_keys) * 128u;
-        const int32_t* table = a.tables + item.seq * a.table_row;
-        if (lane == 0 && item.steps > 0) {
-            const uint32_t rows = static_cast<uint32_t>(p.tile_tokens) * a.group;
-            for (int t = 0; t < item.tiles; ++t) {
-                mbar_arrive_expect_tx(q_full + 8 * t, L::kHalves * rows * 128u);
-                for (int h = 0; h < L::kHalves; ++h) {
-                    tma_load_3d(smem + t * L::kTileBytes + h * L::kHalfBytes, &q_map, 64 * h, item.kv_head * a.group,
-                                item.begin + item.token0 + t * p.tile_tokens, q_full + 8 * t);
+      if (warp == 10) {
+        // Work: 32 pairs at a time, one a lane; lane 0 writes the items.
+        if (lane < 2) p.parts[2 * blockIdx.x + lane].tiles = 0;
+        __syncwarp();
+        int n = 0;
+        const auto put = [&](const TileItem& item) {
+            const int place = n % kTileItems;
+            bool ok = mbar_poll_bounded(item_empty + 8 * place, ((n / kTileItems) & 1) ^ 1, abort, kFaultEmptyBarrierTimeout);
+            ok = __all_sync(0xffffffffu, ok);
+            if (ok && lane == 0) {
+                volatile int* to = reinterpret_cast<volatile int*>(items + place);
+                const int* from = reinterpret_cast<const int*>(&item);
+#pragma unroll
+                for (int i = 0; i < static_cast<int>(sizeof(TileItem) / 4); ++i) to[i] = from[i];
+                mbar_arrive(item_full + 8 * place);
+            }
+            __syncwarp();
+            ++n;
+            return ok;
+        };
+        int64_t left = share_end - share_begin;
+        int skip = begin_weight, head = begin_head;  // weight of this head's pairs before the share
+        TileItem item = {};
+        bool ok = true;
+        for (int base = 0; left > 0 && ok; base += kWarpSize) {
+            if (base >= p.units) base = 0, skip = 0, ++head;
+            if (head >= a.kv_heads) break;
+            TilePair pair = {};
+            const bool exists = tile_pair(p, base + lane, pair);
+            for (uint32_t set = __ballot_sync(0xffffffffu, exists); set != 0 && left > 0 && ok; set &= set - 1) {
+                const int from = __ffs(set) - 1;
+                const int steps = __shfl_sync(0xffffffffu, pair.steps, from), weight = steps + kTilePairCost;
+                if (skip >= weight) {
+                    skip -= weight;
+                    continue;
+                }
+                const int take = static_cast<int>(left < weight - skip ? left : weight - skip);
+                const int step_begin = max(skip - kTilePairCost, 0), step_end = max(skip + take - kTilePairCost, 0);
+                const bool mine = steps > 0 ? step_end > step_begin : skip == 0;
+                skip = 0;
+                left -= take;
+                if (!mine) continue;
+                item.work = 1;
+                item.kv_head = head;
+                item.seq = __shfl_sync(0xffffffffu, pair.seq, from);
+                item.first = __shfl_sync(0xffffffffu, pair.first, from);
+                item.len = __shfl_sync(0xffffffffu, pair.len, from);
+                item.token = __shfl_sync(0xffffffffu, pair.token, from);
+                item.tokens = __shfl_sync(0xffffffffu, pair.tokens, from);
+                item.position = __shfl_sync(0xffffffffu, pair.position, from);
+                item.tiles = item.tokens > p.tile_tokens ? 2 : 1;
+                item.key0 = __shfl_sync(0xffffffffu, pair.key0, from) + step_begin * kTileKeys;
+                item.steps = step_end - step_begin;
+                item.slot = -1;
+                if (item.steps < steps) {
+                    item.slot = 2 * blockIdx.x + (step_begin == 0 ? 1 : 0);
+                    if (lane == 0) {
+                        TilePart& part = p.parts[item.slot];
+                        part.token = item.token;
+                        part.tokens = item.tokens;
+                        part.kv_head = head;
+                        part.last = step_end == steps;
+                        part.tiles = item.tiles;
+                    }
+                }
+                ok = put(item);
+                item.loads += 2 * item.steps;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (t < item.tiles) item.tile_steps[t] += item.steps, item.tile_items[t] += item.steps > 0;
                 }
             }
         }
+        item.work = 0;
+        if (ok) put(item);
+      } else if (warp == 9) {
+        // Producer. Lane l loads box l % boxes, half l / boxes of a stage.
+        const int boxes = kTileKeys / p.box_keys;
+        const uint32_t box_bytes = static_cast<uint32_t>(p.box_keys) * 128u;
+        const uint32_t q_bytes = L::kHalves * static_cast<uint32_t>(p.tile_tokens) * a.group * 128u;
         bool ok = true;
-        int loads = 0;
-        for (int step = 0; step < item.steps && ok; ++step) {
-            const int key0 = item.key0 + step * kTileKeys;
-            const int box = lane % boxes, half = lane / boxes;
-            const int key = key0 + box * p.box_keys;
-            int page = -1;
-            const bool wanted = key < item.len && key + p.box_keys > item.first;
-            if (wanted) {
-                page = table[key / a.page_size];
-                if (page < 0 || page >= a.num_pages) {
-                    atomicOr(&g_fault_word, kFaultIndexOutOfRange);
-                    page = -1;
+        int loads = 0, q_loads = 0, tile_loads[2] = {0, 0};
+        for (int n = 0;; ++n) {
+            const volatile TileItem& item = items[n % kTileItems];
+            ok = ok && mbar_poll_bounded(item_full + 8 * (n % kTileItems), (n / kTileItems) & 1, abort, kFaultFullBarrierTimeout);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok || item.work == 0) break;
+            const int32_t* table = a.tables + item.seq * a.table_row;
+            const int len = item.len, first = item.first, steps = item.steps, kv_head = item.kv_head, tiles = item.tiles;
+            for (int step = 0; step < steps && ok; ++step) {
+                const int key0 = item.key0 + step * kTileKeys;
+                const int box = lane % boxes, half = lane / boxes;
+                const int key = key0 + box * p.box_keys;
+                int page = -1;
+                const bool wanted = key < len && key + p.box_keys > first;
+                if (wanted) {
+                    page = table[key / a.page_size];
+                    if (page < 0 || page >= a.num_pages) {
+                        atomicOr(&g_fault_word, kFaultIndexOutOfRange);
+                        page = -1;
+                    }
+                }
+                // One bit a block of 16 keys: set unless the box's page is missing.
+                const uint32_t per_box = p.box_keys / kAttentionBlock;
+                uint32_t mask = wanted && page < 0 ? ((1u << per_box) - 1u) << (box * per_box) : 0u;
+                mask = ~__reduce_or_sync(0xffffffffu, mask) & kAllBlocks;
+                const uint32_t count = __popc(__ballot_sync(0xffffffffu, page >= 0 && lane < boxes)) * L::kHalves;
+                if (lane == 0) block_masks[(loads / 2) % 8] = mask;
+                const int in_page = key % a.page_size;
+                for (int which = 0; which < 2; ++which, ++loads) {
+                    const int stage = loads % L::kStages;
+                    ok = mbar_poll_bounded(stage_empty + 8 * stage, ((loads / L::kStages) & 1) ^ 1, abort, kFaultEmptyBarrierTimeout);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    const uint32_t full = stage_full + 8 * stage;
+                    if (lane == 0) mbar_arrive_expect_tx(full, count * box_bytes);
+                    __syncwarp();
+                    if (page >= 0 && half < L::kHalves) {
+                        const uint32_t dst = smem + L::kStageBase + stage * L::kTileBytes + half * L::kHalfBytes + box * box_bytes;
+                        tma_load_4d(dst, which == 0 ? &k_map : &v_map, 64 * half, kv_head, in_page, page, full);
+                    }
+                    if (step == 0 && which == 0) {
+                        // Q behind the first keys, once the scores of the item before are done with its place.
+                        ok = mbar_poll_bounded(q_empty, (q_loads & 1) ^ 1, abort, kFaultEmptyBarrierTimeout);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) {
+                            ++loads;
+                            break;
+                        }
+                        ++q_loads;
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) {
+                            if (t >= tiles) break;
+                            if (lane == 0) {
+                                mbar_arrive_expect_tx(q_full + 8 * t, q_bytes);
+                                for (int h = 0; h < L::kHalves; ++h) {
+                                    tma_load_3d(smem + t * L::kTileBytes + h * L::kHalfBytes, &q_map, 64 * h, kv_head * a.group,
+                                                item.token + t * p.tile_tokens, q_full + 8 * t);
+                                }
+                            }
+                            ++tile_loads[t];
+                        }
+                        __syncwarp();
+                    }
                 }
             }
-            // One bit a block of 16 keys: set unless the box's page is missing.
-            const uint32_t per_box = p.box_keys / kAttentionBlock;
-            uint32_t mask = wanted && page < 0 ? ((1u << per_box) - 1u) << (box * per_box) : 0u;
-            mask = ~__reduce_or_sync(0xffffffffu, mask) & ((1u << kTileBoxes) - 1u);
-            const uint32_t count = __popc(__ballot_sync(0xffffffffu, page >= 0 && lane < boxes)) * L::kHalves;
-            if (lane == 0) block_masks[step % 8] = mask;
-            const int in_page = key % a.page_size;
-            for (int which = 0; which < 2; ++which, ++loads) {
-                const int stage = loads % L::kStages;
-                ok = mbar_wait_bounded(stage_empty + 8 * stage, ((loads / L::kStages) & 1) ^ 1, abort, kFaultEmptyBarrierTimeout);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                const uint32_t full = stage_full + 8 * stage;
-                if (lane == 0) mbar_arrive_expect_tx(full, count * box_bytes);
-                __syncwarp();
-                if (page >= 0 && half < L::kHalves) {
-                    const uint32_t dst = smem + L::kStageBase + stage * L::kTileBytes + half * L::kHalfBytes + box * box_bytes;
-                    tma_load_4d(dst, which == 0 ? &k_map : &v_map, 64 * half, item.kv_head, in_page, page, full);
-                }
-            }
+            if (ok && lane == 0) mbar_arrive(item_empty + 8 * (n % kTileItems));
+            __syncwarp();
         }
         if (*abort) {
             // Let every copy issued land before the CTA may leave.
             for (int i = loads - L::kStages > 0 ? loads - L::kStages : 0; i < loads; ++i) {
                 mbar_wait_timed(stage_full + 8 * (i % L::kStages), (i / L::kStages) & 1, kFaultCopyDrainTimeout);
             }
-            for (int t = 0; t < item.tiles && item.steps > 0; ++t) mbar_wait_timed(q_full + 8 * t, 0, kFaultCopyDrainTimeout);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                if (tile_loads[t] > 0) mbar_wait_timed(q_full + 8 * t, (tile_loads[t] - 1) & 1, kFaultCopyDrainTimeout);
+            }
         }
-      } else if (work && warp == 8) {
+      } else if (warp == 8) {
         // Issuer: the whole warp walks, one elected lane issues.
-        const int steps = __shfl_sync(0xffffffffu, item.steps, 0), tiles = __shfl_sync(0xffffffffu, item.tiles, 0);
         constexpr uint32_t kScores = mma_descriptor(kTileRows, kTileKeys, false);
         constexpr uint32_t kOutput = mma_descriptor(kTileRows, kDim, true);
         constexpr uint32_t kHigh = smem_descriptor_high(1024);
@@ -270,7 +418,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
         const uint32_t v_low = smem_descriptor_low(smem + L::kStageBase, L::kHalfBytes);
         bool ok = true;
         const auto wait = [&](uint32_t bar, uint32_t parity) {
-            ok = ok && mbar_wait_bounded(bar, parity, abort, kFaultFullBarrierTimeout);
+            ok = ok && mbar_poll_bounded(bar, parity, abort, kFaultFullBarrierTimeout);
             ok = __all_sync(0xffffffffu, ok);
             tcgen05_fence_after();
             return ok;
@@ -288,14 +436,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             }
             __syncwarp();
         };
-        const auto output = [&](int t, int stage, int half, bool first) {
+        // The products of 16 keys each with weights that are there: from 0 to 5 and 6, 7.
+        const auto output = [&](int t, int stage, bool head, bool first) {
             const uint32_t v = v_low + stage * (L::kTileBytes >> 4);
             if (elect_lane()) {
 #pragma unroll
-                for (int j = 0; j < kTileKeys / 32; ++j) {
-                    const int i = half * (kTileKeys / 32) + j;
+                for (int i = 0; i < kTileKeys / 16; ++i) {
+                    if ((i < kTileHeadKeys / 16) != head) continue;
                     mma_tmem(tmem + kTmemOutput + 128 * t, tmem + kTmemScores + 128 * t + 8 * i,
-                             smem_descriptor(v + i * (2048u >> 4), kHigh), kOutput, !first || j > 0);
+                             smem_descriptor(v + i * (2048u >> 4), kHigh), kOutput, !first || i > 0);
                 }
             }
             __syncwarp();
@@ -304,93 +453,124 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             if (elect_lane()) mma_commit(bar);
             __syncwarp();
         };
-        if (steps > 0 && wait(stage_full, 0)) {
-            for (int t = 0; t < tiles; ++t) {
-                if (!wait(q_full + 8 * t, 0)) break;
-                scores(t, 0);
+        int stage = 0, phase = 0;  // of the next load to be consumed
+        const auto next_stage = [&](int& s, int& f) {
+            if (++s == L::kStages) s = 0, f ^= 1;
+        };
+        int tile_steps[2] = {0, 0}, tile_items[2] = {0, 0};
+        for (int n = 0;; ++n) {
+            const volatile TileItem& item = items[n % kTileItems];
+            if (!wait(item_full + 8 * (n % kTileItems), (n / kTileItems) & 1) || item.work == 0) break;
+            const int steps = __shfl_sync(0xffffffffu, item.steps, 0), tiles = __shfl_sync(0xffffffffu, item.tiles, 0);
+            if (steps > 0 && wait(stage_full + 8 * stage, phase)) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (t >= tiles) break;
+                    if (!wait(q_full + 8 * t, tile_items[t] & 1)) break;
+                    ++tile_items[t];
+                    scores(t, stage);
+                }
+                if (ok) commit(stage_empty + 8 * stage);
+                if (ok && steps == 1) commit(q_empty);
+                next_stage(stage, phase);
             }
-            if (ok && steps > 1) commit(stage_empty);
-        }
-        int v_stage = 1, v_phase = 0;
-        for (int step = 0; step < steps && ok; ++step) {
-            const bool more = step + 1 < steps;
-            int k_stage = v_stage + 1, k_phase = v_phase;
-            if (k_stage == L::kStages) k_stage = 0, k_phase ^= 1;
-            if (!wait(stage_full + 8 * v_stage, v_phase)) break;
-            if (more && !wait(stage_full + 8 * k_stage, k_phase)) break;
-            for (int t = 0; t < tiles; ++t) {
-                if (!wait(p_ready + 16 * t, step & 1)) break;
-                output(t, v_stage, 0, step == 0);
-                if (!wait(p_ready + 16 * t + 8, step & 1)) break;
-                output(t, v_stage, 1, false);
-                if (more) scores(t, k_stage);
-                else commit(o_full + 8 * t);
+            for (int step = 0; step < steps && ok; ++step) {
+                const bool more = step + 1 < steps;
+                int k_stage = stage, k_phase = phase;
+                next_stage(k_stage, k_phase);
+                if (!wait(stage_full + 8 * stage, phase)) break;
+                if (more && !wait(stage_full + 8 * k_stage, k_phase)) break;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (t >= tiles) break;
+                    if (!wait(p_ready + 16 * t, tile_steps[t] & 1)) break;
+                    output(t, stage, true, step == 0);
+                    if (!wait(p_ready + 16 * t + 8, tile_steps[t] & 1)) break;
+                    ++tile_steps[t];
+                    output(t, stage, false, false);
+                    if (more) scores(t, k_stage);
+                    else commit(o_full + 8 * t);
+                }
+                if (!ok) break;
+                commit(stage_empty + 8 * stage);
+                next_stage(stage, phase);
+                if (more) {
+                    commit(stage_empty + 8 * k_stage);
+                    if (step + 2 == steps) commit(q_empty);
+                    next_stage(stage, phase);
+                }
             }
-            // None after the last step's: an arrival must not outlive the CTA.
-            if (ok && more) {
-                commit(stage_empty + 8 * v_stage);
-                commit(stage_empty + 8 * k_stage);
-            }
-            v_stage = k_stage + 1, v_phase = k_phase;
-            if (v_stage == L::kStages) v_stage = 0, v_phase ^= 1;
+            if (!ok) break;
+            if (lane == 0) mbar_arrive(item_empty + 8 * (n % kTileItems));
+            __syncwarp();
         }
-        if (*abort) {
-            commit(drain);
-            mbar_wait_timed(drain, 0, kFaultCopyDrainTimeout);
-        }
+        // No product and no arrival outlives the CTA.
+        commit(drain);
+        mbar_wait_timed(drain, 0, kFaultCopyDrainTimeout);
       }
     } else {
       warpgroup_take_registers<kSoftmaxRegisters>();
-      if (work) {
-        // Softmax of tile t; this thread's row is r = token (in the tile) * group + head.
-        const int t = warp >> 2;
+      // Softmax of tile t; this thread's row is r = token (in the tile) * group + head.
+      const int t = warp >> 2;
+      const auto row = [&] {  // of the tile; computed anew where it is used, so that it takes no registers between
+          uint32_t tid;
+          asm volatile("mov.u32 %0, %%tid.x;" : "=r"(tid));
+          return static_cast<int>(tid) % kTileRows;
+      };
+      const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
+      const uint32_t s_tmem = tmem + lanes + kTmemScores + 128 * t, o_tmem = tmem + lanes + kTmemOutput + 128 * t;
+      bool ok = true;
+      for (int n = 0;; ++n) {
+        const volatile TileItem& item = items[n % kTileItems];
+        ok = mbar_poll_bounded(item_full + 8 * (n % kTileItems), (n / kTileItems) & 1, abort, kFaultFullBarrierTimeout);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok || item.work == 0) break;
         if (t < item.tiles) {
-            const int r = (warp & 3) * kWarpSize + lane;
-            const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
-            const uint32_t s_tmem = tmem + lanes + kTmemScores + 128 * t, o_tmem = tmem + lanes + kTmemOutput + 128 * t;
-            const int in_tile = r / a.group;
-            const int token = min(item.token0 + t * p.tile_tokens + in_tile, item.new_tokens - 1);
-            const bool real = in_tile < p.tile_tokens && item.token0 + t * p.tile_tokens + in_tile < item.new_tokens;
-            const int position = item.true_len - item.new_tokens + token;
+            const int in_pair = t * p.tile_tokens + row() / a.group;  // token of the pair
+            const bool padding = row() / a.group >= p.tile_tokens || in_pair >= item.tokens;
+            const int position = item.position + min(in_pair, item.tokens - 1);
             const int see_first = position >= a.window ? position - a.window + 1 : 0;
             const int see_stop = min(position + 1, item.len);
-            float top = -INFINITY, sum = 0.0f;
-            bool ok = true;
+            // A row of padding holds anything; its reference point never moves.
+            float top = padding ? INFINITY : -INFINITY, sum = 0.0f;
             for (int step = 0; step < item.steps; ++step) {
-                ok = mbar_wait_bounded(s_full + 8 * t, step & 1, abort, kFaultFullBarrierTimeout);
+                const int key0 = item.key0 + step * kTileKeys;
+                const int begin = see_first - key0, end = see_stop - key0;
+                const bool edge = __any_sync(0xffffffffu, begin > 0 || end < kTileKeys);
+                const bool hole = t == 0 && (key0 < item.first || key0 + kTileKeys > item.len);
+                ok = mbar_poll_bounded(s_full + 8 * t, (item.tile_steps[t] + step) & 1, abort, kFaultFullBarrierTimeout);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tcgen05_fence_after();
+                // The second half arrives while the first one is searched.
                 float s[4][32];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_load_32(s_tmem + 32 * c, s[c]);
-                const int key0 = item.key0 + step * kTileKeys;
-                const int begin = see_first - key0, end = see_stop - key0;
-                const uint32_t mask = block_masks[step % 8];
-                const bool partial = begin > 0 || end < kTileKeys || mask != (1u << kTileBoxes) - 1u;
+                tmem_load_32(s_tmem, s[0]);
+                tmem_load_32(s_tmem + 32, s[1]);
+                const uint32_t mask = block_masks[(item.loads / 2 + step) % 8];
+                const bool partial = edge || mask != kAllBlocks;
                 tmem_wait_loads();
-                const bool any_partial = __any_sync(0xffffffffu, partial);
-                if (any_partial) {
+                tmem_load_32(s_tmem + 64, s[2]);
+                tmem_load_32(s_tmem + 96, s[3]);
+                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
+                for (int h = 0; h < 2; ++h) {
+                    if (h == 1) tmem_wait_loads();
+                    if (partial) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const int key = 32 * c + i;
-                            if (key < begin || key >= end || !(mask >> (key / kAttentionBlock) & 1u)) s[c][i] = -INFINITY;
+                        for (int i = 0; i < 64; ++i) {
+                            const int key = 64 * h + i;
+                            if (key < begin || key >= end || !(mask >> (key / kAttentionBlock) & 1u)) s[2 * h + i / 32][i % 32] = -INFINITY;
                         }
                     }
-                }
-                float m4[4];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    m4[c] = s[c][0];
-#pragma unroll
-                    for (int i = 1; i < 31; i += 2) m4[c] = max3(m4[c], s[c][i], s[c][i + 1]);
-                    m4[c] = max3(m4[c], s[c][31], s[c][31]);
+                    for (int i = 0; i < 64; i += 2) {
+                        float& m = m4[(i / 2) % 4];
+                        m = max3(m, s[2 * h + i / 32][i % 32], s[2 * h + i / 32][i % 32 + 1]);
+                    }
                 }
                 const float m = max3(max3(m4[0], m4[1], m4[2]), m4[3], m4[3]) * a.scale_log2;
                 // Move the reference point when it is left behind by more than 2^8, and to NaN if a score is.
-                const bool move = real && !(m <= top + 8.0f);
+                const bool move = top < INFINITY && !(m <= top + 8.0f);
                 if (__any_sync(0xffffffffu, move)) {
                     const float keep = move ? exp2_approx(top - m) : 1.0f;
                     if (move) {
@@ -410,14 +590,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     }
                 }
                 const float shift = top == -INFINITY ? 0.0f : top;
-                if (t == 0 && (key0 < item.first || key0 + kTileKeys > item.len || mask != (1u << kTileBoxes) - 1u)) {
+                if (hole || (t == 0 && mask != kAllBlocks)) {
                     // Value rows that no token sees may hold anything, NaN included: they become zeros before
                     // the product, which would carry a NaN into every row.
-                    const int load = 2 * step + 1, stage = load % L::kStages;
-                    ok = mbar_wait_bounded(stage_full + 8 * stage, (load / L::kStages) & 1, abort, kFaultFullBarrierTimeout);
+                    const int load = item.loads + 2 * step + 1, stage = load % L::kStages;
+                    ok = mbar_poll_bounded(stage_full + 8 * stage, (load / L::kStages) & 1, abort, kFaultFullBarrierTimeout);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
-                    const int key = key0 + r;
+                    const int r = row(), key = key0 + r;
                     if (key < item.first || key >= item.len || !(mask >> (r / kAttentionBlock) & 1u)) {
                         const uint32_t row = smem + L::kStageBase + stage * L::kTileBytes + r * 128u;
 #pragma unroll
@@ -433,15 +613,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     uint32_t w[16];
-                    if (any_partial) tile_weights<0>(s[c], scale, minus_shift, w, sums);
+                    if (partial) tile_weights<0>(s[c], scale, minus_shift, w, sums);
                     else tile_weights<kTilePolynomial>(s[c], scale, minus_shift, w, sums);
                     tmem_store_16(s_tmem + 16 * c, w);
-                    if (c & 1) {
-                        // Half of the weights are there: their product can begin.
+                    if (c >= kTileHeadKeys / 32 - 1) {
+                        // The weights of the first keys are there: their product can begin.
                         tmem_wait_stores();
                         tcgen05_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(p_ready + 16 * t + 8 * (c >> 1));
+                        if (lane == 0) mbar_arrive(p_ready + 16 * t + 8 * (c - (kTileHeadKeys / 32 - 1)));
                     }
                 }
                 float parts[4];
@@ -450,40 +630,101 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 sum += (parts[0] + parts[1]) + (parts[2] + parts[3]);
             }
             if (ok && item.steps > 0) {
-                ok = mbar_wait_bounded(o_full + 8 * t, 0, abort, kFaultFullBarrierTimeout);
+                ok = mbar_poll_bounded(o_full + 8 * t, item.tile_items[t] & 1, abort, kFaultFullBarrierTimeout);
                 ok = __all_sync(0xffffffffu, ok);
                 tcgen05_fence_after();
             }
-            if (ok) {
-                const float inverse = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-                const int head = item.kv_head * a.group + r - in_tile * a.group;
-                uint16_t* out = a.out + static_cast<int64_t>(item.begin + token) * a.out_token + head * a.out_head;
+            if (!ok) break;
+            const float inverse = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+            const int r = row(), in_tile = r / a.group;
+            const bool real = in_tile < p.tile_tokens && t * p.tile_tokens + in_tile < item.tokens;
+            const int head = item.kv_head * a.group + r - in_tile * a.group;
+            const int token = item.token + t * p.tile_tokens + in_tile;
+            uint16_t* out = a.out + static_cast<int64_t>(token) * a.out_token + head * a.out_head;
+            const int slot = item.slot;
+            const int64_t part = static_cast<int64_t>(slot) * (2 * kTileRows) + t * kTileRows + r;
+            if (slot >= 0 && real) p.part_stats[part] = make_float2(top, sum);
 #pragma unroll
-                for (int c = 0; c < kDim / 32; ++c) {
-                    float o[32] = {};
-                    if (item.steps > 0) {
-                        tmem_load_32(o_tmem + 32 * c, o);
-                        tmem_wait_loads();
-                    }
-                    if (!real) continue;
+            for (int c = 0; c < kDim / 32; ++c) {
+                float o[32] = {};
+                if (item.steps > 0) {
+                    tmem_load_32(o_tmem + 32 * c, o);
+                    tmem_wait_loads();
+                }
+                if (!real) continue;
+                if (slot >= 0) {
+                    float4* to = reinterpret_cast<float4*>(p.part_sums + part * kDim + 32 * c);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (32 * c + 8 * i >= a.dim) break;
-                        U32x4 v;
+                    for (int i = 0; i < 8; ++i) to[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    continue;
+                }
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) v.v[j] = pack_bf16x2(o[8 * i + 2 * j] * inverse, o[8 * i + 2 * j + 1] * inverse);
-                        st_v4(out + 32 * c + 8 * i, v);
-                    }
+                for (int i = 0; i < 4; ++i) {
+                    if (32 * c + 8 * i >= a.dim) break;
+                    U32x4 v;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v.v[j] = pack_bf16x2(o[8 * i + 2 * j] * inverse, o[8 * i + 2 * j + 1] * inverse);
+                    st_v4(out + 32 * c + 8 * i, v);
                 }
             }
-            tmem_wait_stores();
         }
-    }
+        // The output has been read before the next item's first product overwrites it: that waits for weights
+        // which these threads write later.
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(item_empty + 8 * (n % kTileItems));
+      }
+      tmem_wait_stores();
     }
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
     if (warp == 8) tmem_free(tmem);
+}
+
+// Adds the parts of pairs that several CTAs of the tile kernel shared: block (c, y) takes 8 rows, one a warp, of
+// the pair whose first steps are in slot 2 c + 1; the others' follow in slots 2 (c + 1), 2 (c + 2), ...
+constexpr int kTileJoinWarps = 8;
+
+template <int kDim>
+__global__ void __launch_bounds__(kTileJoinWarps * kWarpSize) attention_tile_join_kernel(const TileParams p) {
+    grid_dependency_wait();
+    grid_launch_dependents();
+    constexpr int kMine = kDim / kWarpSize;
+    const int first = 2 * blockIdx.x + 1, ctas = gridDim.x;
+    const TilePart part = p.parts[first];
+    const int warp = threadIdx.x / kWarpSize, lane = threadIdx.x % kWarpSize;
+    const int row = blockIdx.y * kTileJoinWarps + warp, t = row / kTileRows, r = row % kTileRows;
+    const int in_tile = r / p.a.group, token = t * p.tile_tokens + in_tile;
+    if (part.tiles <= t || in_tile >= p.tile_tokens || token >= part.tokens) return;
+    float m = -INFINITY, l = 0.0f, total[kMine] = {};
+    bool last = false;
+    for (int cta = blockIdx.x; cta < ctas && !last; ++cta) {
+        const int slot = cta == static_cast<int>(blockIdx.x) ? first : 2 * cta;
+        const int64_t at = static_cast<int64_t>(slot) * (2 * kTileRows) + row;
+        if (p.parts[slot].tiles == 0) continue;  // a CTA without a share
+        last = p.parts[slot].last != 0;
+        const float2 stats = p.part_stats[at];
+        float x[kMine];
+        const float* from = p.part_sums + at * kDim + lane * kMine;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) x[i] = from[i];
+        const float top = fmaxf(m, stats.x), shift = top == -INFINITY ? 0.0f : top;
+        const float keep = exp2_approx(m - shift), add = exp2_approx(stats.x - shift);
+        l = l * keep + stats.y * add;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) total[i] = total[i] * keep + x[i] * add;
+        m = top;
+    }
+    const float inverse = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    const int d = lane * kMine;
+    if (d >= p.a.dim) return;
+    const int head = part.kv_head * p.a.group + r - in_tile * p.a.group;
+    uint16_t* out = p.a.out + static_cast<int64_t>(part.token + token) * p.a.out_token + head * p.a.out_head + d;
+#pragma unroll
+    for (int i = 0; i < kMine; i += 2) {
+        *reinterpret_cast<uint32_t*>(out + i) = pack_bf16x2(total[i] * inverse, total[i + 1] * inverse);
+    }
 }
 
 }  // namespace ipl
