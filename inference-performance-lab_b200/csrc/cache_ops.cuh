@@ -323,9 +323,8 @@ ipl_status launch_short(const AttentionPlan& plan, const AttentionParams& p, cud
                                                         : launch(attention_short_kernel<kDim, 2>, ctas, kThreads, 0, stream, p),
                                         "paged attention");
     if (st != IPL_SUCCESS || plan.splits == 1) return st;
-    const int64_t rows = static_cast<int64_t>(p.num_tokens) * p.heads;
-    return launch_status(launch(attention_join_kernel<kDim>, static_cast<unsigned>((rows + kJoinWarps - 1) / kJoinWarps),
-                                kJoinWarps * kWarpSize, 0, stream, p),
+    return launch_status(launch(attention_join_kernel<kDim>, static_cast<unsigned>(p.num_seqs * p.kv_heads), kJoinWarps * kWarpSize,
+                                0, stream, p),
                          "paged attention");
 }
 

@@ -386,8 +386,9 @@ __global__ void __launch_bounds__(kShortWarps * kWarpSize, kTiles == 1 ? 3 : 2) 
     }
 }
 
-// Adds the parts of split rows: a warp for each (token, head), kDim / 32 elements a lane.
-constexpr int kJoinWarps = 4;
+// Adds the parts of split rows: a CTA for each sequence and key head, a warp for each row in turn, kDim / 32
+// elements a lane.
+constexpr int kJoinWarps = 8;
 
 template <int kDim>
 __global__ void __launch_bounds__(kJoinWarps * kWarpSize) attention_join_kernel(const AttentionParams p) {
@@ -395,13 +396,10 @@ __global__ void __launch_bounds__(kJoinWarps * kWarpSize) attention_join_kernel(
     grid_launch_dependents();
     constexpr int kMine = kDim / kWarpSize;
     const int lane = threadIdx.x % kWarpSize;
+    const int seq = blockIdx.x / p.kv_heads, kv_head = blockIdx.x - seq * p.kv_heads;
     const int64_t rows = static_cast<int64_t>(p.num_tokens) * p.heads;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * kJoinWarps + threadIdx.x / kWarpSize;
-    if (row >= rows) return;
-    const int token = static_cast<int>(row / p.heads), head = static_cast<int>(row % p.heads);
-    const int seq = sequence_of_token(p.starts, p.num_seqs, token);
     const int begin = p.starts[seq], new_tokens = min(p.starts[seq + 1], p.num_tokens) - begin;
-    if (token < begin || token >= begin + new_tokens || new_tokens * p.group > p.short_rows) return;
+    if (begin < 0 || new_tokens <= 0 || new_tokens * p.group > p.short_rows) return;
     const KeyRange range = visible_keys(p, p.lens[seq], new_tokens);
     const int first_block = range.first / kAttentionBlock;
     const int stop = min(range.stop, table_bounded_length(p, seq));
@@ -409,33 +407,37 @@ __global__ void __launch_bounds__(kJoinWarps * kWarpSize) attention_join_kernel(
     const int split_blocks = p.split_len / kAttentionBlock;
     const int used = min(p.splits, max(1, (blocks + split_blocks - 1) / split_blocks));
     if (used == 1) return;  // written already
-    float m = -INFINITY;
-    for (int s = lane; s < used; s += kWarpSize) m = fmaxf(m, p.part_stats[s * rows + row].x);
-    m = warp_max(m);
-    const float shift = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f, total[kMine] = {};
+    for (int mine = threadIdx.x / kWarpSize; mine < new_tokens * p.group; mine += kJoinWarps) {
+        const int token = begin + mine / p.group, head = kv_head * p.group + mine % p.group;
+        const int64_t row = static_cast<int64_t>(token) * p.heads + head;
+        float m = -INFINITY;
+        for (int s = lane; s < used; s += kWarpSize) m = fmaxf(m, p.part_stats[s * rows + row].x);
+        m = warp_max(m);
+        const float shift = m == -INFINITY ? 0.0f : m;
+        float l = 0.0f, total[kMine] = {};
 #pragma unroll 4
-    for (int s = 0; s < used; ++s) {
-        const float2 part = p.part_stats[s * rows + row];
-        const float f = exp2_approx(part.x - shift);
-        l += f * part.y;
-        const float* x = p.part_sums + (s * rows + row) * kDim + lane * kMine;
-        if constexpr (kMine == 4) {
-            const float4 y = *reinterpret_cast<const float4*>(x);
-            total[0] += f * y.x, total[1] += f * y.y, total[2] += f * y.z, total[3] += f * y.w;
-        } else {
-            const float2 y = *reinterpret_cast<const float2*>(x);
-            total[0] += f * y.x, total[1] += f * y.y;
+        for (int s = 0; s < used; ++s) {
+            const float2 part = p.part_stats[s * rows + row];
+            const float f = exp2_approx(part.x - shift);
+            l += f * part.y;
+            const float* x = p.part_sums + (s * rows + row) * kDim + lane * kMine;
+            if constexpr (kMine == 4) {
+                const float4 y = *reinterpret_cast<const float4*>(x);
+                total[0] += f * y.x, total[1] += f * y.y, total[2] += f * y.z, total[3] += f * y.w;
+            } else {
+                const float2 y = *reinterpret_cast<const float2*>(x);
+                total[0] += f * y.x, total[1] += f * y.y;
+            }
         }
-    }
-    const float inverse = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    const int d = lane * kMine;
-    if (d >= p.dim) return;
-    uint16_t* out = p.out + token * p.out_token + head * p.out_head + d;
-    if constexpr (kMine == 4) {
-        st_v2(out, pack_bf16x2(total[0] * inverse, total[1] * inverse), pack_bf16x2(total[2] * inverse, total[3] * inverse));
-    } else {
-        *reinterpret_cast<uint32_t*>(out) = pack_bf16x2(total[0] * inverse, total[1] * inverse);
+        const float inverse = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+        const int d = lane * kMine;
+        if (d >= p.dim) continue;
+        uint16_t* out = p.out + token * p.out_token + head * p.out_head + d;
+        if constexpr (kMine == 4) {
+            st_v2(out, pack_bf16x2(total[0] * inverse, total[1] * inverse), pack_bf16x2(total[2] * inverse, total[3] * inverse));
+        } else {
+            *reinterpret_cast<uint32_t*>(out) = pack_bf16x2(total[0] * inverse, total[1] * inverse);
+        }
     }
 }
 

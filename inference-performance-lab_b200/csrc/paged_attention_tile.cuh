@@ -36,7 +36,7 @@ constexpr int kTilePolynomial = 0;  // of 16 pairs of weights, by the polynomial
 constexpr int kTileBoxes = kTileKeys / kAttentionBlock;  // boxes of at least 16 keys a tile
 constexpr uint32_t kAllBlocks = (1u << kTileBoxes) - 1u;
 
-constexpr int kTilePairCost = 1;  // of a pair beside its steps (first scores, output), in steps
+constexpr int kTilePairCost = 2;  // of a pair beside its steps (first scores, output), in steps
 constexpr int kTileItems = 4;     // ring of work items
 
 struct TileParams {
@@ -241,7 +241,37 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     const int64_t all_weight = static_cast<int64_t>(head_weight) * a.kv_heads;
     const int64_t share_begin = all_weight * blockIdx.x / gridDim.x, share_end = all_weight * (blockIdx.x + 1) / gridDim.x;
     const int begin_head = head_weight > 0 ? static_cast<int>(share_begin / head_weight) : 0;
-    const int begin_weight = static_cast<int>(share_begin - static_cast<int64_t>(begin_head) * head_weight);
+    int begin_weight = static_cast<int>(share_begin - static_cast<int64_t>(begin_head) * head_weight);
+    // The pair the share begins in, and its weight before the share.
+    int* const found = scratch + kTileThreads / kWarpSize;
+    if (share_begin < share_end) {
+        for (int base = 0, before = 0; base < p.units; base += kTileThreads) {
+            const int w = weight(base + threadIdx.x);
+            int through = w;
+#pragma unroll
+            for (int offset = 1; offset < kWarpSize; offset *= 2) {
+                const int below = __shfl_up_sync(0xffffffffu, through, offset);
+                if (lane >= offset) through += below;
+            }
+            __syncthreads();
+            if (lane == kWarpSize - 1) scratch[warp] = through;
+            __syncthreads();
+            int total = before;
+            for (int i = 0; i < kTileThreads / kWarpSize; ++i) {
+                if (i == warp) through += total;
+                total += scratch[i];
+            }
+            if (begin_weight < through && begin_weight >= through - w) {
+                found[0] = base + threadIdx.x;
+                found[1] = begin_weight - (through - w);
+            }
+            before = total;
+            if (begin_weight < total) break;
+        }
+        __syncthreads();
+    }
+    const int begin_unit = found[0];
+    begin_weight = found[1];
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
@@ -270,11 +300,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             return ok;
         };
         int64_t left = share_end - share_begin;
-        int skip = begin_weight, head = begin_head;  // weight of this head's pairs before the share
+        int skip = begin_weight, head = begin_head;
         TileItem item = {};
         bool ok = true;
-        for (int base = 0; left > 0 && ok; base += kWarpSize) {
-            if (base >= p.units) base = 0, skip = 0, ++head;
+        for (int base = begin_unit; left > 0 && ok; base += kWarpSize) {
+            if (base >= p.units) base = 0, ++head;
             if (head >= a.kv_heads) break;
             TilePair pair = {};
             const bool exists = tile_pair(p, base + lane, pair);
@@ -697,24 +727,32 @@ __global__ void __launch_bounds__(kTileJoinWarps * kWarpSize) attention_tile_joi
     const int row = blockIdx.y * kTileJoinWarps + warp, t = row / kTileRows, r = row % kTileRows;
     const int in_tile = r / p.a.group, token = t * p.tile_tokens + in_tile;
     if (part.tiles <= t || in_tile >= p.tile_tokens || token >= part.tokens) return;
+    // The slots of the pair, 32 CTAs at a time, one a lane: those with a share, up to the pair's last steps.
     float m = -INFINITY, l = 0.0f, total[kMine] = {};
-    bool last = false;
-    for (int cta = blockIdx.x; cta < ctas && !last; ++cta) {
-        const int slot = cta == static_cast<int>(blockIdx.x) ? first : 2 * cta;
-        const int64_t at = static_cast<int64_t>(slot) * (2 * kTileRows) + row;
-        if (p.parts[slot].tiles == 0) continue;  // a CTA without a share
-        last = p.parts[slot].last != 0;
-        const float2 stats = p.part_stats[at];
-        float x[kMine];
-        const float* from = p.part_sums + at * kDim + lane * kMine;
-#pragma unroll
-        for (int i = 0; i < kMine; ++i) x[i] = from[i];
-        const float top = fmaxf(m, stats.x), shift = top == -INFINITY ? 0.0f : top;
+    for (int base = blockIdx.x; base < ctas; base += kWarpSize) {
+        const int slot = base + lane == static_cast<int>(blockIdx.x) ? first : 2 * (base + lane);
+        const bool there = base + lane < ctas && p.parts[slot].tiles != 0;
+        const uint32_t ends = __ballot_sync(0xffffffffu, there && p.parts[slot].last != 0);
+        const bool mine = there && (ends == 0 || lane < __ffs(ends));
+        const float2 stats = mine ? p.part_stats[static_cast<int64_t>(slot) * (2 * kTileRows) + row] : make_float2(-INFINITY, 0.0f);
+        const float top = fmaxf(m, warp_max(stats.x)), shift = top == -INFINITY ? 0.0f : top;
         const float keep = exp2_approx(m - shift), add = exp2_approx(stats.x - shift);
-        l = l * keep + stats.y * add;
+        l = l * keep + warp_sum(stats.y * add);
 #pragma unroll
-        for (int i = 0; i < kMine; ++i) total[i] = total[i] * keep + x[i] * add;
+        for (int i = 0; i < kMine; ++i) total[i] *= keep;
+        const uint32_t set = __ballot_sync(0xffffffffu, mine);
+        const int count = 32 - __clz(set);
+#pragma unroll 8
+        for (int j = 0; j < count; ++j) {
+            const float f = __shfl_sync(0xffffffffu, add, j);
+            if (!(set >> j & 1u)) continue;
+            const int from = __shfl_sync(0xffffffffu, slot, j);
+            const float* x = p.part_sums + (static_cast<int64_t>(from) * (2 * kTileRows) + row) * kDim + lane * kMine;
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) total[i] += x[i] * f;
+        }
         m = top;
+        if (ends != 0) break;
     }
     const float inverse = l > 0.0f || l != l ? 1.0f / l : 0.0f;
     const int d = lane * kMine;
