@@ -345,6 +345,9 @@ ipl_status launch_tile(const ipl_paged_attention_args& a, const AttentionPlan& p
     t.box_keys = kAttentionBlock;
     while (t.box_keys < kTileKeys && p.page_size % (2 * t.box_keys) == 0) t.box_keys *= 2;
     t.units = p.num_tokens / (2 * t.tile_tokens) + p.num_seqs;
+    t.pair_tokens = make_fast_div32(static_cast<uint32_t>(2 * t.tile_tokens));
+    t.page_size = make_fast_div32(static_cast<uint32_t>(p.page_size));
+    t.group_reciprocal = 65536 / p.group + 1;
     const size_t rows = static_cast<size_t>(plan.tile_ctas) * 2 * 2 * kTileRows;
     t.part_sums = static_cast<float*>(a.workspace);
     t.part_stats = reinterpret_cast<float2*>(t.part_sums + rows * kDim);

@@ -255,17 +255,17 @@ __device__ __forceinline__ bool mbar_poll(uint32_t bar, uint32_t parity) {
 }
 // mbar_wait_bounded by mbar_poll.
 __device__ __forceinline__ bool mbar_poll_bounded(uint32_t bar, uint32_t parity, volatile int* abort, uint32_t fault_bit) {
-    if (mbar_poll(bar, parity)) return true;
-    const uint64_t start = global_timer_ns();
-    for (;;) {
-        if (mbar_poll(bar, parity)) return true;
-        if (*abort) return false;
-        if (global_timer_ns() - start > kWaitLimitNs) {
-            atomicOr(&g_fault_word, fault_bit);
-            *abort = 1;
-            return false;
-        }
+    bool done = mbar_poll(bar, parity), late = false;
+    const uint64_t start = done ? 0 : global_timer_ns();
+    while (!done && !late) {
+        done = mbar_poll(bar, parity);
+        late = !done && (*abort != 0 || global_timer_ns() - start > kWaitLimitNs);
     }
+    if (late && *abort == 0) {
+        atomicOr(&g_fault_word, fault_bit);
+        *abort = 1;
+    }
+    return done;
 }
 
 // Waits for the phase with the given parity to complete. Returns false (after recording

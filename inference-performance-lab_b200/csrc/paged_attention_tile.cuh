@@ -21,6 +21,7 @@
 #pragma once
 
 #include "paged_attention.cuh"
+#include "silu_and_mul.cuh"
 #include "tensor_core.cuh"
 
 namespace ipl {
@@ -42,6 +43,8 @@ constexpr int kTileItems = 4;     // ring of work items
 struct TileParams {
     AttentionParams a;
     int tile_tokens;  // tokens a tile: 128 / group
+    FastDiv32 pair_tokens, page_size;
+    int group_reciprocal;  // 65536 / group + 1: row / group of a row below 128 is the product's high half
     int box_keys;     // keys a TMA box: the largest power of two up to 128 that divides the page size
     int units;        // upper bound of the tile pairs of all sequences
     // Parts of pairs that several CTAs share. CTA c leaves at most two: in slot 2 c the last steps (or a middle
@@ -100,6 +103,36 @@ __device__ __forceinline__ F32x2 exp2_pair_polynomial(F32x2 x) {
                       __uint_as_float(__float_as_uint(b) + (__float_as_uint(nb) << 23)));
 }
 
+// The lowest n bits (none for n <= 0, all from 32 on).
+__device__ __forceinline__ uint32_t bits_below(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
+
+// Bit 31 - i: key 32 c + i of a step is seen, one from `begin` to `end` whose block's page is there.
+__device__ __forceinline__ uint32_t seen_bits(int c, int begin, int end, uint32_t blocks) {
+    const uint32_t there = (blocks >> (2 * c) & 1u ? 0x0000ffffu : 0u) | (blocks >> (2 * c) & 2u ? 0xffff0000u : 0u);
+    return __brev(there & bits_below(end - 32 * c) & ~bits_below(begin - 32 * c));
+}
+
+// Eight threads of adjacent rows hold eight chunks of 16 bytes of their rows each; afterwards thread j holds chunk
+// j of row k in v[4 k] and on, so that a store of the warp writes 128 bytes of each of four rows. (Every thread
+// storing its own row, 16 or 32 bytes a row and instruction, took 4000-6000 cycles a tile of 128 x 128.)
+__device__ __forceinline__ void transpose_chunks(uint32_t (&v)[32], int lane) {
+#pragma unroll
+    for (int s = 4; s > 0; s /= 2) {
+        const bool upper = lane & s;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (i & s) continue;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                uint32_t &low = v[4 * i + w], &high = v[4 * (i + s) + w];
+                const uint32_t got = __shfl_xor_sync(0xffffffffu, upper ? low : high, s);
+                low = upper ? got : low;
+                high = upper ? high : got;
+            }
+        }
+    }
+}
+
 // The largest of three, NaN if one is.
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float m;
@@ -155,11 +188,12 @@ __device__ __forceinline__ bool tile_pair(const TileParams& p, int u, TilePair& 
     int lo = 0, hi = a.num_seqs - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (a.starts[mid] / pair_tokens + mid <= u) lo = mid;
+        // starts[mid] / pair_tokens + mid <= u
+        if (a.starts[mid] < static_cast<int64_t>(u - mid + 1) * pair_tokens) lo = mid;
         else hi = mid - 1;
     }
     const int begin = a.starts[lo], new_tokens = min(a.starts[lo + 1], a.num_tokens) - begin;
-    const int token0 = (u - (begin / pair_tokens + lo)) * pair_tokens;
+    const int token0 = (u - (static_cast<int>(fast_div(static_cast<uint32_t>(max(begin, 0)), p.pair_tokens)) + lo)) * pair_tokens;
     if (u >= p.units || begin < 0 || token0 < 0 || token0 >= new_tokens || new_tokens * a.group <= a.short_rows) return false;
     pair.seq = lo;
     pair.token = begin + token0;
@@ -227,6 +261,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     // This CTA's share of the steps: of the pairs of one key head in their order, then of the next head. The
     // items' memory serves the sums. Pair u weighs its steps and kTilePairCost.
     int* const scratch = reinterpret_cast<int*>(at(smem + L::kItemBase));
+    if (threadIdx.x < a.num_seqs) {
+        // The searches below go through these one load after the other: bring them near at once.
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(a.starts + threadIdx.x));
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(a.lens + threadIdx.x));
+    }
     const auto weight = [&](int u) {
         TilePair pair;
         return u < p.units && tile_pair(p, u, pair) ? pair.steps + kTilePairCost : 0;
@@ -361,21 +400,44 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
         const uint32_t q_bytes = L::kHalves * static_cast<uint32_t>(p.tile_tokens) * a.group * 128u;
         bool ok = true;
         int loads = 0, q_loads = 0, tile_loads[2] = {0, 0};
+        const auto load_q = [&](const volatile TileItem& item) {
+            bool free = mbar_poll_bounded(q_empty, (q_loads & 1) ^ 1, abort, kFaultEmptyBarrierTimeout);
+            free = __all_sync(0xffffffffu, free);
+            if (!free) return false;
+            ++q_loads;
+            const int tiles = item.tiles, head = item.kv_head * a.group, token = item.token;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                if (t >= tiles) break;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(q_full + 8 * t, q_bytes);
+                    for (int h = 0; h < L::kHalves; ++h) {
+                        tma_load_3d(smem + t * L::kTileBytes + h * L::kHalfBytes, &q_map, 64 * h, head, token + t * p.tile_tokens,
+                                    q_full + 8 * t);
+                    }
+                }
+                ++tile_loads[t];
+            }
+            __syncwarp();
+            return true;
+        };
         for (int n = 0;; ++n) {
             const volatile TileItem& item = items[n % kTileItems];
             ok = ok && mbar_poll_bounded(item_full + 8 * (n % kTileItems), (n / kTileItems) & 1, abort, kFaultFullBarrierTimeout);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok || item.work == 0) break;
             const int32_t* table = a.tables + item.seq * a.table_row;
-            const int len = item.len, first = item.first, steps = item.steps, kv_head = item.kv_head, tiles = item.tiles;
+            const int len = item.len, first = item.first, steps = item.steps, kv_head = item.kv_head;
+            if (n == 0 && steps > 0) ok = load_q(item);
             for (int step = 0; step < steps && ok; ++step) {
                 const int key0 = item.key0 + step * kTileKeys;
                 const int box = lane % boxes, half = lane / boxes;
                 const int key = key0 + box * p.box_keys;
                 int page = -1;
+                const int key_page = static_cast<int>(fast_div(static_cast<uint32_t>(key), p.page_size));
                 const bool wanted = key < len && key + p.box_keys > first;
                 if (wanted) {
-                    page = table[key / a.page_size];
+                    page = table[key_page];
                     if (page < 0 || page >= a.num_pages) {
                         atomicOr(&g_fault_word, kFaultIndexOutOfRange);
                         page = -1;
@@ -387,7 +449,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 mask = ~__reduce_or_sync(0xffffffffu, mask) & kAllBlocks;
                 const uint32_t count = __popc(__ballot_sync(0xffffffffu, page >= 0 && lane < boxes)) * L::kHalves;
                 if (lane == 0) block_masks[(loads / 2) % 8] = mask;
-                const int in_page = key % a.page_size;
+                const int in_page = key - key_page * a.page_size;
                 for (int which = 0; which < 2; ++which, ++loads) {
                     const int stage = loads % L::kStages;
                     ok = mbar_poll_bounded(stage_empty + 8 * stage, ((loads / L::kStages) & 1) ^ 1, abort, kFaultEmptyBarrierTimeout);
@@ -400,28 +462,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                         const uint32_t dst = smem + L::kStageBase + stage * L::kTileBytes + half * L::kHalfBytes + box * box_bytes;
                         tma_load_4d(dst, which == 0 ? &k_map : &v_map, 64 * half, kv_head, in_page, page, full);
                     }
-                    if (step == 0 && which == 0) {
-                        // Q behind the first keys, once the scores of the item before are done with its place.
-                        ok = mbar_poll_bounded(q_empty, (q_loads & 1) ^ 1, abort, kFaultEmptyBarrierTimeout);
-                        ok = __all_sync(0xffffffffu, ok);
+                    if (step == 0 && which == 0 && n > 0) {
+                        // Q behind the first keys: its place is free when the item before is done with its scores.
+                        ok = load_q(item);
                         if (!ok) {
                             ++loads;
                             break;
                         }
-                        ++q_loads;
-#pragma unroll
-                        for (int t = 0; t < 2; ++t) {
-                            if (t >= tiles) break;
-                            if (lane == 0) {
-                                mbar_arrive_expect_tx(q_full + 8 * t, q_bytes);
-                                for (int h = 0; h < L::kHalves; ++h) {
-                                    tma_load_3d(smem + t * L::kTileBytes + h * L::kHalfBytes, &q_map, 64 * h, kv_head * a.group,
-                                                item.token + t * p.tile_tokens, q_full + 8 * t);
-                                }
-                            }
-                            ++tile_loads[t];
-                        }
-                        __syncwarp();
                     }
                 }
             }
@@ -547,6 +594,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
           asm volatile("mov.u32 %0, %%tid.x;" : "=r"(tid));
           return static_cast<int>(tid) % kTileRows;
       };
+      const auto row_token = [&](int r) { return r * p.group_reciprocal >> 16; };
       const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
       const uint32_t s_tmem = tmem + lanes + kTmemScores + 128 * t, o_tmem = tmem + lanes + kTmemOutput + 128 * t;
       bool ok = true;
@@ -556,18 +604,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
         ok = __all_sync(0xffffffffu, ok);
         if (!ok || item.work == 0) break;
         if (t < item.tiles) {
-            const int in_pair = t * p.tile_tokens + row() / a.group;  // token of the pair
-            const bool padding = row() / a.group >= p.tile_tokens || in_pair >= item.tokens;
-            const int position = item.position + min(in_pair, item.tokens - 1);
+            const int tokens = item.tokens, row_in_tile = row_token(row()), in_pair = t * p.tile_tokens + row_in_tile;
+            const bool padding = row_in_tile >= p.tile_tokens || in_pair >= tokens;
+            const int position = item.position + min(in_pair, tokens - 1);
             const int see_first = position >= a.window ? position - a.window + 1 : 0;
             const int see_stop = min(position + 1, item.len);
             // A row of padding holds anything; its reference point never moves.
             float top = padding ? INFINITY : -INFINITY, sum = 0.0f;
             for (int step = 0; step < item.steps; ++step) {
-                const int key0 = item.key0 + step * kTileKeys;
-                const int begin = see_first - key0, end = see_stop - key0;
-                const bool edge = __any_sync(0xffffffffu, begin > 0 || end < kTileKeys);
-                const bool hole = t == 0 && (key0 < item.first || key0 + kTileKeys > item.len);
+                const auto key0 = [&] { return item.key0 + step * kTileKeys; };
+                const bool edge = __any_sync(0xffffffffu, see_first > key0() || see_stop < key0() + kTileKeys);
+                const bool hole = t == 0 && (key0() < item.first || key0() + kTileKeys > item.len);
                 ok = mbar_poll_bounded(s_full + 8 * t, (item.tile_steps[t] + step) & 1, abort, kFaultFullBarrierTimeout);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
@@ -581,17 +628,24 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 tmem_wait_loads();
                 tmem_load_32(s_tmem + 64, s[2]);
                 tmem_load_32(s_tmem + 96, s[3]);
+                if (partial) {
+                    tmem_wait_loads();
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t seen = seen_bits(c, see_first - key0(), see_stop - key0(), mask);
+                        // Shifted along, so that each test is of the same bit.
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const uint32_t keep = static_cast<uint32_t>(static_cast<int>(seen) >> 31);
+                            s[c][i] = __uint_as_float((__float_as_uint(s[c][i]) & keep) | (0xff800000u & ~keep));
+                            seen += seen;
+                        }
+                    }
+                }
                 float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     if (h == 1) tmem_wait_loads();
-                    if (partial) {
-#pragma unroll
-                        for (int i = 0; i < 64; ++i) {
-                            const int key = 64 * h + i;
-                            if (key < begin || key >= end || !(mask >> (key / kAttentionBlock) & 1u)) s[2 * h + i / 32][i % 32] = -INFINITY;
-                        }
-                    }
 #pragma unroll
                     for (int i = 0; i < 64; i += 2) {
                         float& m = m4[(i / 2) % 4];
@@ -609,13 +663,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     }
                     if (step > 0) {
 #pragma unroll
-                        for (int c = 0; c < kDim / 32; ++c) {
-                            float o[32];
-                            tmem_load_32(o_tmem + 32 * c, o);
+                        for (int c = 0; c < kDim / 16; ++c) {
+                            uint32_t o[16];
+                            tmem_load_16(o_tmem + 16 * c, o);
                             tmem_wait_loads();
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] *= keep;
-                            tmem_store_32(o_tmem + 32 * c, o);
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+                            tmem_store_16(o_tmem + 16 * c, o);
                         }
                     }
                 }
@@ -627,13 +681,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     ok = mbar_poll_bounded(stage_full + 8 * stage, (load / L::kStages) & 1, abort, kFaultFullBarrierTimeout);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
-                    const int r = row(), key = key0 + r;
+                    const int r = row(), key = key0() + r;
                     if (key < item.first || key >= item.len || !(mask >> (r / kAttentionBlock) & 1u)) {
                         const uint32_t row = smem + L::kStageBase + stage * L::kTileBytes + r * 128u;
 #pragma unroll
                         for (int h = 0; h < L::kHalves; ++h) {
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) sts_pairs(row + h * L::kHalfBytes + 16u * i, 0ull, 0ull);
+                            for (int i = 0; i < 8; ++i) sts_pairs(row + h * L::kHalfBytes + 16u * ((i + r) % 8), 0ull, 0ull);
                         }
                     }
                     fence_async_shared();
@@ -666,35 +720,48 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             }
             if (!ok) break;
             const float inverse = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-            const int r = row(), in_tile = r / a.group;
-            const bool real = in_tile < p.tile_tokens && t * p.tile_tokens + in_tile < item.tokens;
-            const int head = item.kv_head * a.group + r - in_tile * a.group;
-            const int token = item.token + t * p.tile_tokens + in_tile;
-            uint16_t* out = a.out + static_cast<int64_t>(token) * a.out_token + head * a.out_head;
+            const int r = row(), in_tile = row_token(r);
+            const uint32_t real = __ballot_sync(0xffffffffu, in_tile < p.tile_tokens && t * p.tile_tokens + in_tile < item.tokens);
             const int slot = item.slot;
             const int64_t part = static_cast<int64_t>(slot) * (2 * kTileRows) + t * kTileRows + r;
-            if (slot >= 0 && real) p.part_stats[part] = make_float2(top, sum);
+            if (slot >= 0) p.part_stats[part] = make_float2(top, sum);
+            // Bytes of this thread's row; the rows of the eight threads that share their rows' chunks.
+            const int64_t mine = slot >= 0 ? part * (kDim * 4)
+                                           : 2 * (static_cast<int64_t>(item.token + t * p.tile_tokens + in_tile) * a.out_token +
+                                                  (item.kv_head * a.group + r - in_tile * a.group) * a.out_head);
+            char* const to = (slot >= 0 ? reinterpret_cast<char*>(p.part_sums) : reinterpret_cast<char*>(a.out)) + 16 * (lane & 7);
+            const int columns = slot >= 0 ? 32 : 64;  // of a pass: 128 bytes a row
+            for (int c = 0; c < kDim; c += columns) {
+                uint32_t v[32];
+                if (item.steps == 0) {
 #pragma unroll
-            for (int c = 0; c < kDim / 32; ++c) {
-                float o[32] = {};
-                if (item.steps > 0) {
-                    tmem_load_32(o_tmem + 32 * c, o);
+                    for (int i = 0; i < 32; ++i) v[i] = 0;
+                } else {
+                    tmem_load_32(o_tmem + c, reinterpret_cast<float(&)[32]>(v));
                     tmem_wait_loads();
+                    if (slot < 0) {
+                        uint32_t high[32];
+                        tmem_load_32(o_tmem + c + 32, reinterpret_cast<float(&)[32]>(high));
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            v[i] = pack_bf16x2(__uint_as_float(v[2 * i]) * inverse, __uint_as_float(v[2 * i + 1]) * inverse);
+                        }
+                        tmem_wait_loads();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            v[16 + i] = pack_bf16x2(__uint_as_float(high[2 * i]) * inverse, __uint_as_float(high[2 * i + 1]) * inverse);
+                        }
+                    }
                 }
-                if (!real) continue;
-                if (slot >= 0) {
-                    float4* to = reinterpret_cast<float4*>(p.part_sums + part * kDim + 32 * c);
+                transpose_chunks(v, lane);
+                const bool inside = slot >= 0 || c + 8 * (lane & 7) < a.dim;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) to[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-                    continue;
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (32 * c + 8 * i >= a.dim) break;
-                    U32x4 v;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) v.v[j] = pack_bf16x2(o[8 * i + 2 * j] * inverse, o[8 * i + 2 * j + 1] * inverse);
-                    st_v4(out + 32 * c + 8 * i, v);
+                for (int k = 0; k < 8; ++k) {
+                    const int from = (lane & 24) + k;
+                    const int64_t at = __shfl_sync(0xffffffffu, mine, from);
+                    if (inside && (slot >= 0 || (real >> from & 1u))) {
+                        st_v4(to + at + (slot >= 0 ? 4 : 2) * c, U32x4{v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]});
+                    }
                 }
             }
         }
