@@ -247,7 +247,7 @@ struct AttentionPlan {
     int short_rows = 0;
     int tile_ctas = 0;
     size_t tile_workspace = 0;  // at the beginning of the workspace; the short kernel's parts follow
-    int splits = 1, split_len = 0;
+    int splits = 1, split_len = 0, cluster = 1;
     size_t workspace = 0;
 };
 
@@ -284,19 +284,26 @@ AttentionPlan plan_attention(const ipl_paged_attention_args& a, int sm_count) {
             plan.short_rows = 0;
         }
     }
-    // Keys a CTA takes: about a quarter of what fills the GPU once, so that ragged lengths even out,
-    // but a block for each of its warps at the least.
+    // CTAs a sequence and key head: enough to fill the GPU about four times over, so that ragged lengths even
+    // out, but a block of keys for each warp at the least; a cluster of up to 8 of them, and several clusters
+    // where that is not half of what the GPU holds.
     int64_t keys = a.max_seq_len > 1 ? a.max_seq_len : 1;
     if (a.window > 0 && a.window + a.max_query_len < keys) keys = a.window + a.max_query_len;
     const int64_t pairs = a.num_seqs * a.num_kv_heads;
     const int64_t resident = static_cast<int64_t>(sm_count) * (plan.tiles == 1 ? 3 : 2);
     constexpr int64_t kLeast = kShortWarps * kAttentionBlock;
-    int64_t len = round_up(pairs * keys / (resident * 4) + 1, kLeast);
-    int64_t splits = (keys + len - 1) / len;
-    if (splits > 256) {
-        len = round_up((keys + 255) / 256, kLeast);
-        splits = (keys + len - 1) / len;
+    const int64_t most = (keys + kLeast - 1) / kLeast;
+    int64_t wanted = (resident * 4 + pairs - 1) / pairs;
+    if (wanted > most) wanted = most;
+    plan.cluster = 1;
+    while (plan.cluster < kShortCluster && plan.cluster < wanted) plan.cluster *= 2;
+    int64_t splits = 1;
+    if (pairs * plan.cluster * 2 < resident && wanted > plan.cluster) {
+        splits = (resident + pairs * plan.cluster - 1) / (pairs * plan.cluster);
+        if (splits > wanted / plan.cluster) splits = wanted / plan.cluster;
     }
+    const int64_t len = round_up((keys + splits - 1) / splits, kAttentionBlock);
+    splits = (keys + len - 1) / len;
     plan.split_len = static_cast<int>(len);
     plan.splits = static_cast<int>(splits);
     if (plan.tiles == 0) plan.splits = 1;
@@ -315,13 +322,14 @@ AttentionPlan plan_attention(const ipl_paged_attention_args& a, int sm_count) {
 
 template <int kDim>
 ipl_status launch_short(const AttentionPlan& plan, const AttentionParams& p, cudaStream_t stream) {
-    const int64_t grid = static_cast<int64_t>(p.num_seqs) * p.kv_heads * plan.splits;
+    const int64_t grid = static_cast<int64_t>(p.num_seqs) * p.kv_heads * plan.splits * plan.cluster;
     if (grid > INT_MAX) return fail(IPL_ERROR_TOO_LARGE, "too many sequences and heads");
     constexpr unsigned kThreads = kShortWarps * kWarpSize;
-    const unsigned ctas = static_cast<unsigned>(grid);
-    const ipl_status st = launch_status(plan.tiles == 1 ? launch(attention_short_kernel<kDim, 1>, ctas, kThreads, 0, stream, p)
-                                                        : launch(attention_short_kernel<kDim, 2>, ctas, kThreads, 0, stream, p),
-                                        "paged attention");
+    const unsigned ctas = static_cast<unsigned>(grid), cluster = static_cast<unsigned>(plan.cluster);
+    ipl_status st = launch_status(
+        plan.tiles == 1 ? launch_clustered(attention_short_kernel<kDim, 1>, ctas, cluster, kThreads, 0, stream, p)
+                        : launch_clustered(attention_short_kernel<kDim, 2>, ctas, cluster, kThreads, 0, stream, p),
+        "paged attention");
     if (st != IPL_SUCCESS || plan.splits == 1) return st;
     return launch_status(launch(attention_join_kernel<kDim>, static_cast<unsigned>(p.num_seqs * p.kv_heads), kJoinWarps * kWarpSize,
                                 0, stream, p),

@@ -33,9 +33,9 @@ struct AttentionParams {
     // Sequences of at most short_rows rows (new tokens x group) belong to the short kernel, the others
     // to the tile kernel.
     int short_rows;
-    int splits;     // CTAs along a sequence's keys, at most
+    int splits;     // clusters along a sequence's keys, at most
     int split_len;  // keys each takes, a multiple of kAttentionBlock (the last one: all that are left)
-    // Parts of rows whose keys several CTAs share: for split s of row r = token * heads + head, at
+    // Parts of rows whose keys several clusters share: for split s of row r = token * heads + head, at
     // s * num_tokens * heads + r, the unnormalised sum [padded dim] and (maximum, sum of weights).
     float* part_sums;
     float2* part_stats;
@@ -102,10 +102,13 @@ __device__ __forceinline__ float warp_max(float value) {
 //   O^T = V^T P^T:  lane (g, t) takes chunk g of keys 2t, 2t + 1, 2t + 8, 2t + 9 and pairs the keys'
 //     elements by byte permutes; P^T comes from the score registers by movmatrix.
 // The loads of the next block are issued as soon as the registers are free, keys behind S^T, values behind
-// O^T. The warps of a CTA take blocks in turn and are joined through shared memory at the end; several
-// CTAs share a sequence's keys where there are few sequences (attention_join_kernel adds their parts).
+// O^T. The warps of a CTA take blocks in turn and are joined through shared memory at the end. Where sequences
+// and key heads are few, a cluster of up to 8 CTAs shares a sequence's keys and adds its parts through
+// distributed shared memory, which needs no workspace and no second launch; where even that leaves SMs idle,
+// several clusters do, and attention_join_kernel adds theirs.
 
 constexpr int kShortWarps = 4;
+constexpr int kShortCluster = 8;  // CTAs a cluster, at most
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -136,16 +139,20 @@ __global__ void __launch_bounds__(kShortWarps * kWarpSize, kTiles == 1 ? 3 : 2) 
     constexpr int kChunks = kDim / 32;   // 16-byte chunks of a row a lane takes
     constexpr int kPasses = kDim / 64;   // 64-element halves of a value row
     constexpr int kMmas = kDim / 16;     // products of 16 head elements
-    __shared__ float joined[kShortWarps][kRows][kDim + 4];
-    __shared__ float2 stats[kShortWarps][kRows];
+    constexpr int kThreads = kShortWarps * kWarpSize;
+    __shared__ __align__(16) float joined[kShortWarps][kRows][kDim + 4];
+    __shared__ float2 stats[kShortWarps][kRows], cta_stats[kRows];
     grid_dependency_wait();
     grid_launch_dependents();
 
-    const uint32_t pair = blockIdx.x % (static_cast<uint32_t>(p.num_seqs) * p.kv_heads);
-    const int split = blockIdx.x / (static_cast<uint32_t>(p.num_seqs) * p.kv_heads);
+    const uint32_t rank = cluster_ctarank(), ctas = cluster_nctarank();
+    const uint32_t unit = blockIdx.x / ctas;
+    const uint32_t pair = unit % (static_cast<uint32_t>(p.num_seqs) * p.kv_heads);
+    const int split = unit / (static_cast<uint32_t>(p.num_seqs) * p.kv_heads);
     const int seq = pair / p.kv_heads, kv_head = pair - seq * p.kv_heads;
     const int begin = p.starts[seq], new_tokens = min(p.starts[seq + 1], p.num_tokens) - begin;
     const int rows = new_tokens * p.group;
+    // The CTAs of a cluster leave together: here and below the conditions are the same for all of them.
     if (begin < 0 || new_tokens <= 0 || rows > p.short_rows) return;
     const int true_len = p.lens[seq];
     const int len = table_bounded_length(p, seq);
@@ -155,8 +162,9 @@ __global__ void __launch_bounds__(kShortWarps * kWarpSize, kTiles == 1 ? 3 : 2) 
     const int split_blocks = p.split_len / kAttentionBlock;
     const int used = min(p.splits, max(1, (blocks + split_blocks - 1) / split_blocks));
     if (split >= used) return;
-    const int block_begin = split * split_blocks;
-    const int block_end = split == used - 1 ? blocks : block_begin + split_blocks;
+    const int share_begin = split * split_blocks, share = (split == used - 1 ? blocks : share_begin + split_blocks) - share_begin;
+    const int block_begin = share_begin + static_cast<int>(static_cast<int64_t>(share) * rank / ctas);
+    const int block_end = share_begin + static_cast<int>(static_cast<int64_t>(share) * (rank + 1) / ctas);
 
     const int warp = threadIdx.x / kWarpSize, lane = threadIdx.x % kWarpSize;
     const int g = lane >> 2, t = lane & 3;
@@ -354,23 +362,9 @@ __global__ void __launch_bounds__(kShortWarps * kWarpSize, kTiles == 1 ? 3 : 2) 
             }
         }
         __syncthreads();
-        for (int e = threadIdx.x; e < kRows * (kDim / 4); e += kShortWarps * kWarpSize) {
-            const int local = e / (kDim / 4), d = e % (kDim / 4) * 4;
+        const auto write = [&](int local, int d, float m, float l, float4 total) {
             const int row = row0 + local;
-            if (row >= rows || d >= p.dim) continue;
-            float m = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < kShortWarps; ++w) m = fmaxf(m, stats[w][local].x);
-            float l = 0.0f;
-            float4 total = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-            for (int w = 0; w < kShortWarps; ++w) {
-                const float2 part = stats[w][local];
-                const float f = part.x == -INFINITY ? 0.0f : exp2_approx(part.x - m);
-                const float4 x = *reinterpret_cast<const float4*>(&joined[w][local][d]);
-                l += f * part.y;
-                total.x += f * x.x, total.y += f * x.y, total.z += f * x.z, total.w += f * x.w;
-            }
+            if (row >= rows || d >= p.dim) return;
             const int token = begin + row / p.group, head = kv_head * p.group + row % p.group;
             if (used > 1) {
                 const int64_t at = (static_cast<int64_t>(split) * p.num_tokens + token) * p.heads + head;
@@ -381,8 +375,71 @@ __global__ void __launch_bounds__(kShortWarps * kWarpSize, kTiles == 1 ? 3 : 2) 
                 st_v2(p.out + token * p.out_token + head * p.out_head + d, pack_bf16x2(total.x * inverse, total.y * inverse),
                       pack_bf16x2(total.z * inverse, total.w * inverse));
             }
+        };
+        // Four elements a thread, from all the warps; in a cluster the sum takes the place of warp 0's.
+        for (int e = threadIdx.x; e < kRows * (kDim / 4); e += kThreads) {
+            const int local = e / (kDim / 4), d = e % (kDim / 4) * 4;
+            float m = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kShortWarps; ++w) m = fmaxf(m, stats[w][local].x);
+            const float shift = m == -INFINITY ? 0.0f : m;
+            float l = 0.0f;
+            float4 total = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < kShortWarps; ++w) {
+                const float2 part = stats[w][local];
+                const float f = exp2_approx(part.x - shift);
+                const float4 x = *reinterpret_cast<const float4*>(&joined[w][local][d]);
+                l += f * part.y;
+                total.x += f * x.x, total.y += f * x.y, total.z += f * x.z, total.w += f * x.w;
+            }
+            if (ctas > 1) {
+                *reinterpret_cast<float4*>(&joined[0][local][d]) = total;
+                if (d == 0) cta_stats[local] = make_float2(m, l);
+            } else {
+                write(local, d, m, l, total);
+            }
         }
-        __syncthreads();
+        if (ctas > 1) {
+            __syncwarp();
+            cluster_arrive_release();
+            cluster_wait_acquire();
+            // Every CTA writes its share of the elements.
+            const uint32_t sums_at = smem_addr(joined), stats_at = smem_addr(cta_stats);
+            for (uint32_t e = rank * kThreads + threadIdx.x; e < kRows * (kDim / 4); e += ctas * kThreads) {
+                const int local = e / (kDim / 4), d = e % (kDim / 4) * 4;
+                float2 part[kShortCluster];
+                float4 x[kShortCluster];
+                float m = -INFINITY, l = 0.0f;
+#pragma unroll
+                for (uint32_t c = 0; c < kShortCluster; ++c) {
+                    if (c >= ctas) {
+                        part[c] = make_float2(-INFINITY, 0.0f);
+                        x[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        continue;
+                    }
+                    part[c] = ld_shared_cluster_f32x2(map_shared_to_rank(stats_at, c) + 8u * local);
+                    x[c] = ld_shared_cluster_f32x4(map_shared_to_rank(sums_at, c) + 4u * (local * (kDim + 4) + d));
+                }
+#pragma unroll
+                for (int c = 0; c < kShortCluster; ++c) m = fmaxf(m, part[c].x);
+                const float shift = m == -INFINITY ? 0.0f : m;
+                float4 total = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int c = 0; c < kShortCluster; ++c) {
+                    const float f = exp2_approx(part[c].x - shift);
+                    l += f * part[c].y;
+                    total.x += f * x[c].x, total.y += f * x[c].y, total.z += f * x[c].z, total.w += f * x[c].w;
+                }
+                write(local, d, m, l, total);
+            }
+            // No CTA's shared memory goes, or is written again, while another reads it.
+            __syncwarp();
+            cluster_arrive_release();
+            cluster_wait_acquire();
+        } else {
+            __syncthreads();
+        }
     }
 }
 

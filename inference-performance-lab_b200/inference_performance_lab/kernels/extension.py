@@ -185,7 +185,7 @@ def paged_attention(
     """
     load_extension()
 
-    output = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    output = torch.empty_like(query, memory_format=torch.contiguous_format)
     torch.ops.inference_performance_lab.paged_attention(
         output, query, key_cache, value_cache, block_tables, query_start_loc, seq_lens, max_query_len, max_seq_len,
         scale, window
@@ -253,9 +253,9 @@ def compact_pages(
     number of pages in use (int32 ``[1]``); the old tables stay valid until moved pages are claimed."""
     load_extension()
 
-    new_tables = torch.empty(block_tables.shape, dtype=block_tables.dtype, device=block_tables.device)
-    new_counts = torch.empty(ref_counts.shape, dtype=ref_counts.dtype, device=ref_counts.device)
-    live = torch.empty(1, dtype=torch.int32, device=block_tables.device)
+    new_tables = torch.empty_like(block_tables, memory_format=torch.contiguous_format)
+    new_counts = torch.empty_like(ref_counts)
+    live = ref_counts.new_empty(1)
     torch.ops.inference_performance_lab.compact_pages(caches, block_tables, ref_counts, new_tables, new_counts, live)
 
     return new_tables, new_counts, live
