@@ -4,6 +4,7 @@
 #include "cache_pages.cuh"
 #include "ipl_host.cuh"
 #include "paged_attention.cuh"
+#include "paged_attention_short.cuh"
 #include "paged_attention_tile.cuh"
 #include "rotary.cuh"
 
@@ -240,15 +241,14 @@ ipl_status make_tensor_map(CUtensorMap* map, const void* base, int rank, const i
 
 // Which kernels a call runs, a pure function of its sizes, strides, alignment and the SM count.
 struct AttentionPlan {
-    bool vector = false;  // the short kernel; else a warp per row
+    bool vector = false;  // the short and tile kernels; else a warp per row
     int dim = 0;          // head size padded to 64 or 128
-    int tiles = 0;        // short kernel: column tiles of 8 rows; 0: not launched
     bool tile = false;    // the tile kernel takes the sequences of more than short_rows rows
     int short_rows = 0;
-    int tile_ctas = 0;
-    size_t tile_workspace = 0;  // at the beginning of the workspace; the short kernel's parts follow
-    int splits = 1, split_len = 0, cluster = 1;
-    size_t workspace = 0;
+    int tiles = 0;        // short kernels: column tiles of 8 rows; 0: not launched
+    int cluster = 0;      // CTAs a sequence and key head of the short kernel; 0: the shared kernel
+    int tile_ctas = 0, shared_ctas = 0;
+    size_t tile_workspace = 0, workspace = 0;  // the tile kernel's at the beginning
 };
 
 // 16-byte chunks of every row, and 16 keys of a block in one page.
@@ -258,6 +258,21 @@ bool attention_vectorises(const ipl_paged_attention_args& a) {
                             a.value_cache_page_stride | a.value_cache_token_stride | a.value_cache_head_stride;
     return a.head_size % 8 == 0 && a.head_size <= 128 && a.page_size % kAttentionBlock == 0 && strides % 8 == 0 &&
            aligned(a.output, 16) && aligned(a.query, 16) && aligned(a.key_cache, 16) && aligned(a.value_cache, 16);
+}
+
+// Workspace of the parts that `ctas` CTAs leave.
+size_t parts_bytes(int64_t ctas, int64_t slot_rows, int64_t dim) {
+    return static_cast<size_t>(round_up(2 * ctas * (slot_rows * (dim * 4 + 8) + static_cast<int64_t>(sizeof(AttentionPart))), 16));
+}
+AttentionParts attention_parts(void* workspace, int64_t ctas, int slot_rows, int64_t dim, int tile_rows, int tile_tokens) {
+    AttentionParts parts;
+    parts.sums = static_cast<float*>(workspace);
+    parts.stats = reinterpret_cast<float2*>(parts.sums + 2 * ctas * slot_rows * dim);
+    parts.parts = reinterpret_cast<AttentionPart*>(parts.stats + 2 * ctas * slot_rows);
+    parts.slot_rows = slot_rows;
+    parts.tile_rows = tile_rows;
+    parts.tile_tokens = tile_tokens;
+    return parts;
 }
 
 AttentionPlan plan_attention(const ipl_paged_attention_args& a, int sm_count) {
@@ -284,56 +299,52 @@ AttentionPlan plan_attention(const ipl_paged_attention_args& a, int sm_count) {
             plan.short_rows = 0;
         }
     }
-    // CTAs a sequence and key head: enough to fill the GPU about four times over, so that ragged lengths even
-    // out, but a block of keys for each warp at the least; a cluster of up to 8 of them, and several clusters
-    // where that is not half of what the GPU holds.
-    int64_t keys = a.max_seq_len > 1 ? a.max_seq_len : 1;
-    if (a.window > 0 && a.window + a.max_query_len < keys) keys = a.window + a.max_query_len;
-    const int64_t pairs = a.num_seqs * a.num_kv_heads;
-    const int64_t resident = static_cast<int64_t>(sm_count) * (plan.tiles == 1 ? 3 : 2);
-    constexpr int64_t kLeast = kShortWarps * kAttentionBlock;
-    const int64_t most = (keys + kLeast - 1) / kLeast;
-    int64_t wanted = (resident * 4 + pairs - 1) / pairs;
-    if (wanted > most) wanted = most;
-    plan.cluster = 1;
-    while (plan.cluster < kShortCluster && plan.cluster < wanted) plan.cluster *= 2;
-    int64_t splits = 1;
-    if (pairs * plan.cluster * 2 < resident && wanted > plan.cluster) {
-        splits = (resident + pairs * plan.cluster - 1) / (pairs * plan.cluster);
-        if (splits > wanted / plan.cluster) splits = wanted / plan.cluster;
-    }
-    const int64_t len = round_up((keys + splits - 1) / splits, kAttentionBlock);
-    splits = (keys + len - 1) / len;
-    plan.split_len = static_cast<int>(len);
-    plan.splits = static_cast<int>(splits);
-    if (plan.tiles == 0) plan.splits = 1;
     if (plan.tile) {
         plan.tile_ctas = sm_count;
-        const size_t slots = 2 * static_cast<size_t>(sm_count), rows = slots * 2 * kTileRows;
-        plan.tile_workspace = rows * (plan.dim * sizeof(float) + sizeof(float2)) + round_up(slots * sizeof(TilePart), 16);
+        plan.tile_workspace = parts_bytes(plan.tile_ctas, 2 * kTileRows, plan.dim);
         plan.workspace = plan.tile_workspace;
     }
-    if (plan.splits > 1) {
-        const size_t rows = static_cast<size_t>(splits) * a.num_tokens * a.num_heads;
-        plan.workspace += rows * (plan.dim * sizeof(float) + sizeof(float2));
+    if (plan.tiles > 0) {
+        // A cluster for each sequence and key head where the GPU holds all of them and no warp has more than 16
+        // blocks of keys; otherwise equal shares.
+        int64_t keys = a.max_seq_len > 1 ? a.max_seq_len : 1;
+        if (a.window > 0 && a.window + a.max_query_len < keys) keys = a.window + a.max_query_len;
+        const int64_t pairs = a.num_seqs * a.num_kv_heads, resident = static_cast<int64_t>(sm_count) * short_ctas(plan.tiles);
+        const int64_t turns = (keys + kShortWarps * kAttentionBlock - 1) / (kShortWarps * kAttentionBlock);
+        plan.cluster = 1;
+        while (plan.cluster < kShortCluster && plan.cluster < turns && pairs * plan.cluster * 2 <= resident) plan.cluster *= 2;
+        if (pairs * plan.cluster > resident || turns > 16 * plan.cluster) {
+            plan.cluster = 0;
+            plan.shared_ctas = static_cast<int>(resident);
+            plan.workspace += parts_bytes(plan.shared_ctas, 8 * plan.tiles, plan.dim);
+        }
     }
     return plan;
 }
 
 template <int kDim>
-ipl_status launch_short(const AttentionPlan& plan, const AttentionParams& p, cudaStream_t stream) {
-    const int64_t grid = static_cast<int64_t>(p.num_seqs) * p.kv_heads * plan.splits * plan.cluster;
-    if (grid > INT_MAX) return fail(IPL_ERROR_TOO_LARGE, "too many sequences and heads");
-    constexpr unsigned kThreads = kShortWarps * kWarpSize;
-    const unsigned ctas = static_cast<unsigned>(grid), cluster = static_cast<unsigned>(plan.cluster);
-    ipl_status st = launch_status(
-        plan.tiles == 1 ? launch_clustered(attention_short_kernel<kDim, 1>, ctas, cluster, kThreads, 0, stream, p)
-                        : launch_clustered(attention_short_kernel<kDim, 2>, ctas, cluster, kThreads, 0, stream, p),
-        "paged attention");
-    if (st != IPL_SUCCESS || plan.splits == 1) return st;
-    return launch_status(launch(attention_join_kernel<kDim>, static_cast<unsigned>(p.num_seqs * p.kv_heads), kJoinWarps * kWarpSize,
-                                0, stream, p),
+ipl_status launch_join(const AttentionParams& p, const AttentionParts& parts, int ctas, cudaStream_t stream) {
+    return launch_status(launch_2d(attention_join_kernel<kDim>, static_cast<unsigned>(ctas),
+                                   static_cast<unsigned>(parts.slot_rows / kJoinWarps), kJoinWarps * kWarpSize, stream, p, parts),
                          "paged attention");
+}
+
+template <int kDim>
+ipl_status launch_short(const AttentionPlan& plan, const AttentionParams& p, char* workspace, cudaStream_t stream) {
+    if (plan.cluster > 0) {
+        const unsigned cluster = static_cast<unsigned>(plan.cluster), grid = static_cast<unsigned>(p.num_seqs * p.kv_heads) * cluster;
+        return launch_status(
+            plan.tiles == 1 ? launch_clustered(attention_short_kernel<kDim, 1>, grid, cluster, kShortThreads, 0, stream, p)
+                            : launch_clustered(attention_short_kernel<kDim, 2>, grid, cluster, kShortThreads, 0, stream, p),
+            "paged attention");
+    }
+    const AttentionParts parts = attention_parts(workspace, plan.shared_ctas, 8 * plan.tiles, kDim, 8 * plan.tiles, 8 * plan.tiles);
+    const unsigned grid = static_cast<unsigned>(plan.shared_ctas);
+    const ipl_status st = launch_status(
+        plan.tiles == 1 ? launch(attention_shared_kernel<kDim, 1>, grid, kShortThreads, 0, stream, p, parts)
+                        : launch(attention_shared_kernel<kDim, 2>, grid, kShortThreads, 0, stream, p, parts),
+        "paged attention");
+    return st == IPL_SUCCESS ? launch_join<kDim>(p, parts, plan.shared_ctas, stream) : st;
 }
 
 template <int kDim>
@@ -356,10 +367,7 @@ ipl_status launch_tile(const ipl_paged_attention_args& a, const AttentionPlan& p
     t.pair_tokens = make_fast_div32(static_cast<uint32_t>(2 * t.tile_tokens));
     t.page_size = make_fast_div32(static_cast<uint32_t>(p.page_size));
     t.group_reciprocal = 65536 / p.group + 1;
-    const size_t rows = static_cast<size_t>(plan.tile_ctas) * 2 * 2 * kTileRows;
-    t.part_sums = static_cast<float*>(a.workspace);
-    t.part_stats = reinterpret_cast<float2*>(t.part_sums + rows * kDim);
-    t.parts = reinterpret_cast<TilePart*>(t.part_stats + rows);
+    t.parts = attention_parts(a.workspace, plan.tile_ctas, 2 * kTileRows, kDim, kTileRows, t.tile_tokens);
     CUtensorMap q, k, v;
     const int64_t q_sizes[3] = {p.dim, p.heads, p.num_tokens}, q_strides[2] = {p.q_head, p.q_token};
     const int q_box[3] = {64, p.group, t.tile_tokens};
@@ -375,9 +383,7 @@ ipl_status launch_tile(const ipl_paged_attention_args& a, const AttentionPlan& p
     st = launch_status(launch(attention_tile_kernel<kDim>, ctas, kTileThreads, Layout::kDynamic, stream, t, q, k, v),
                        "paged attention");
     if (st != IPL_SUCCESS) return st;
-    return launch_status(launch_2d(attention_tile_join_kernel<kDim>, ctas, 2 * kTileRows / kTileJoinWarps,
-                                   kTileJoinWarps * kWarpSize, stream, t),
-                         "paged attention");
+    return launch_join<kDim>(p, t.parts, plan.tile_ctas, stream);
 }
 
 template <int kDim>
@@ -385,7 +391,7 @@ ipl_status launch_attention(const ipl_paged_attention_args& a, const AttentionPl
                             DeviceInfo* info, cudaStream_t stream) {
     ipl_status st = IPL_SUCCESS;
     if (plan.tile) st = launch_tile<kDim>(a, plan, p, info, stream);
-    if (st == IPL_SUCCESS && plan.tiles > 0) st = launch_short<kDim>(plan, p, stream);
+    if (st == IPL_SUCCESS && plan.tiles > 0) st = launch_short<kDim>(plan, p, static_cast<char*>(a.workspace) + plan.tile_workspace, stream);
     return st;
 }
 
@@ -408,10 +414,6 @@ ipl_status run_attention(const ipl_paged_attention_args* a, cudaStream_t stream)
         return fail(IPL_ERROR_INVALID_VALUE, "workspace must be non-null and 16-byte aligned");
     }
     p.short_rows = plan.short_rows;
-    p.splits = plan.splits;
-    p.split_len = plan.split_len;
-    p.part_sums = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + plan.tile_workspace);
-    p.part_stats = reinterpret_cast<float2*>(p.part_sums + static_cast<size_t>(plan.splits) * a->num_tokens * a->num_heads * plan.dim);
     return plan.dim == 64 ? launch_attention<64>(*a, plan, p, info, stream) : launch_attention<128>(*a, plan, p, info, stream);
 }
 
@@ -550,14 +552,13 @@ const char* ipl_paged_attention_plan(const ipl_paged_attention_args* args) {
     const AttentionPlan plan = plan_attention(*args, sms);
     if (!plan.vector) return "attention_row_kernel";
     static const char* const kNames[2][5] = {
-        {"attention_short_kernel<1>", "attention_short_kernel<2>", "attention_short_kernel<1> + attention_join_kernel",
-         "attention_short_kernel<2> + attention_join_kernel", "invalid"},
-        {"attention_tile_kernel + attention_tile_join_kernel + attention_short_kernel<1>",
-         "attention_tile_kernel + attention_tile_join_kernel + attention_short_kernel<2>",
-         "attention_tile_kernel + attention_tile_join_kernel + attention_short_kernel<1> + attention_join_kernel",
-         "attention_tile_kernel + attention_tile_join_kernel + attention_short_kernel<2> + attention_join_kernel",
-         "attention_tile_kernel + attention_tile_join_kernel"}};
-    return kNames[plan.tile ? 1 : 0][plan.tiles == 0 ? 4 : plan.tiles - 1 + (plan.splits > 1 ? 2 : 0)];
+        {"invalid", "attention_short_kernel<1>", "attention_short_kernel<2>", "attention_shared_kernel<1> + attention_join_kernel",
+         "attention_shared_kernel<2> + attention_join_kernel"},
+        {"attention_tile_kernel + attention_join_kernel", "attention_tile_kernel + attention_join_kernel + attention_short_kernel<1>",
+         "attention_tile_kernel + attention_join_kernel + attention_short_kernel<2>",
+         "attention_tile_kernel + attention_join_kernel + attention_shared_kernel<1> + attention_join_kernel",
+         "attention_tile_kernel + attention_join_kernel + attention_shared_kernel<2> + attention_join_kernel"}};
+    return kNames[plan.tile ? 1 : 0][plan.tiles == 0 ? 0 : plan.tiles + (plan.cluster > 0 ? 0 : 2)];
 }
 
 ipl_status ipl_pages_workspace(int64_t num_pages, int64_t count, size_t* bytes) {

@@ -11,7 +11,7 @@
 //   warp 9           loads Q, and K and V page by page (TMA), into a ring of shared-memory stages;
 //   warp 10          hands out the work.
 // A CTA on every SM takes an equal share of the steps of all pairs of tiles and key heads, laid end to end;
-// a pair that a share's border cuts leaves parts in the workspace, which attention_tile_join_kernel adds.
+// a pair that a share's border cuts leaves parts in the workspace, which attention_join_kernel adds.
 // Against a CTA for each pair, that evens out the last wave (57 pairs x 4 heads on 148 SMs are 1.54 waves)
 // and hides each pair's first loads behind the pair before.
 // P overwrites the first half of its S; the products are issued in the order P_t V (step j), Q_t K^T (step
@@ -47,18 +47,7 @@ struct TileParams {
     int group_reciprocal;  // 65536 / group + 1: row / group of a row below 128 is the product's high half
     int box_keys;     // keys a TMA box: the largest power of two up to 128 that divides the page size
     int units;        // upper bound of the tile pairs of all sequences
-    // Parts of pairs that several CTAs share. CTA c leaves at most two: in slot 2 c the last steps (or a middle
-    // stretch) of a pair that the CTA before began, in slot 2 c + 1 the first steps of one that it leaves to
-    // the next. A slot holds [256 rows][padded dim] sums and [256] (maximum, sum of weights).
-    float* part_sums;
-    float2* part_stats;
-    struct TilePart* parts;
-};
-
-// What is in a slot: nothing (tiles 0), or rows of a pair.
-struct TilePart {
-    int tiles, token, tokens, kv_head;  // first token, number of tokens of the pair
-    int last;                           // the pair's last steps
+    AttentionParts parts;  // of pairs that several CTAs share
 };
 
 // Shared memory: the two Q tiles, the stages, the barriers. A tile of kDim 128 is two halves of 64
@@ -320,7 +309,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
       warpgroup_leave_registers<kOtherRegisters>();
       if (warp == 10) {
         // Work: 32 pairs at a time, one a lane; lane 0 writes the items.
-        if (lane < 2) p.parts[2 * blockIdx.x + lane].tiles = 0;
+        if (lane < 2) p.parts.parts[2 * blockIdx.x + lane].tokens = 0;
         __syncwarp();
         int n = 0;
         const auto put = [&](const TileItem& item) {
@@ -375,12 +364,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 if (item.steps < steps) {
                     item.slot = 2 * blockIdx.x + (step_begin == 0 ? 1 : 0);
                     if (lane == 0) {
-                        TilePart& part = p.parts[item.slot];
-                        part.token = item.token;
-                        part.tokens = item.tokens;
-                        part.kv_head = head;
-                        part.last = step_end == steps;
-                        part.tiles = item.tiles;
+                        p.parts.parts[item.slot] = AttentionPart{item.tokens, item.token, head, step_end == steps};
                     }
                 }
                 ok = put(item);
@@ -724,12 +708,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             const uint32_t real = __ballot_sync(0xffffffffu, in_tile < p.tile_tokens && t * p.tile_tokens + in_tile < item.tokens);
             const int slot = item.slot;
             const int64_t part = static_cast<int64_t>(slot) * (2 * kTileRows) + t * kTileRows + r;
-            if (slot >= 0) p.part_stats[part] = make_float2(top, sum);
+            if (slot >= 0) p.parts.stats[part] = make_float2(top, sum);
             // Bytes of this thread's row; the rows of the eight threads that share their rows' chunks.
             const int64_t mine = slot >= 0 ? part * (kDim * 4)
                                            : 2 * (static_cast<int64_t>(item.token + t * p.tile_tokens + in_tile) * a.out_token +
                                                   (item.kv_head * a.group + r - in_tile * a.group) * a.out_head);
-            char* const to = (slot >= 0 ? reinterpret_cast<char*>(p.part_sums) : reinterpret_cast<char*>(a.out)) + 16 * (lane & 7);
+            char* const to = (slot >= 0 ? reinterpret_cast<char*>(p.parts.sums) : reinterpret_cast<char*>(a.out)) + 16 * (lane & 7);
             const int columns = slot >= 0 ? 32 : 64;  // of a pass: 128 bytes a row
             for (int c = 0; c < kDim; c += columns) {
                 uint32_t v[32];
@@ -777,59 +761,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     __syncthreads();
     tcgen05_fence_after();
     if (warp == 8) tmem_free(tmem);
-}
-
-// Adds the parts of pairs that several CTAs of the tile kernel shared: block (c, y) takes 8 rows, one a warp, of
-// the pair whose first steps are in slot 2 c + 1; the others' follow in slots 2 (c + 1), 2 (c + 2), ...
-constexpr int kTileJoinWarps = 8;
-
-template <int kDim>
-__global__ void __launch_bounds__(kTileJoinWarps * kWarpSize) attention_tile_join_kernel(const TileParams p) {
-    grid_dependency_wait();
-    grid_launch_dependents();
-    constexpr int kMine = kDim / kWarpSize;
-    const int first = 2 * blockIdx.x + 1, ctas = gridDim.x;
-    const TilePart part = p.parts[first];
-    const int warp = threadIdx.x / kWarpSize, lane = threadIdx.x % kWarpSize;
-    const int row = blockIdx.y * kTileJoinWarps + warp, t = row / kTileRows, r = row % kTileRows;
-    const int in_tile = r / p.a.group, token = t * p.tile_tokens + in_tile;
-    if (part.tiles <= t || in_tile >= p.tile_tokens || token >= part.tokens) return;
-    // The slots of the pair, 32 CTAs at a time, one a lane: those with a share, up to the pair's last steps.
-    float m = -INFINITY, l = 0.0f, total[kMine] = {};
-    for (int base = blockIdx.x; base < ctas; base += kWarpSize) {
-        const int slot = base + lane == static_cast<int>(blockIdx.x) ? first : 2 * (base + lane);
-        const bool there = base + lane < ctas && p.parts[slot].tiles != 0;
-        const uint32_t ends = __ballot_sync(0xffffffffu, there && p.parts[slot].last != 0);
-        const bool mine = there && (ends == 0 || lane < __ffs(ends));
-        const float2 stats = mine ? p.part_stats[static_cast<int64_t>(slot) * (2 * kTileRows) + row] : make_float2(-INFINITY, 0.0f);
-        const float top = fmaxf(m, warp_max(stats.x)), shift = top == -INFINITY ? 0.0f : top;
-        const float keep = exp2_approx(m - shift), add = exp2_approx(stats.x - shift);
-        l = l * keep + warp_sum(stats.y * add);
-#pragma unroll
-        for (int i = 0; i < kMine; ++i) total[i] *= keep;
-        const uint32_t set = __ballot_sync(0xffffffffu, mine);
-        const int count = 32 - __clz(set);
-#pragma unroll 8
-        for (int j = 0; j < count; ++j) {
-            const float f = __shfl_sync(0xffffffffu, add, j);
-            if (!(set >> j & 1u)) continue;
-            const int from = __shfl_sync(0xffffffffu, slot, j);
-            const float* x = p.part_sums + (static_cast<int64_t>(from) * (2 * kTileRows) + row) * kDim + lane * kMine;
-#pragma unroll
-            for (int i = 0; i < kMine; ++i) total[i] += x[i] * f;
-        }
-        m = top;
-        if (ends != 0) break;
-    }
-    const float inverse = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    const int d = lane * kMine;
-    if (d >= p.a.dim) return;
-    const int head = part.kv_head * p.a.group + r - in_tile * p.a.group;
-    uint16_t* out = p.a.out + static_cast<int64_t>(part.token + token) * p.a.out_token + head * p.a.out_head + d;
-#pragma unroll
-    for (int i = 0; i < kMine; i += 2) {
-        *reinterpret_cast<uint32_t*>(out + i) = pack_bf16x2(total[i] * inverse, total[i + 1] * inverse);
-    }
 }
 
 }  // namespace ipl
