@@ -224,8 +224,8 @@ IPL_API const char* ipl_paged_attention_plan(const ipl_paged_attention_args* arg
  * 16-byte aligned).
  *
  * status receives 0, or the number of free pages lacking, or -1 for an entry out of range (a row, a
- * length, a row given twice, a child that holds tokens); unless it is 0 nothing has changed. The
- * workspace (ipl_pages_workspace bytes, 4-byte aligned) may be reused by later work on the stream.
+ * length, a row given twice, a child that holds tokens); unless it is 0 nothing has changed. A call
+ * takes up to 16384 rows.
  *
  * ipl_copy_pages: page pairs[2 i] to page pairs[2 i + 1] in every cache; negative entries are skipped.
  *   No target may be the source or target of another pair.
@@ -235,7 +235,8 @@ IPL_API const char* ipl_paged_attention_plan(const ipl_paged_attention_args* arg
  * ipl_release_sequences: the pages of rows[i] lose one reference each, the row becomes empty.
  * ipl_compact_pages: the pages in use past the first `live` numbers move, in order, to the free numbers
  *   below. The renumbered tables ([num_rows, width] contiguous) and counts are written beside the old
- *   ones, which stay valid for work in flight: moved pages keep their data until they are claimed.
+ *   ones, which stay valid for work in flight: moved pages keep their data until they are claimed. The
+ *   workspace (ipl_compact_pages_workspace bytes, 4-byte aligned) may be reused by later work on the stream.
  */
 typedef struct ipl_page_pool {
     int32_t* block_tables;
@@ -249,16 +250,14 @@ typedef struct ipl_page_caches {
     int64_t num_caches, page_stride_bytes, page_bytes;
 } ipl_page_caches;
 
-IPL_API ipl_status ipl_pages_workspace(int64_t num_pages, int64_t count, size_t* bytes);
 IPL_API ipl_status ipl_copy_pages(const ipl_page_caches* caches, int64_t num_pages, const int32_t* pairs,
                                   int64_t count, void* stream);
 IPL_API ipl_status ipl_reserve_pages(const ipl_page_pool* pool, const int32_t* rows, const int32_t* new_lens,
-                                     int64_t count, void* workspace, size_t workspace_bytes, int32_t* status,
-                                     void* stream);
+                                     int64_t count, int32_t* status, void* stream);
 IPL_API ipl_status ipl_fork_sequences(const ipl_page_caches* caches, const ipl_page_pool* pool, const int32_t* parents,
-                                      const int32_t* children, int64_t count, void* workspace,
-                                      size_t workspace_bytes, int32_t* status, void* stream);
+                                      const int32_t* children, int64_t count, int32_t* status, void* stream);
 IPL_API ipl_status ipl_release_sequences(const ipl_page_pool* pool, const int32_t* rows, int64_t count, void* stream);
+IPL_API ipl_status ipl_compact_pages_workspace(int64_t num_pages, size_t* bytes);
 IPL_API ipl_status ipl_compact_pages(const ipl_page_caches* caches, const ipl_page_pool* pool,
                                      int32_t* new_block_tables, int32_t* new_ref_counts, int32_t* live,
                                      void* workspace, size_t workspace_bytes, void* stream);

@@ -322,16 +322,26 @@ AttentionPlan plan_attention(const ipl_paged_attention_args& a, int sm_count) {
     return plan;
 }
 
-template <int kDim>
+// Rows of a join block and warps a row: many pairs of tiles are cut in two or three, few short rows in up to 150.
+template <int kDim, int kRows, int kSplit>
 ipl_status launch_join(const AttentionParams& p, const AttentionParts& parts, int ctas, cudaStream_t stream) {
-    return launch_status(launch_2d(attention_join_kernel<kDim>, static_cast<unsigned>(ctas),
-                                   static_cast<unsigned>(parts.slot_rows / kJoinWarps), kJoinWarps * kWarpSize, stream, p, parts),
+    return launch_status(launch_2d(attention_join_kernel<kDim, kRows, kSplit>, static_cast<unsigned>(ctas),
+                                   static_cast<unsigned>(parts.slot_rows / kRows), kRows * kSplit * kWarpSize, stream, p, parts),
                          "paged attention");
 }
 
 template <int kDim>
-ipl_status launch_short(const AttentionPlan& plan, const AttentionParams& p, char* workspace, cudaStream_t stream) {
+ipl_status launch_short(const AttentionPlan& plan, const AttentionParams& p, char* workspace, DeviceInfo* info, cudaStream_t stream) {
     if (plan.cluster > 0) {
+        const uint32_t bit = 1u << (kDim == 64 ? 28 : 29);
+        if (plan.cluster > 8 && !(info->smem_configured.load(std::memory_order_acquire) & bit)) {
+            cudaError_t err = cudaFuncSetAttribute(attention_short_kernel<kDim, 1>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            if (err == cudaSuccess) {
+                err = cudaFuncSetAttribute(attention_short_kernel<kDim, 2>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            }
+            if (err != cudaSuccess) return fail(IPL_ERROR_CUDA, "paged attention kernel setup failed: %s", cudaGetErrorString(err));
+            info->smem_configured.fetch_or(bit, std::memory_order_acq_rel);
+        }
         const unsigned cluster = static_cast<unsigned>(plan.cluster), grid = static_cast<unsigned>(p.num_seqs * p.kv_heads) * cluster;
         return launch_status(
             plan.tiles == 1 ? launch_clustered(attention_short_kernel<kDim, 1>, grid, cluster, kShortThreads, 0, stream, p)
@@ -344,7 +354,7 @@ ipl_status launch_short(const AttentionPlan& plan, const AttentionParams& p, cha
         plan.tiles == 1 ? launch(attention_shared_kernel<kDim, 1>, grid, kShortThreads, 0, stream, p, parts)
                         : launch(attention_shared_kernel<kDim, 2>, grid, kShortThreads, 0, stream, p, parts),
         "paged attention");
-    return st == IPL_SUCCESS ? launch_join<kDim>(p, parts, plan.shared_ctas, stream) : st;
+    return st == IPL_SUCCESS ? launch_join<kDim, 2, 8>(p, parts, plan.shared_ctas, stream) : st;
 }
 
 template <int kDim>
@@ -383,7 +393,7 @@ ipl_status launch_tile(const ipl_paged_attention_args& a, const AttentionPlan& p
     st = launch_status(launch(attention_tile_kernel<kDim>, ctas, kTileThreads, Layout::kDynamic, stream, t, q, k, v),
                        "paged attention");
     if (st != IPL_SUCCESS) return st;
-    return launch_join<kDim>(p, t.parts, plan.tile_ctas, stream);
+    return launch_join<kDim, 8, 1>(p, t.parts, plan.tile_ctas, stream);
 }
 
 template <int kDim>
@@ -391,7 +401,7 @@ ipl_status launch_attention(const ipl_paged_attention_args& a, const AttentionPl
                             DeviceInfo* info, cudaStream_t stream) {
     ipl_status st = IPL_SUCCESS;
     if (plan.tile) st = launch_tile<kDim>(a, plan, p, info, stream);
-    if (st == IPL_SUCCESS && plan.tiles > 0) st = launch_short<kDim>(plan, p, static_cast<char*>(a.workspace) + plan.tile_workspace, stream);
+    if (st == IPL_SUCCESS && plan.tiles > 0) st = launch_short<kDim>(plan, p, static_cast<char*>(a.workspace) + plan.tile_workspace, info, stream);
     return st;
 }
 
@@ -487,32 +497,29 @@ int cache_list(const ipl_page_caches& c, int64_t from, CacheList* list) {
     return n;
 }
 
-// Workspace of the page calls: first and parent_lens [count], then three lists of num_pages, then one.
-size_t pages_workspace_bytes(int64_t num_pages, int64_t count) {
-    return static_cast<size_t>(2 * count + 3 * num_pages + 1) * sizeof(int32_t);
-}
+// Workspace of a compaction: three lists of num_pages, then a count.
+size_t compact_workspace_bytes(int64_t num_pages) { return static_cast<size_t>(3 * num_pages + 1) * sizeof(int32_t); }
 
-ipl_status check_workspace(const void* workspace, size_t bytes, int64_t num_pages, int64_t count) {
-    if (workspace == nullptr || !aligned(workspace, 4)) {
-        return fail(IPL_ERROR_INVALID_VALUE, "workspace must be non-null and 4-byte aligned");
+ipl_status check_claim(const ipl_page_pool* pool, const void* rows, const void* other, int64_t count, const int32_t* status) {
+    ipl_status st = check_pool(pool);
+    if (st == IPL_SUCCESS) st = check_rows(pool, rows, other, count);
+    if (st != IPL_SUCCESS) return st;
+    if (count > kMaxClaimRows) return fail(IPL_ERROR_TOO_LARGE, "number of rows must be at most %d", kMaxClaimRows);
+    if (status == nullptr || !aligned(status, 4)) {
+        return fail(IPL_ERROR_INVALID_VALUE, "status must be non-null and 4-byte aligned");
     }
-    if (bytes < pages_workspace_bytes(num_pages, count)) return fail(IPL_ERROR_INVALID_VALUE, "workspace is too small");
     return IPL_SUCCESS;
 }
 
-ClaimParams claim_params(const ipl_page_pool& pool, const int32_t* parents, const int32_t* rows, const int32_t* new_lens,
-                         int64_t count, void* workspace, int32_t* status) {
-    ClaimParams p = {};
-    p.state = page_state(pool);
-    p.parents = parents;
-    p.rows = rows;
-    p.new_lens = new_lens;
-    p.count = static_cast<int>(count);
-    p.first = static_cast<int32_t*>(workspace);
-    p.parent_lens = p.first + count;
-    p.fresh = p.parent_lens + count;
-    p.status = status;
-    return p;
+template <bool kFork>
+ipl_status launch_claim(const ClaimParams& p, cudaStream_t stream) {
+    const size_t smem = 2 * sizeof(int) * static_cast<size_t>(p.count);
+    if (smem > 40 * 1024) {
+        const cudaError_t err = cudaFuncSetAttribute(page_claim_kernel<kFork>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                     2 * sizeof(int) * kMaxClaimRows);
+        if (err != cudaSuccess) return fail(IPL_ERROR_CUDA, "page claim kernel setup failed: %s", cudaGetErrorString(err));
+    }
+    return launch_status(launch(page_claim_kernel<kFork>, 1, kPlanThreads, smem, stream, p), "page claim");
 }
 
 }  // namespace
@@ -561,12 +568,12 @@ const char* ipl_paged_attention_plan(const ipl_paged_attention_args* args) {
     return kNames[plan.tile ? 1 : 0][plan.tiles == 0 ? 0 : plan.tiles + (plan.cluster > 0 ? 0 : 2)];
 }
 
-ipl_status ipl_pages_workspace(int64_t num_pages, int64_t count, size_t* bytes) {
+ipl_status ipl_compact_pages_workspace(int64_t num_pages, size_t* bytes) {
     using namespace ipl;
-    if (bytes == nullptr || num_pages < 0 || count < 0 || num_pages > INT_MAX || count > INT_MAX) {
-        return fail(IPL_ERROR_INVALID_VALUE, "bytes must be non-null and the sizes non-negative 32-bit numbers");
+    if (bytes == nullptr || num_pages < 0 || num_pages > INT_MAX / 2) {
+        return fail(IPL_ERROR_INVALID_VALUE, "bytes must be non-null and the number of pages a non-negative 31-bit number");
     }
-    *bytes = pages_workspace_bytes(num_pages, count);
+    *bytes = compact_workspace_bytes(num_pages);
     return IPL_SUCCESS;
 }
 
@@ -596,35 +603,23 @@ ipl_status ipl_copy_pages(const ipl_page_caches* caches, int64_t num_pages, cons
 }
 
 ipl_status ipl_reserve_pages(const ipl_page_pool* pool, const int32_t* rows, const int32_t* new_lens, int64_t count,
-                             void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+                             int32_t* status, void* stream) {
     using namespace ipl;
-    ipl_status st = check_pool(pool);
-    if (st == IPL_SUCCESS) st = check_rows(pool, rows, new_lens, count);
-    if (st == IPL_SUCCESS) st = check_workspace(workspace, workspace_bytes, pool->num_pages, count);
+    const ipl_status st = check_claim(pool, rows, new_lens, count, status);
     if (st != IPL_SUCCESS) return st;
-    if (status == nullptr || !aligned(status, 4)) {
-        return fail(IPL_ERROR_INVALID_VALUE, "status must be non-null and 4-byte aligned");
-    }
-    const ClaimParams p = claim_params(*pool, nullptr, rows, new_lens, count, workspace, status);
-    return launch_status(launch(page_claim_kernel<false>, 1, kPlanThreads, 0, static_cast<cudaStream_t>(stream), p), "page claim");
+    const ClaimParams p = {page_state(*pool), nullptr, rows, new_lens, static_cast<int>(count), status};
+    return launch_claim<false>(p, static_cast<cudaStream_t>(stream));
 }
 
 ipl_status ipl_fork_sequences(const ipl_page_caches* caches, const ipl_page_pool* pool, const int32_t* parents,
-                              const int32_t* children, int64_t count, void* workspace, size_t workspace_bytes,
-                              int32_t* status, void* stream) {
+                              const int32_t* children, int64_t count, int32_t* status, void* stream) {
     using namespace ipl;
     ipl_status st = check_caches(caches);
-    if (st == IPL_SUCCESS) st = check_pool(pool);
-    if (st == IPL_SUCCESS) st = check_rows(pool, parents, children, count);
-    if (st == IPL_SUCCESS) st = check_workspace(workspace, workspace_bytes, pool->num_pages, count);
+    if (st == IPL_SUCCESS) st = check_claim(pool, children, parents, count, status);
     if (st != IPL_SUCCESS) return st;
-    if (status == nullptr || !aligned(status, 4)) {
-        return fail(IPL_ERROR_INVALID_VALUE, "status must be non-null and 4-byte aligned");
-    }
-    if (count > INT_MAX / kMaxCachesPerLaunch) return fail(IPL_ERROR_TOO_LARGE, "number of rows is too large");
-    const ClaimParams claim = claim_params(*pool, parents, children, nullptr, count, workspace, status);
+    const ClaimParams claim = {page_state(*pool), parents, children, nullptr, static_cast<int>(count), status};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    st = launch_status(launch(page_claim_kernel<true>, 1, kPlanThreads, 0, s, claim), "page claim");
+    st = launch_claim<true>(claim, s);
     if (st != IPL_SUCCESS || count == 0) return st;
     int64_t from = 0;
     do {
@@ -634,9 +629,6 @@ ipl_status ipl_fork_sequences(const ipl_page_caches* caches, const ipl_page_pool
         p.state = claim.state;
         p.parents = parents;
         p.children = children;
-        p.first = claim.first;
-        p.parent_lens = claim.parent_lens;
-        p.fresh = claim.fresh;
         p.status = status;
         p.page_stride = caches->page_stride_bytes;
         p.page_bytes = caches->page_bytes;
@@ -668,8 +660,13 @@ ipl_status ipl_compact_pages(const ipl_page_caches* caches, const ipl_page_pool*
     using namespace ipl;
     ipl_status st = check_caches(caches);
     if (st == IPL_SUCCESS) st = check_pool(pool);
-    if (st == IPL_SUCCESS) st = check_workspace(workspace, workspace_bytes, pool->num_pages, 0);
     if (st != IPL_SUCCESS) return st;
+    if (workspace == nullptr || !aligned(workspace, 4)) {
+        return fail(IPL_ERROR_INVALID_VALUE, "workspace must be non-null and 4-byte aligned");
+    }
+    if (workspace_bytes < compact_workspace_bytes(pool->num_pages)) {
+        return fail(IPL_ERROR_INVALID_VALUE, "workspace is too small");
+    }
     if ((pool->num_rows > 0 && pool->width > 0 && new_block_tables == nullptr) ||
         (pool->num_pages > 0 && new_ref_counts == nullptr) || live == nullptr) {
         return fail(IPL_ERROR_INVALID_VALUE, "new_block_tables, new_ref_counts and live must be non-null");

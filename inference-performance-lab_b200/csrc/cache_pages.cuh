@@ -69,20 +69,22 @@ struct ClaimParams {
     const int32_t* parents;   // fork; null: reserve
     const int32_t* rows;      // fork: the children; reserve: the rows that grow
     const int32_t* new_lens;  // reserve
-    int count;
-    int32_t* first;        // workspace [count]: rank of a row's first fresh page
-    int32_t* parent_lens;  // workspace [count] (fork)
-    int32_t* fresh;        // workspace [num_pages]: the claimed pages in order
+    int count;                // at most kMaxClaimRows
     int32_t* status;
 };
+constexpr int kMaxClaimRows = 16384;  // two words of shared memory each
+constexpr int kClaimPages = 4;        // pages a thread looks at in a round
 
 __device__ __forceinline__ int pages_of(int len, int page_size) { return len / page_size + (len % page_size != 0); }
 
-// One CTA. Counts the pages each row needs (fork: one where the parent's last page is partly filled),
-// finds that many free ones, and only then changes anything: the counts, the lengths and (reserve)
-// the tables. The tables and data of a fork follow in page_fork_kernel.
+// One CTA. Counts the pages each row needs (fork: one where the parent's last page is partly filled) and the
+// free ones, and only if they suffice changes anything: the tables' new entries, the counts and the lengths.
+// The shared pages and the data of a fork follow in page_fork_kernel.
 template <bool kFork>
 __global__ void __launch_bounds__(kPlanThreads) page_claim_kernel(const ClaimParams p) {
+    extern __shared__ int claim_rows[];
+    int* const first = claim_rows;           // rank of a row's first fresh page; -1: not marked by this entry
+    int* const base_len = claim_rows + p.count;  // fork: the parent's length; reserve: the row's
     __shared__ int warp_sums[kPlanWarps];
     __shared__ int invalid;
     const PageState& s = p.state;
@@ -96,10 +98,10 @@ __global__ void __launch_bounds__(kPlanThreads) page_claim_kernel(const ClaimPar
     for (int base = 0; base < p.count; base += kPlanThreads) {
         const int i = base + tid;
         int need = 0;
+        bool marked = false;
         if (i < p.count) {
             const int row = p.rows[i];
             bool ok = row >= 0 && row < s.num_rows;
-            bool marked = false;
             int len = 0;
             if (ok) {
                 // A row that appears twice finds the mark of its first appearance.
@@ -114,54 +116,72 @@ __global__ void __launch_bounds__(kPlanThreads) page_claim_kernel(const ClaimPar
                     parent_len = *static_cast<volatile int32_t*>(&s.lens[parent]) & ~kRowMarked;
                     ok = pages_of(parent_len, s.page_size) <= s.width;
                 }
-                p.parent_lens[i] = parent_len;
+                base_len[i] = parent_len;
                 need = ok && parent_len % s.page_size != 0;
-            } else if (ok) {
-                const int new_len = p.new_lens[i];
-                ok = new_len >= 0 && pages_of(new_len, s.page_size) <= s.width;
-                if (ok) need = max(0, pages_of(new_len, s.page_size) - pages_of(len, s.page_size));
+            } else {
+                base_len[i] = len;
+                if (ok) {
+                    const int new_len = p.new_lens[i];
+                    ok = new_len >= 0 && pages_of(new_len, s.page_size) <= s.width;
+                    if (ok) need = max(0, pages_of(new_len, s.page_size) - pages_of(len, s.page_size));
+                }
             }
             if (!ok) invalid = 1;
-            p.first[i] = marked ? 0 : -1;
         }
         int total = 0;
         const int before = block_exclusive_sum(need, warp_sums, &total);
-        if (i < p.count && p.first[i] == 0) p.first[i] = needed + before;
+        if (i < p.count) first[i] = marked ? needed + before : -1;
         needed = total > INT32_MAX - needed ? INT32_MAX : needed + total;
     }
 
     int found = 0;
-    for (int base = 0; base < s.num_pages && found < needed; base += kPlanThreads) {
-        const int page = base + tid;
-        const int free = page < s.num_pages && s.ref_counts[page] == 0;
+    for (int base = 0; base < s.num_pages && found < needed; base += kPlanThreads * kClaimPages) {
+        int free = 0;
+        for (int i = 0; i < kClaimPages; ++i) {
+            const int page = base + tid * kClaimPages + i;
+            free += page < s.num_pages && s.ref_counts[page] == 0;
+        }
         int total = 0;
-        const int rank = found + block_exclusive_sum(free, warp_sums, &total);
-        if (free && rank < needed) p.fresh[rank] = page;
+        block_exclusive_sum(free, warp_sums, &total);
         found += total;
     }
     __syncthreads();
     const int status = invalid ? kClaimInvalid : found < needed ? needed - found : 0;
     if (tid == 0) *p.status = status;
     for (int i = tid; i < p.count; i += kPlanThreads) {
-        const int first = p.first[i];
-        if (first < 0) continue;  // not marked by this entry
+        if (first[i] < 0) continue;
         const int row = p.rows[i];
-        const int len = s.lens[row] & ~kRowMarked;
-        if (status != 0) {
-            s.lens[row] = len;
-        } else if (kFork) {
-            s.lens[row] = p.parent_lens[i];
-            if (p.parent_lens[i] % s.page_size != 0) s.ref_counts[p.fresh[first]] = 1;
-        } else {
-            const int new_len = p.new_lens[i];
-            const int have = pages_of(len, s.page_size);
-            const int more = pages_of(new_len, s.page_size) - have;
-            for (int j = 0; j < more; ++j) {
-                const int page = p.fresh[first + j];
-                s.tables[row * s.table_row + have + j] = page;
-                s.ref_counts[page] = 1;
+        s.lens[row] = status != 0 ? (kFork ? s.lens[row] & ~kRowMarked : base_len[i]) : kFork ? base_len[i] : max(base_len[i], p.new_lens[i]);
+    }
+    if (status != 0) return;
+    // The k-th free page goes to the last row whose first rank is at most k.
+    found = 0;
+    for (int base = 0; found < needed; base += kPlanThreads * kClaimPages) {
+        bool is_free[kClaimPages];
+        int free = 0;
+#pragma unroll
+        for (int i = 0; i < kClaimPages; ++i) {
+            const int page = base + tid * kClaimPages + i;
+            is_free[i] = page < s.num_pages && s.ref_counts[page] == 0;
+            free += is_free[i];
+        }
+        int total = 0;
+        int rank = found + block_exclusive_sum(free, warp_sums, &total);
+        found += total;
+#pragma unroll
+        for (int i = 0; i < kClaimPages; ++i) {
+            if (!is_free[i] || rank >= needed) continue;
+            int lo = 0, hi = p.count - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (first[mid] <= rank) lo = mid;
+                else hi = mid - 1;
             }
-            s.lens[row] = max(len, new_len);
+            const int page = base + tid * kClaimPages + i;
+            const int entry = kFork ? base_len[lo] / s.page_size : pages_of(base_len[lo], s.page_size) + rank - first[lo];
+            s.tables[p.rows[lo] * s.table_row + entry] = page;
+            s.ref_counts[page] = 1;
+            ++rank;
         }
     }
 }
@@ -214,9 +234,6 @@ struct ForkParams {
     PageState state;
     const int32_t* parents;
     const int32_t* children;
-    const int32_t* first;
-    const int32_t* parent_lens;
-    const int32_t* fresh;
     const int32_t* status;
     int64_t page_stride, page_bytes;
 };
@@ -229,19 +246,17 @@ __global__ void __launch_bounds__(kPageCopyThreads) page_fork_kernel(const __gri
     if (*p.status != 0) return;
     const PageState& s = p.state;
     const uint32_t child = blockIdx.x / p.num_caches, cache = blockIdx.x - child * p.num_caches;
-    const int len = p.parent_lens[child];
+    const int row = p.children[child], len = s.lens[row];  // the parent's
     const int whole = len / s.page_size, used = len % s.page_size;
     const int32_t* from = s.tables + p.parents[child] * s.table_row;
-    const int fresh = used != 0 ? p.fresh[p.first[child]] : -1;
+    int32_t* to = s.tables + row * s.table_row;
     if (cache == 0 && p.with_tables) {
-        int32_t* to = s.tables + p.children[child] * s.table_row;
         for (int j = threadIdx.x; j < whole; j += kPageCopyThreads) {
             const int page = from[j];
             to[j] = page;
             if (page >= 0 && page < s.num_pages) atomicAdd(&s.ref_counts[page], 1);
             else atomicOr(&g_fault_word, kFaultIndexOutOfRange);
         }
-        if (used != 0 && threadIdx.x == 0) to[whole] = fresh;
     }
     if (used == 0) return;
     const int last = from[whole];
@@ -249,7 +264,7 @@ __global__ void __launch_bounds__(kPageCopyThreads) page_fork_kernel(const __gri
         if (threadIdx.x == 0) atomicOr(&g_fault_word, kFaultIndexOutOfRange);
         return;
     }
-    copy_page(p.caches.cache[cache], p.page_stride, last, fresh, p.page_bytes);
+    copy_page(p.caches.cache[cache], p.page_stride, last, to[whole], p.page_bytes);
 }
 
 // ---- releasing ---------------------------------------------------------------------------------

@@ -30,7 +30,7 @@ constexpr int kMaxDevices = 64;
 struct DeviceInfo {
     std::atomic<int> sm_count{0};
     std::atomic<int> max_smem_optin{0};
-    std::atomic<uint32_t> smem_configured{0};  // bit per kernel instance given the shared-memory opt-in
+    std::atomic<uint32_t> smem_configured{0};  // bit per kernel instance given the shared-memory (or cluster-size) opt-in
 };
 DeviceInfo g_devices[kMaxDevices];
 

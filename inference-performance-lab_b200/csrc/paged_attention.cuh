@@ -95,6 +95,12 @@ __device__ __forceinline__ int table_bounded_length(const AttentionParams& p, in
     return len;
 }
 
+// a / b of non-negative numbers, in 32 bits where they fit (a 64-bit division takes several hundred cycles).
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+    if ((a | b) >> 32 == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
+}
+
 __device__ __forceinline__ float warp_max(float value) {
 #pragma unroll
     for (int offset = kWarpSize / 2; offset > 0; offset >>= 1) {
@@ -103,57 +109,79 @@ __device__ __forceinline__ float warp_max(float value) {
     return value;
 }
 
-// Adds the parts: block (c, y) takes 8 rows, one a warp, of those whose first part is in slot 2 c + 1; the others
-// follow in slots 2 (c + 1), 2 (c + 2), ...
-constexpr int kJoinWarps = 8;
-
-template <int kDim>
-__global__ void __launch_bounds__(kJoinWarps * kWarpSize) attention_join_kernel(const AttentionParams p, const AttentionParts parts) {
+// Adds the parts: block (c, y) takes kRows rows of those whose first part is in slot 2 c + 1; the others follow in
+// slots 2 (c + 1), 2 (c + 2), ... kSplit warps share a row's parts, kDim / 32 elements a lane.
+template <int kDim, int kRows, int kSplit>
+__global__ void __launch_bounds__(kRows * kSplit * kWarpSize) attention_join_kernel(const AttentionParams p, const AttentionParts parts) {
+    constexpr int kMine = kDim / kWarpSize;
+    __shared__ float sums[kRows * kSplit][kDim];
+    __shared__ float2 stats[kRows * kSplit];
     grid_dependency_wait();
     grid_launch_dependents();
-    constexpr int kMine = kDim / kWarpSize;
     const int first = 2 * blockIdx.x + 1, ctas = gridDim.x;
     const AttentionPart part = parts.parts[first];
+    const int row0 = blockIdx.y * kRows;
+    if (row0 / parts.tile_rows * parts.tile_tokens + row0 % parts.tile_rows / p.group >= part.tokens) return;
     const int warp = threadIdx.x / kWarpSize, lane = threadIdx.x % kWarpSize;
-    const int row = blockIdx.y * kJoinWarps + warp, in_tile = row % parts.tile_rows;
-    const int token_in_tile = in_tile / p.group, token = row / parts.tile_rows * parts.tile_tokens + token_in_tile;
-    if (token_in_tile >= parts.tile_tokens || token >= part.tokens) return;
-    // The slots of the rows, 32 CTAs at a time, one a lane: those that hold something, up to the last part.
+    const int row = row0 + warp / kSplit, turn = warp % kSplit;
     float m = -INFINITY, l = 0.0f, total[kMine] = {};
+    // The slots, 32 CTAs at a time, one a lane: those that hold something, up to the last part.
     for (int base = blockIdx.x; base < ctas; base += kWarpSize) {
         const int slot = base + lane == static_cast<int>(blockIdx.x) ? first : 2 * (base + lane);
         const bool there = base + lane < ctas && parts.parts[slot].tokens != 0;
         const uint32_t ends = __ballot_sync(0xffffffffu, there && parts.parts[slot].last != 0);
-        const bool mine = there && (ends == 0 || lane < __ffs(ends));
-        const float2 stats = mine ? parts.stats[static_cast<int64_t>(slot) * parts.slot_rows + row] : make_float2(-INFINITY, 0.0f);
-        const float top = fmaxf(m, warp_max(stats.x)), shift = top == -INFINITY ? 0.0f : top;
-        const float keep = exp2_approx(m - shift), add = exp2_approx(stats.x - shift);
-        l = l * keep + warp_sum(stats.y * add);
+        const bool mine = there && (ends == 0 || lane < __ffs(ends)) && lane % kSplit == turn;
+        const int64_t at = static_cast<int64_t>(slot) * parts.slot_rows + row;
+        const float2 own = mine ? parts.stats[at] : make_float2(-INFINITY, 0.0f);
+        const float top = fmaxf(m, warp_max(own.x)), shift = top == -INFINITY ? 0.0f : top;
+        const float keep = exp2_approx(m - shift), add = exp2_approx(own.x - shift);
+        l = l * keep + warp_sum(own.y * add);
+        m = top;
 #pragma unroll
         for (int i = 0; i < kMine; ++i) total[i] *= keep;
         const uint32_t set = __ballot_sync(0xffffffffu, mine);
-        const int count = 32 - __clz(set);
-#pragma unroll 8
-        for (int j = 0; j < count; ++j) {
-            const float f = __shfl_sync(0xffffffffu, add, j);
-            if (!(set >> j & 1u)) continue;
-            const int from = __shfl_sync(0xffffffffu, slot, j);
-            const float* x = parts.sums + (static_cast<int64_t>(from) * parts.slot_rows + row) * kDim + lane * kMine;
 #pragma unroll
-            for (int i = 0; i < kMine; ++i) total[i] += x[i] * f;
+        for (int j = 0; j < kWarpSize / kSplit; ++j) {
+            const int from = j * kSplit + turn;
+            const float f = __shfl_sync(0xffffffffu, add, from);
+            const int64_t there_at = __shfl_sync(0xffffffffu, at, from);
+            if (!(set >> from & 1u)) continue;
+            const float* x = parts.sums + there_at * kDim + lane * kMine;
+            if constexpr (kMine == 4) {
+                const float4 y = *reinterpret_cast<const float4*>(x);
+                total[0] += y.x * f, total[1] += y.y * f, total[2] += y.z * f, total[3] += y.w * f;
+            } else {
+                const float2 y = *reinterpret_cast<const float2*>(x);
+                total[0] += y.x * f, total[1] += y.y * f;
+            }
         }
-        m = top;
         if (ends != 0) break;
     }
+    if constexpr (kSplit > 1) {
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) sums[warp][lane * kMine + i] = total[i];
+        if (lane == 0) stats[warp] = make_float2(m, l);
+        __syncthreads();
+        if (turn != 0) return;
+#pragma unroll
+        for (int w = 1; w < kSplit; ++w) {
+            const float2 other = stats[warp + w];
+            const float top = fmaxf(m, other.x), shift = top == -INFINITY ? 0.0f : top;
+            const float keep = exp2_approx(m - shift), add = exp2_approx(other.x - shift);
+            l = l * keep + other.y * add;
+            m = top;
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) total[i] = total[i] * keep + sums[warp + w][lane * kMine + i] * add;
+        }
+    }
+    const int in_tile = row % parts.tile_rows, token_in_tile = in_tile / p.group;
+    const int token = row / parts.tile_rows * parts.tile_tokens + token_in_tile, d = lane * kMine;
+    if (token_in_tile >= parts.tile_tokens || token >= part.tokens || d >= p.dim) return;
     const float inverse = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    const int d = lane * kMine;
-    if (d >= p.dim) return;
     const int head = part.kv_head * p.group + in_tile - token_in_tile * p.group;
     uint16_t* out = p.out + static_cast<int64_t>(part.token + token) * p.out_token + head * p.out_head + d;
 #pragma unroll
-    for (int i = 0; i < kMine; i += 2) {
-        *reinterpret_cast<uint32_t*>(out + i) = pack_bf16x2(total[i] * inverse, total[i + 1] * inverse);
-    }
+    for (int i = 0; i < kMine; i += 2) *reinterpret_cast<uint32_t*>(out + i) = pack_bf16x2(total[i] * inverse, total[i + 1] * inverse);
 }
 
 // ---- everything else --------------------------------------------------------------------------------

@@ -21,7 +21,7 @@
 namespace ipl {
 
 constexpr int kShortWarps = 4;
-constexpr int kShortCluster = 8;  // CTAs a cluster, at most
+constexpr int kShortCluster = 16;  // CTAs a cluster, at most (above 8 a kernel has to be allowed them)
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -380,7 +380,8 @@ __global__ void __launch_bounds__(kShortThreads, short_ctas(kTiles)) attention_s
     }
 }
 
-constexpr int kShortPairCost = 16;  // of a sequence and key head beside its blocks, in blocks
+constexpr int kShortPairCost = 8;   // of a sequence and key head beside its blocks, in blocks
+constexpr int kShortLeast = 24;     // of a stretch, in blocks: shorter ones cost more parts than they save time
 
 template <int kDim, int kTiles>
 __global__ void __launch_bounds__(kShortThreads, short_ctas(kTiles)) attention_shared_kernel(const AttentionParams p,
@@ -405,8 +406,8 @@ __global__ void __launch_bounds__(kShortThreads, short_ctas(kTiles)) attention_s
     __syncthreads();
     int head_weight = 0;
     for (int w = 0; w < kShortWarps; ++w) head_weight += sums[w];
-    const int64_t all_weight = static_cast<int64_t>(head_weight) * p.kv_heads;
-    const int64_t share_begin = all_weight * blockIdx.x / gridDim.x, share_end = all_weight * (blockIdx.x + 1) / gridDim.x;
+    const int64_t all_weight = static_cast<int64_t>(head_weight) * p.kv_heads, share = max(divide(all_weight + gridDim.x - 1, gridDim.x), int64_t{kShortLeast});
+    const int64_t share_begin = share * blockIdx.x, share_end = min(share_begin + share, all_weight);
     if (share_begin >= share_end) return;
     for (int base = 0, before = 0; base < p.num_seqs; base += kShortThreads) {
         const int w = weight(base + threadIdx.x);
@@ -438,7 +439,7 @@ __global__ void __launch_bounds__(kShortThreads, short_ctas(kTiles)) attention_s
     bool exists = short_sequence(p, seq, s);
     int64_t left = share_end - share_begin;
     const int64_t into = share_begin - static_cast<int64_t>(sums[kShortWarps + 1]) * p.kv_heads;
-    int kv_head = static_cast<int>(into / (s.blocks + kShortPairCost));
+    int kv_head = static_cast<int>(divide(into, s.blocks + kShortPairCost));
     int skip = static_cast<int>(into - static_cast<int64_t>(kv_head) * (s.blocks + kShortPairCost));
     while (left > 0) {
         if (!exists || kv_head == p.kv_heads) {

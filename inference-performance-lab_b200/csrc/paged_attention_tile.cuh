@@ -267,8 +267,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     int head_weight = 0;
     for (int w = 0; w < kTileThreads / kWarpSize; ++w) head_weight += scratch[w];
     const int64_t all_weight = static_cast<int64_t>(head_weight) * a.kv_heads;
-    const int64_t share_begin = all_weight * blockIdx.x / gridDim.x, share_end = all_weight * (blockIdx.x + 1) / gridDim.x;
-    const int begin_head = head_weight > 0 ? static_cast<int>(share_begin / head_weight) : 0;
+    const int64_t share = divide(all_weight + gridDim.x - 1, gridDim.x);
+    const int64_t share_begin = min(share * blockIdx.x, all_weight), share_end = min(share_begin + share, all_weight);
+    const int begin_head = head_weight > 0 ? static_cast<int>(divide(share_begin, head_weight)) : 0;
     int begin_weight = static_cast<int>(share_begin - static_cast<int64_t>(begin_head) * head_weight);
     // The pair the share begins in, and its weight before the share.
     int* const found = scratch + kTileThreads / kWarpSize;

@@ -324,11 +324,6 @@ struct Caches {
 const int32_t* int_ptr(const ts::Tensor& t) { return static_cast<const int32_t*>(t.const_data_ptr()); }
 int32_t* mutable_int_ptr(ts::Tensor& t) { return static_cast<int32_t*>(t.mutable_data_ptr()); }
 
-ts::Tensor pages_workspace(const ts::Tensor& like, int64_t num_pages, int64_t count, size_t* bytes) {
-    raise_on_error(ipl_pages_workspace(num_pages, count, bytes));
-    return new_ints(like, static_cast<int64_t>(*bytes / sizeof(int32_t)));
-}
-
 }  // namespace
 
 void rotary_embedding_cuda(const ts::Tensor& positions, ts::Tensor& query, ts::Tensor& key,
@@ -462,11 +457,9 @@ ts::Tensor reserve_pages_cuda(ts::Tensor& block_tables, ts::Tensor& seq_lens, ts
     pool.page_size = page_size;
     const int32_t device = block_tables.get_device_index();
     const ts::accelerator::DeviceGuard device_guard(device);
-    size_t bytes = 0;
-    ts::Tensor workspace = pages_workspace(block_tables, pool.num_pages, rows.size(0), &bytes);
     ts::Tensor status = new_ints(block_tables, 1);
-    raise_on_error(ipl_reserve_pages(&pool, int_ptr(rows), int_ptr(new_lens), rows.size(0), workspace.mutable_data_ptr(),
-                                     bytes, mutable_int_ptr(status), current_stream(device)));
+    raise_on_error(ipl_reserve_pages(&pool, int_ptr(rows), int_ptr(new_lens), rows.size(0), mutable_int_ptr(status),
+                                     current_stream(device)));
     return status;
 }
 
@@ -483,11 +476,9 @@ ts::Tensor fork_sequences_cuda(std::vector<ts::Tensor> caches, ts::Tensor& block
     STD_TORCH_CHECK(c.num_pages == pool.num_pages, "ref_counts must have a count for each page of the caches");
     pool.page_size = c.page_size;
     const ts::accelerator::DeviceGuard device_guard(device);
-    size_t bytes = 0;
-    ts::Tensor workspace = pages_workspace(block_tables, pool.num_pages, parents.size(0), &bytes);
     ts::Tensor status = new_ints(block_tables, 1);
     raise_on_error(ipl_fork_sequences(&c.args, &pool, int_ptr(parents), int_ptr(children), parents.size(0),
-                                      workspace.mutable_data_ptr(), bytes, mutable_int_ptr(status), current_stream(device)));
+                                      mutable_int_ptr(status), current_stream(device)));
     return status;
 }
 
@@ -520,7 +511,8 @@ void compact_pages_cuda(std::vector<ts::Tensor> caches, const ts::Tensor& block_
     pool.page_size = c.page_size;
     const ts::accelerator::DeviceGuard device_guard(device);
     size_t bytes = 0;
-    ts::Tensor workspace = pages_workspace(block_tables, pool.num_pages, 0, &bytes);
+    raise_on_error(ipl_compact_pages_workspace(pool.num_pages, &bytes));
+    ts::Tensor workspace = new_ints(block_tables, static_cast<int64_t>(bytes / sizeof(int32_t)));
     raise_on_error(ipl_compact_pages(&c.args, &pool, mutable_int_ptr(new_block_tables), mutable_int_ptr(new_ref_counts),
                                      mutable_int_ptr(live), workspace.mutable_data_ptr(), bytes, current_stream(device)));
 }

@@ -130,7 +130,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [ctypes.POINTER(PagedAttentionArgs), ctypes.POINTER(ctypes.c_size_t)],
     ),
     "ipl_paged_attention_plan": (ctypes.c_char_p, [ctypes.POINTER(PagedAttentionArgs)]),
-    "ipl_pages_workspace": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, ctypes.POINTER(ctypes.c_size_t)]),
+    "ipl_compact_pages_workspace": (ctypes.c_int, [ctypes.c_int64, ctypes.POINTER(ctypes.c_size_t)]),
     "ipl_copy_pages": (
         ctypes.c_int,
         [ctypes.POINTER(PageCaches), ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p],
@@ -143,8 +143,6 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             ctypes.c_void_p,
             ctypes.c_int64,
             ctypes.c_void_p,
-            ctypes.c_size_t,
-            ctypes.c_void_p,
             ctypes.c_void_p,
         ],
     ),
@@ -156,8 +154,6 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             ctypes.c_void_p,
             ctypes.c_void_p,
             ctypes.c_int64,
-            ctypes.c_void_p,
-            ctypes.c_size_t,
             ctypes.c_void_p,
             ctypes.c_void_p,
         ],
@@ -314,9 +310,9 @@ def paged_attention_plan(args: PagedAttentionArgs) -> str:
     return library().ipl_paged_attention_plan(ctypes.byref(args)).decode()
 
 
-def pages_workspace(num_pages: int, count: int) -> int:
+def compact_pages_workspace(num_pages: int) -> int:
     size = ctypes.c_size_t(0)
-    _check(library().ipl_pages_workspace(num_pages, count, ctypes.byref(size)))
+    _check(library().ipl_compact_pages_workspace(num_pages, ctypes.byref(size)))
     return size.value
 
 
@@ -330,20 +326,9 @@ def copy_pages(caches: PageCaches, num_pages: int, pairs_ptr: int, count: int, s
 
 
 def reserve_pages(
-    pool: PagePool,
-    rows_ptr: int,
-    new_lens_ptr: int,
-    count: int,
-    workspace_ptr: int,
-    workspace_bytes: int,
-    status_ptr: int,
-    stream: int = 0,
+    pool: PagePool, rows_ptr: int, new_lens_ptr: int, count: int, status_ptr: int, stream: int = 0
 ) -> None:
-    _check(
-        library().ipl_reserve_pages(
-            ctypes.byref(pool), rows_ptr, new_lens_ptr, count, workspace_ptr, workspace_bytes, status_ptr, stream
-        )
-    )
+    _check(library().ipl_reserve_pages(ctypes.byref(pool), rows_ptr, new_lens_ptr, count, status_ptr, stream))
 
 
 def fork_sequences(
@@ -352,15 +337,12 @@ def fork_sequences(
     parents_ptr: int,
     children_ptr: int,
     count: int,
-    workspace_ptr: int,
-    workspace_bytes: int,
     status_ptr: int,
     stream: int = 0,
 ) -> None:
     _check(
         library().ipl_fork_sequences(
-            ctypes.byref(caches), ctypes.byref(pool), parents_ptr, children_ptr, count, workspace_ptr,
-            workspace_bytes, status_ptr, stream
+            ctypes.byref(caches), ctypes.byref(pool), parents_ptr, children_ptr, count, status_ptr, stream
         )
     )
 

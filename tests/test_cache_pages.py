@@ -114,6 +114,15 @@ def test_more_rows_and_pages_than_threads():
 
 
 @gpu
+def test_as_many_rows_as_a_call_takes():
+    require_cuda()
+    d = Device(16384, 2, 20000, 4, layers=1, kv_heads=1, dim=4)
+    d.reserve(list(range(16384)), [i % 8 for i in range(16384)])
+    with pytest.raises(RuntimeError, match="at most 16384"):
+        extension.reserve_pages(d.tables, d.lens, d.refs, d.ints([0] * 16385), d.ints([1] * 16385), 4)
+
+
+@gpu
 def test_many_caches_take_several_launches():
     require_cuda()
     d = Device(4, 4, 12, 8, layers=70)
@@ -250,17 +259,19 @@ def caches(stride=4096, size=4096, bases=(BASE, BASE + 4096)):
 
 
 @pytest.mark.parametrize("call, status, message", [
-    (lambda: capi.reserve_pages(pool(num_rows=-1), BASE, BASE, 1, BASE, 1 << 20, BASE), capi.IPL_ERROR_INVALID_VALUE, "non-negative"),
-    (lambda: capi.reserve_pages(pool(num_pages=2**31), BASE, BASE, 1, BASE, 1 << 20, BASE), capi.IPL_ERROR_TOO_LARGE, "too large"),
-    (lambda: capi.reserve_pages(pool(), 0, BASE, 1, BASE, 1 << 20, BASE), capi.IPL_ERROR_INVALID_VALUE, "non-null"),
-    (lambda: capi.reserve_pages(pool(), BASE, BASE, 1, BASE, 16, BASE), capi.IPL_ERROR_INVALID_VALUE, "workspace is too small"),
-    (lambda: capi.reserve_pages(pool(), BASE, BASE, 1, BASE, 1 << 20, 0), capi.IPL_ERROR_INVALID_VALUE, "status must be non-null"),
+    (lambda: capi.reserve_pages(pool(num_rows=-1), BASE, BASE, 1, BASE), capi.IPL_ERROR_INVALID_VALUE, "non-negative"),
+    (lambda: capi.reserve_pages(pool(num_pages=2**31), BASE, BASE, 1, BASE), capi.IPL_ERROR_TOO_LARGE, "too large"),
+    (lambda: capi.reserve_pages(pool(), 0, BASE, 1, BASE), capi.IPL_ERROR_INVALID_VALUE, "non-null"),
+    (lambda: capi.reserve_pages(pool(), BASE, BASE, 16385, BASE), capi.IPL_ERROR_TOO_LARGE, "at most 16384"),
+    (lambda: capi.compact_pages(caches(), pool(), BASE + 64, BASE + 128, BASE, BASE, 16), capi.IPL_ERROR_INVALID_VALUE,
+     "workspace is too small"),
+    (lambda: capi.reserve_pages(pool(), BASE, BASE, 1, 0), capi.IPL_ERROR_INVALID_VALUE, "status must be non-null"),
     (lambda: capi.release_sequences(pool(ref_counts=0), BASE, 1), capi.IPL_ERROR_INVALID_VALUE, "non-null"),
     (lambda: capi.release_sequences(pool(seq_lens=BASE + 2), BASE, 1), capi.IPL_ERROR_INVALID_VALUE, "4-byte aligned"),
     (lambda: capi.copy_pages(caches(stride=2048), 20, BASE, 1), capi.IPL_ERROR_INVALID_VALUE, "must not overlap"),
     (lambda: capi.copy_pages(caches(size=4088), 20, BASE, 1), capi.IPL_ERROR_MISALIGNED, "16"),
     (lambda: capi.copy_pages(caches(bases=(BASE + 8,)), 20, BASE, 1), capi.IPL_ERROR_MISALIGNED, "16"),
-    (lambda: capi.fork_sequences(caches(), pool(), BASE, 0, 1, BASE, 1 << 20, BASE), capi.IPL_ERROR_INVALID_VALUE, "non-null"),
+    (lambda: capi.fork_sequences(caches(), pool(), BASE, 0, 1, BASE), capi.IPL_ERROR_INVALID_VALUE, "non-null"),
     (lambda: capi.compact_pages(caches(), pool(), BASE, BASE + 64, BASE, BASE, 1 << 20), capi.IPL_ERROR_INVALID_VALUE, "must not alias"),
 ])
 def test_argument_errors(call, status, message):
@@ -270,6 +281,6 @@ def test_argument_errors(call, status, message):
 
 
 def test_workspace_and_empty_calls():
-    assert capi.pages_workspace(100, 7) >= 4 * (100 + 14)
+    assert capi.compact_pages_workspace(100) >= 4 * 300
     capi.copy_pages(caches(), 20, 0, 0)
     capi.release_sequences(pool(), 0, 0)
