@@ -246,7 +246,8 @@ struct AttentionPlan {
     bool tile = false;    // the tile kernel takes the sequences of more than short_rows rows
     int short_rows = 0;
     int tiles = 0;        // short kernels: column tiles of 8 rows; 0: not launched
-    int cluster = 0;      // CTAs a sequence and key head of the short kernel; 0: the shared kernel
+    int cluster = 0;      // CTAs a sequence, key head and row tile of the short kernel; 0: the shared kernel
+    int row_tiles = 1;
     int tile_ctas = 0, shared_ctas = 0;
     size_t tile_workspace = 0, workspace = 0;  // the tile kernel's at the beginning
 };
@@ -275,6 +276,35 @@ AttentionParts attention_parts(void* workspace, int64_t ctas, int slot_rows, int
     return parts;
 }
 
+// Turns of a CTA of the short kernel over `keys` keys, a block a warp.
+int64_t key_turns(int64_t keys) { return (keys + kShortWarps * kAttentionBlock - 1) / (kShortWarps * kAttentionBlock); }
+
+// CTAs of the short kernel that the GPU holds in clusters of this size: a cluster stays within a part of the GPU,
+// which leaves some SMs out (72 clusters of 4 and 36 of 8 took a second wave on 296 places, 116 of 2 did not).
+int64_t short_resident(int tiles, int sm_count, int cluster) {
+    const int64_t places = static_cast<int64_t>(sm_count) * short_ctas(tiles);
+    return cluster == 1 ? places : cluster <= 4 ? places * 7 / 8 : places * 3 / 4;
+}
+
+// CTAs a cluster: as many as the GPU holds of all of them, up to one for each turn.
+int short_cluster(int64_t units, int64_t keys, int tiles, int sm_count) {
+    int cluster = 1;
+    while (cluster < kShortCluster && cluster < key_turns(keys) && units * cluster * 2 <= short_resident(tiles, sm_count, cluster * 2)) {
+        cluster *= 2;
+    }
+    return cluster;
+}
+
+// Estimates of the two kernels' times in ns, within a fifth of those measured at 1-256 tokens a sequence, 1-148
+// sequences and 36-8192 keys (28 and 4 heads of 128).
+int64_t short_time(int64_t units, int64_t keys, int tiles, int sm_count, int cluster) {
+    const int64_t held = short_resident(tiles, sm_count, cluster), waves = (units * cluster + held - 1) / held;
+    return 3000 + waves * (2500 + 1300 * ((key_turns(keys) + cluster - 1) / cluster));
+}
+int64_t tile_time(int64_t pairs, int64_t keys, int sm_count) {
+    return 16000 + 1900 * (pairs * (keys / kTileKeys + 2) / sm_count);
+}
+
 AttentionPlan plan_attention(const ipl_paged_attention_args& a, int sm_count) {
     AttentionPlan plan;
     if (!attention_vectorises(a)) return plan;
@@ -284,19 +314,29 @@ AttentionPlan plan_attention(const ipl_paged_attention_args& a, int sm_count) {
     const int64_t rows = a.max_query_len * group;
     plan.tiles = rows <= 8 ? 1 : 2;
     plan.short_rows = INT_MAX;
+    int64_t keys = a.max_seq_len > 1 ? a.max_seq_len : 1;
+    if (a.window > 0 && a.window + a.max_query_len < keys) keys = a.window + a.max_query_len;
     // TMA takes strides of up to 2^40 bytes and no zero ones.
     const int64_t strides[] = {a.query_token_stride, a.query_head_stride, a.key_cache_page_stride, a.key_cache_token_stride,
                                a.key_cache_head_stride, a.value_cache_page_stride, a.value_cache_token_stride, a.value_cache_head_stride};
     bool mappable = a.num_pages > 0;
     for (const int64_t s : strides) mappable = mappable && s > 0 && s < (INT64_C(1) << 38);
-    if (rows > 16 && group <= kTileRows && mappable) {
-        plan.tile = true;
-        plan.tiles = group <= 8 ? 1 : 2;
-        plan.short_rows = plan.tiles * 8;
-        // Sequences of one length have no short one among them.
-        if (group > 16 || a.num_tokens == a.max_query_len * a.num_seqs) {
-            plan.tiles = 0;
-            plan.short_rows = 0;
+    if (rows > 16) {
+        // Small calls stay with the short kernel, its row tiles side by side.
+        const int64_t most = (rows + 15) / 16, tiles = a.num_tokens * group / 16 + a.num_seqs;
+        const int64_t units = (tiles < most * a.num_seqs ? tiles : most * a.num_seqs) * a.num_kv_heads;
+        const int64_t pairs = (a.num_tokens * group / (2 * kTileRows) + a.num_seqs) * a.num_kv_heads;
+        if (group <= kTileRows && mappable && short_time(units, keys, 2, sm_count, short_cluster(units, keys, 2, sm_count)) > tile_time(pairs, keys, sm_count)) {
+            plan.tile = true;
+            plan.tiles = group <= 8 ? 1 : 2;
+            plan.short_rows = plan.tiles * 8;
+            // Sequences of one length have no short one among them.
+            if (group > 16 || a.num_tokens == a.max_query_len * a.num_seqs) {
+                plan.tiles = 0;
+                plan.short_rows = 0;
+            }
+        } else {
+            plan.row_tiles = static_cast<int>(most < 4096 ? most : 4096);
         }
     }
     if (plan.tile) {
@@ -305,15 +345,12 @@ AttentionPlan plan_attention(const ipl_paged_attention_args& a, int sm_count) {
         plan.workspace = plan.tile_workspace;
     }
     if (plan.tiles > 0) {
-        // A cluster for each sequence and key head where the GPU holds all of them and no warp has more than 16
-        // blocks of keys; otherwise equal shares.
-        int64_t keys = a.max_seq_len > 1 ? a.max_seq_len : 1;
-        if (a.window > 0 && a.window + a.max_query_len < keys) keys = a.window + a.max_query_len;
-        const int64_t pairs = a.num_seqs * a.num_kv_heads, resident = static_cast<int64_t>(sm_count) * short_ctas(plan.tiles);
-        const int64_t turns = (keys + kShortWarps * kAttentionBlock - 1) / (kShortWarps * kAttentionBlock);
-        plan.cluster = 1;
-        while (plan.cluster < kShortCluster && plan.cluster < turns && pairs * plan.cluster * 2 <= resident) plan.cluster *= 2;
-        if (pairs * plan.cluster > resident || turns > 16 * plan.cluster) {
+        // A cluster for each sequence, key head and row tile where the GPU holds all of them and no warp has more
+        // than 16 blocks of keys; otherwise equal shares (row tiles: clusters all the same, they are not cut).
+        const int64_t units = a.num_seqs * a.num_kv_heads * plan.row_tiles;
+        const int64_t resident = static_cast<int64_t>(sm_count) * short_ctas(plan.tiles);
+        plan.cluster = short_cluster(units, keys, plan.tiles, sm_count);
+        if (plan.row_tiles == 1 && (units * plan.cluster > resident || key_turns(keys) > 16 * plan.cluster)) {
             plan.cluster = 0;
             plan.shared_ctas = static_cast<int>(resident);
             plan.workspace += parts_bytes(plan.shared_ctas, 8 * plan.tiles, plan.dim);
@@ -342,7 +379,9 @@ ipl_status launch_short(const AttentionPlan& plan, const AttentionParams& p, cha
             if (err != cudaSuccess) return fail(IPL_ERROR_CUDA, "paged attention kernel setup failed: %s", cudaGetErrorString(err));
             info->smem_configured.fetch_or(bit, std::memory_order_acq_rel);
         }
-        const unsigned cluster = static_cast<unsigned>(plan.cluster), grid = static_cast<unsigned>(p.num_seqs * p.kv_heads) * cluster;
+        const int64_t ctas = static_cast<int64_t>(p.num_seqs) * p.kv_heads * plan.row_tiles * plan.cluster;
+        if (ctas > INT_MAX) return fail(IPL_ERROR_TOO_LARGE, "too many sequences and heads");
+        const unsigned cluster = static_cast<unsigned>(plan.cluster), grid = static_cast<unsigned>(ctas);
         return launch_status(
             plan.tiles == 1 ? launch_clustered(attention_short_kernel<kDim, 1>, grid, cluster, kShortThreads, 0, stream, p)
                             : launch_clustered(attention_short_kernel<kDim, 2>, grid, cluster, kShortThreads, 0, stream, p),
@@ -424,6 +463,7 @@ ipl_status run_attention(const ipl_paged_attention_args* a, cudaStream_t stream)
         return fail(IPL_ERROR_INVALID_VALUE, "workspace must be non-null and 16-byte aligned");
     }
     p.short_rows = plan.short_rows;
+    p.row_tiles = plan.row_tiles;
     return plan.dim == 64 ? launch_attention<64>(*a, plan, p, info, stream) : launch_attention<128>(*a, plan, p, info, stream);
 }
 

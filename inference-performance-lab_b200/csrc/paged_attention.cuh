@@ -33,6 +33,7 @@ struct AttentionParams {
     // Sequences of at most short_rows rows (new tokens x group) belong to the short kernels, the others
     // to the tile kernel.
     int short_rows;
+    int row_tiles;  // row tiles of a sequence that the short kernel takes at the same time
 };
 
 // Rows whose keys several CTAs share. The CTAs take equal stretches of all the work, laid end to end, so CTA c

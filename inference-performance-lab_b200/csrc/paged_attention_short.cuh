@@ -10,8 +10,8 @@
 //     elements by byte permutes; P^T comes from the score registers by movmatrix.
 // The loads of the next block are issued as soon as the registers are free, keys behind S^T, values behind
 // O^T. The warps of a CTA take blocks in turn and are joined through shared memory. Two kernels share that:
-// * attention_short_kernel: a cluster of 1 to 8 CTAs for each sequence and key head, joined through distributed
-//   shared memory: one launch, no workspace, for small calls;
+// * attention_short_kernel: a cluster of 1 to 16 CTAs for each sequence, key head and tile of rows, joined through
+//   distributed shared memory: one launch, no workspace, for small calls;
 // * attention_shared_kernel: CTAs that fill the GPU once take equal stretches of all the blocks, laid end to end;
 //   rows that a border cuts leave parts for attention_join_kernel. No last wave, whatever the lengths.
 #pragma once
@@ -319,13 +319,13 @@ __global__ void __launch_bounds__(kShortThreads, short_ctas(kTiles)) attention_s
     grid_dependency_wait();
     grid_launch_dependents();
     const uint32_t rank = cluster_ctarank(), ctas = cluster_nctarank();
-    const int pair = blockIdx.x / ctas, seq = pair / p.kv_heads, kv_head = pair - seq * p.kv_heads;
+    const int unit = blockIdx.x / ctas, pair = unit / p.row_tiles, seq = pair / p.kv_heads, kv_head = pair - seq * p.kv_heads;
     ShortSequence s;
     // The CTAs of a cluster leave together.
     if (!short_sequence(p, seq, s)) return;
     const int block_begin = static_cast<int>(static_cast<int64_t>(s.blocks) * rank / ctas);
     const int block_end = static_cast<int>(static_cast<int64_t>(s.blocks) * (rank + 1) / ctas);
-    for (int row0 = 0; row0 < s.rows; row0 += kRows) {
+    for (int row0 = (unit - pair * p.row_tiles) * kRows; row0 < s.rows; row0 += p.row_tiles * kRows) {
         short_rows(p, s, seq, kv_head, row0, block_begin, block_end, shared);
         for (int e = threadIdx.x; e < kRows * (kDim / 4); e += kShortThreads) {
             const int local = e / (kDim / 4), d = e % (kDim / 4) * 4;

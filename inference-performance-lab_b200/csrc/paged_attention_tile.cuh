@@ -250,57 +250,75 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     // This CTA's share of the steps: of the pairs of one key head in their order, then of the next head. The
     // items' memory serves the sums. Pair u weighs its steps and kTilePairCost.
     int* const scratch = reinterpret_cast<int*>(at(smem + L::kItemBase));
+    int* const found = scratch + kTileThreads / kWarpSize;  // the pair the share begins in, and its weight before it
     if (threadIdx.x < a.num_seqs) {
         // The searches below go through these one load after the other: bring them near at once.
         asm volatile("prefetch.global.L1 [%0];" ::"l"(a.starts + threadIdx.x));
         asm volatile("prefetch.global.L1 [%0];" ::"l"(a.lens + threadIdx.x));
     }
-    const auto weight = [&](int u) {
-        TilePair pair;
-        return u < p.units && tile_pair(p, u, pair) ? pair.steps + kTilePairCost : 0;
+    const auto weight = [&](int u, TilePair& pair) { return u < p.units && tile_pair(p, u, pair) ? pair.steps + kTilePairCost : 0; };
+    // Sum over the CTA up to and with this thread; `total` gets all of it.
+    const auto sum_through = [&](int value, int& total) {
+        int through = value;
+#pragma unroll
+        for (int offset = 1; offset < kWarpSize; offset *= 2) {
+            const int below = __shfl_up_sync(0xffffffffu, through, offset);
+            if (lane >= offset) through += below;
+        }
+        __syncthreads();
+        if (lane == kWarpSize - 1) scratch[warp] = through;
+        __syncthreads();
+        total = 0;
+        for (int i = 0; i < kTileThreads / kWarpSize; ++i) {
+            if (i == warp) through += total;
+            total += scratch[i];
+        }
+        return through;
     };
-    int sum = 0;
-    for (int u = threadIdx.x; u < p.units; u += kTileThreads) sum += weight(u);
-    sum = __reduce_add_sync(0xffffffffu, sum);
-    if (lane == 0) scratch[warp] = sum;
-    __syncthreads();
-    int head_weight = 0;
-    for (int w = 0; w < kTileThreads / kWarpSize; ++w) head_weight += scratch[w];
+    // In the common case every thread has one pair, whose weight serves both sums.
+    TilePair pair = {};
+    int own = weight(threadIdx.x, pair), more = 0;
+    for (int u = threadIdx.x + kTileThreads; u < p.units; u += kTileThreads) {
+        TilePair other;
+        more += weight(u, other);
+    }
+    int through, head_weight;
+    if (p.units <= kTileThreads) {
+        through = sum_through(own, head_weight);
+    } else {
+        sum_through(own + more, head_weight);
+    }
     const int64_t all_weight = static_cast<int64_t>(head_weight) * a.kv_heads;
     const int64_t share = divide(all_weight + gridDim.x - 1, gridDim.x);
     const int64_t share_begin = min(share * blockIdx.x, all_weight), share_end = min(share_begin + share, all_weight);
     const int begin_head = head_weight > 0 ? static_cast<int>(divide(share_begin, head_weight)) : 0;
     int begin_weight = static_cast<int>(share_begin - static_cast<int64_t>(begin_head) * head_weight);
-    // The pair the share begins in, and its weight before the share.
-    int* const found = scratch + kTileThreads / kWarpSize;
-    if (share_begin < share_end) {
-        for (int base = 0, before = 0; base < p.units; base += kTileThreads) {
-            const int w = weight(base + threadIdx.x);
-            int through = w;
-#pragma unroll
-            for (int offset = 1; offset < kWarpSize; offset *= 2) {
-                const int below = __shfl_up_sync(0xffffffffu, through, offset);
-                if (lane >= offset) through += below;
-            }
-            __syncthreads();
-            if (lane == kWarpSize - 1) scratch[warp] = through;
-            __syncthreads();
-            int total = before;
-            for (int i = 0; i < kTileThreads / kWarpSize; ++i) {
-                if (i == warp) through += total;
-                total += scratch[i];
-            }
-            if (begin_weight < through && begin_weight >= through - w) {
-                found[0] = base + threadIdx.x;
-                found[1] = begin_weight - (through - w);
-            }
-            before = total;
-            if (begin_weight < total) break;
+    for (int base = 0, before = 0; share_begin < share_end && base < p.units; base += kTileThreads) {
+        int total = 0;
+        if (p.units > kTileThreads) {
+            own = weight(base + threadIdx.x, pair);
+            through = before + sum_through(own, total);
         }
-        __syncthreads();
+        if (begin_weight < through && begin_weight >= through - own) {
+            found[0] = base + threadIdx.x;
+            found[1] = begin_weight - (through - own);
+        }
+        before += total;
+        if (begin_weight < before) break;
     }
+    // The pairs from there on, for the warp that hands out the work: in the last stage, which is loaded into later.
+    TilePair* const first_pairs = reinterpret_cast<TilePair*>(at(smem + L::kStageBase + (L::kStages - 1) * L::kTileBytes));
+    __syncthreads();
     const int begin_unit = found[0];
     begin_weight = found[1];
+    if (p.units <= kTileThreads && share_begin < share_end) {
+        const int place = static_cast<int>(threadIdx.x) - begin_unit;
+        if (place >= 0 && place < kWarpSize) {
+            pair.seq = own > 0 ? pair.seq : -1;
+            first_pairs[place] = pair;
+        }
+    }
+    fence_async_shared();
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
@@ -336,7 +354,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             if (base >= p.units) base = 0, ++head;
             if (head >= a.kv_heads) break;
             TilePair pair = {};
-            const bool exists = tile_pair(p, base + lane, pair);
+            bool exists;
+            if (base == begin_unit && head == begin_head && p.units <= kTileThreads) {
+                pair = first_pairs[lane];
+                exists = base + lane < kTileThreads && pair.seq >= 0;
+            } else {
+                exists = tile_pair(p, base + lane, pair);
+            }
             for (uint32_t set = __ballot_sync(0xffffffffu, exists); set != 0 && left > 0 && ok; set &= set - 1) {
                 const int from = __ffs(set) - 1;
                 const int steps = __shfl_sync(0xffffffffu, pair.steps, from), weight = steps + kTilePairCost;
@@ -706,46 +730,45 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             if (!ok) break;
             const float inverse = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
             const int r = row(), in_tile = row_token(r);
-            const uint32_t real = __ballot_sync(0xffffffffu, in_tile < p.tile_tokens && t * p.tile_tokens + in_tile < item.tokens);
+            const bool real = in_tile < p.tile_tokens && t * p.tile_tokens + in_tile < item.tokens;
             const int slot = item.slot;
             const int64_t part = static_cast<int64_t>(slot) * (2 * kTileRows) + t * kTileRows + r;
             if (slot >= 0) p.parts.stats[part] = make_float2(top, sum);
-            // Bytes of this thread's row; the rows of the eight threads that share their rows' chunks.
+            // Byte offset of this thread's row (-1: padding), which the eight threads that share their rows' chunks need.
             const int64_t mine = slot >= 0 ? part * (kDim * 4)
+                                 : !real   ? -1
                                            : 2 * (static_cast<int64_t>(item.token + t * p.tile_tokens + in_tile) * a.out_token +
                                                   (item.kv_head * a.group + r - in_tile * a.group) * a.out_head);
             char* const to = (slot >= 0 ? reinterpret_cast<char*>(p.parts.sums) : reinterpret_cast<char*>(a.out)) + 16 * (lane & 7);
-            const int columns = slot >= 0 ? 32 : 64;  // of a pass: 128 bytes a row
-            for (int c = 0; c < kDim; c += columns) {
+            const int columns = slot >= 0 ? 32 : 64, width = 128 / columns;  // of a pass: 128 bytes a row
+            if (item.steps == 0 && real) {  // rows that see nothing
+                for (int d = 0; d < a.dim; d += 8) st_v4(reinterpret_cast<char*>(a.out) + mine + 2 * d, U32x4{});
+            }
+            for (int c = 0; c < kDim && item.steps > 0; c += columns) {
                 uint32_t v[32];
-                if (item.steps == 0) {
+                tmem_load_32(o_tmem + c, reinterpret_cast<float(&)[32]>(v));
+                tmem_wait_loads();
+                if (slot < 0) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = 0;
-                } else {
-                    tmem_load_32(o_tmem + c, reinterpret_cast<float(&)[32]>(v));
+                    for (int i = 0; i < 16; ++i) {
+                        v[i] = pack_bf16x2(__uint_as_float(v[2 * i]) * inverse, __uint_as_float(v[2 * i + 1]) * inverse);
+                    }
+                    uint32_t high[32];
+                    tmem_load_32(o_tmem + c + 32, reinterpret_cast<float(&)[32]>(high));
                     tmem_wait_loads();
-                    if (slot < 0) {
-                        uint32_t high[32];
-                        tmem_load_32(o_tmem + c + 32, reinterpret_cast<float(&)[32]>(high));
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            v[i] = pack_bf16x2(__uint_as_float(v[2 * i]) * inverse, __uint_as_float(v[2 * i + 1]) * inverse);
-                        }
-                        tmem_wait_loads();
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            v[16 + i] = pack_bf16x2(__uint_as_float(high[2 * i]) * inverse, __uint_as_float(high[2 * i + 1]) * inverse);
-                        }
+                    for (int i = 0; i < 16; ++i) {
+                        v[16 + i] = pack_bf16x2(__uint_as_float(high[2 * i]) * inverse, __uint_as_float(high[2 * i + 1]) * inverse);
                     }
                 }
                 transpose_chunks(v, lane);
-                const bool inside = slot >= 0 || c + 8 * (lane & 7) < a.dim;
+                const int64_t outside = slot >= 0 || c + 8 * (lane & 7) < a.dim ? 0 : -1;
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     const int from = (lane & 24) + k;
                     const int64_t at = __shfl_sync(0xffffffffu, mine, from);
-                    if (inside && (slot >= 0 || (real >> from & 1u))) {
-                        st_v4(to + at + (slot >= 0 ? 4 : 2) * c, U32x4{v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]});
+                    if ((at | outside) >= 0) {
+                        st_v4(to + at + width * c, U32x4{v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]});
                     }
                 }
             }
