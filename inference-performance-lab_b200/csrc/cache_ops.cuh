@@ -359,14 +359,6 @@ AttentionPlan plan_attention(const ipl_paged_attention_args& a, int sm_count) {
     return plan;
 }
 
-// Rows of a join block and warps a row: many pairs of tiles are cut in two or three, few short rows in up to 150.
-template <int kDim, int kRows, int kSplit>
-ipl_status launch_join(const AttentionParams& p, const AttentionParts& parts, int ctas, cudaStream_t stream) {
-    return launch_status(launch_2d(attention_join_kernel<kDim, kRows, kSplit>, static_cast<unsigned>(ctas),
-                                   static_cast<unsigned>(parts.slot_rows / kRows), kRows * kSplit * kWarpSize, stream, p, parts),
-                         "paged attention");
-}
-
 template <int kDim>
 ipl_status launch_short(const AttentionPlan& plan, const AttentionParams& p, char* workspace, DeviceInfo* info, cudaStream_t stream) {
     if (plan.cluster > 0) {
@@ -393,7 +385,9 @@ ipl_status launch_short(const AttentionPlan& plan, const AttentionParams& p, cha
         plan.tiles == 1 ? launch(attention_shared_kernel<kDim, 1>, grid, kShortThreads, 0, stream, p, parts)
                         : launch(attention_shared_kernel<kDim, 2>, grid, kShortThreads, 0, stream, p, parts),
         "paged attention");
-    return st == IPL_SUCCESS ? launch_join<kDim, 2, 8>(p, parts, plan.shared_ctas, stream) : st;
+    if (st != IPL_SUCCESS) return st;
+    return launch_status(launch_2d(attention_join_parts_kernel<kDim>, grid, 4u * plan.tiles, 2 * kJoinSplit * kWarpSize, stream, p, parts),
+                         "paged attention");
 }
 
 template <int kDim>
@@ -416,6 +410,7 @@ ipl_status launch_tile(const ipl_paged_attention_args& a, const AttentionPlan& p
     t.pair_tokens = make_fast_div32(static_cast<uint32_t>(2 * t.tile_tokens));
     t.page_size = make_fast_div32(static_cast<uint32_t>(p.page_size));
     t.group_reciprocal = 65536 / p.group + 1;
+    t.wide_out = p.dim % 16 == 0 && (p.out_token | p.out_head) % 16 == 0 && aligned(p.out, 32);
     t.parts = attention_parts(a.workspace, plan.tile_ctas, 2 * kTileRows, kDim, kTileRows, t.tile_tokens);
     CUtensorMap q, k, v;
     const int64_t q_sizes[3] = {p.dim, p.heads, p.num_tokens}, q_strides[2] = {p.q_head, p.q_token};
@@ -432,7 +427,13 @@ ipl_status launch_tile(const ipl_paged_attention_args& a, const AttentionPlan& p
     st = launch_status(launch(attention_tile_kernel<kDim>, ctas, kTileThreads, Layout::kDynamic, stream, t, q, k, v),
                        "paged attention");
     if (st != IPL_SUCCESS) return st;
-    return launch_join<kDim, 8, 1>(p, t.parts, plan.tile_ctas, stream);
+    // Parts a pair, on average at least.
+    const bool split = ctas > 4 * static_cast<int64_t>(t.units) * p.kv_heads;
+    const unsigned blocks = 2 * kTileRows / kJoinRows;
+    return launch_status(split ? launch_2d(attention_join_rows_kernel<kDim, true>, ctas, blocks, kJoinWarps * kWarpSize, stream, p, t.parts)
+                               : launch_2d(attention_join_rows_kernel<kDim, false>, ctas, blocks / kJoinWarps, kJoinWarps * kWarpSize,
+                                           stream, p, t.parts),
+                         "paged attention");
 }
 
 template <int kDim>
@@ -599,12 +600,12 @@ const char* ipl_paged_attention_plan(const ipl_paged_attention_args* args) {
     const AttentionPlan plan = plan_attention(*args, sms);
     if (!plan.vector) return "attention_row_kernel";
     static const char* const kNames[2][5] = {
-        {"invalid", "attention_short_kernel<1>", "attention_short_kernel<2>", "attention_shared_kernel<1> + attention_join_kernel",
-         "attention_shared_kernel<2> + attention_join_kernel"},
-        {"attention_tile_kernel + attention_join_kernel", "attention_tile_kernel + attention_join_kernel + attention_short_kernel<1>",
-         "attention_tile_kernel + attention_join_kernel + attention_short_kernel<2>",
-         "attention_tile_kernel + attention_join_kernel + attention_shared_kernel<1> + attention_join_kernel",
-         "attention_tile_kernel + attention_join_kernel + attention_shared_kernel<2> + attention_join_kernel"}};
+        {"invalid", "attention_short_kernel<1>", "attention_short_kernel<2>", "attention_shared_kernel<1> + attention_join_parts_kernel",
+         "attention_shared_kernel<2> + attention_join_parts_kernel"},
+        {"attention_tile_kernel + attention_join_rows_kernel", "attention_tile_kernel + attention_join_rows_kernel + attention_short_kernel<1>",
+         "attention_tile_kernel + attention_join_rows_kernel + attention_short_kernel<2>",
+         "attention_tile_kernel + attention_join_rows_kernel + attention_shared_kernel<1> + attention_join_parts_kernel",
+         "attention_tile_kernel + attention_join_rows_kernel + attention_shared_kernel<2> + attention_join_parts_kernel"}};
     return kNames[plan.tile ? 1 : 0][plan.tiles == 0 ? 0 : plan.tiles + (plan.cluster > 0 ? 0 : 2)];
 }
 

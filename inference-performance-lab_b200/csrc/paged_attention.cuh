@@ -110,28 +110,141 @@ __device__ __forceinline__ float warp_max(float value) {
     return value;
 }
 
-// Adds the parts: block (c, y) takes kRows rows of those whose first part is in slot 2 c + 1; the others follow in
-// slots 2 (c + 1), 2 (c + 2), ... kSplit warps share a row's parts, kDim / 32 elements a lane.
-template <int kDim, int kRows, int kSplit>
-__global__ void __launch_bounds__(kRows * kSplit * kWarpSize) attention_join_kernel(const AttentionParams p, const AttentionParts parts) {
-    constexpr int kMine = kDim / kWarpSize;
-    __shared__ float sums[kRows * kSplit][kDim];
-    __shared__ float2 stats[kRows * kSplit];
+// Adds the parts. The first of some rows' parts is in slot 2 c + 1; the others follow in slots 2 (c + 1), 2 (c + 2),
+// ..., up to the last, as far as those CTAs have a share. join_slots(base): of the slots of CTAs base to base + 31,
+// one a lane, those that belong to the rows (bits); `last` says whether that is all.
+__device__ __forceinline__ uint32_t join_slots(const AttentionParts& parts, int cta, int base, int lane, int& slot, bool& last) {
+    slot = base + lane == cta ? 2 * cta + 1 : 2 * (base + lane);
+    const bool there = base + lane < static_cast<int>(gridDim.x) && parts.parts[slot].tokens != 0;
+    const uint32_t ends = __ballot_sync(0xffffffffu, there && parts.parts[slot].last != 0);
+    last = ends != 0;
+    return __ballot_sync(0xffffffffu, there && (ends == 0 || lane < __ffs(ends)));
+}
+
+// Output row of row `row` of a slot; null for padding.
+__device__ __forceinline__ uint16_t* join_output(const AttentionParams& p, const AttentionParts& parts, const AttentionPart& part, int row) {
+    const int in_tile = row % parts.tile_rows, token_in_tile = in_tile / p.group;
+    const int token = row / parts.tile_rows * parts.tile_tokens + token_in_tile;
+    if (token_in_tile >= parts.tile_tokens || token >= part.tokens) return nullptr;
+    const int head = part.kv_head * p.group + in_tile - token_in_tile * p.group;
+    return p.out + static_cast<int64_t>(part.token + token) * p.out_token + head * p.out_head;
+}
+
+template <int kMine>
+__device__ __forceinline__ void load_part(const float* from, float (&x)[kMine]) {
+    if constexpr (kMine == 4) {
+        const float4 y = *reinterpret_cast<const float4*>(from);
+        x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
+    } else {
+        const float2 y = *reinterpret_cast<const float2*>(from);
+        x[0] = y.x, x[1] = y.y;
+    }
+}
+
+template <int kMine>
+__device__ __forceinline__ void write_joined(uint16_t* out, float weight, const float (&total)[kMine]) {
+    const float inverse = weight > 0.0f || weight != weight ? 1.0f / weight : 0.0f;
+#pragma unroll
+    for (int i = 0; i < kMine; i += 2) {
+        *reinterpret_cast<uint32_t*>(out + i) = pack_bf16x2(total[i] * inverse, total[i + 1] * inverse);
+    }
+}
+
+// The tile kernel's parts, kDim / 32 elements a lane. Many pairs in few parts each (kSplit false): block (c, y) takes 64
+// rows, a warp 8 of them at once; with a row a warp the blocks were four waves of start-up latency (19 us after 147
+// cut pairs). Few pairs in many parts: block (c, y) takes 8 rows, its warps share the parts (37 parts: 20 us, one after
+// the other 35).
+constexpr int kJoinRows = 8, kJoinWarps = 8;
+
+template <int kDim, bool kSplit>
+__global__ void __launch_bounds__(kJoinWarps * kWarpSize) attention_join_rows_kernel(const AttentionParams p, const AttentionParts parts) {
     grid_dependency_wait();
     grid_launch_dependents();
-    const int first = 2 * blockIdx.x + 1, ctas = gridDim.x;
-    const AttentionPart part = parts.parts[first];
-    const int row0 = blockIdx.y * kRows;
-    if (row0 / parts.tile_rows * parts.tile_tokens + row0 % parts.tile_rows / p.group >= part.tokens) return;
+    constexpr int kMine = kDim / kWarpSize;
+    __shared__ float sums[kSplit ? kJoinWarps : 1][kJoinRows][kDim];
+    __shared__ float2 stats[kSplit ? kJoinWarps : 1][kJoinRows];
     const int warp = threadIdx.x / kWarpSize, lane = threadIdx.x % kWarpSize;
-    const int row = row0 + warp / kSplit, turn = warp % kSplit;
+    const int row0 = (kSplit ? blockIdx.y : blockIdx.y * kJoinWarps + warp) * kJoinRows;
+    const AttentionPart part = parts.parts[2 * blockIdx.x + 1];
+    if (row0 / parts.tile_rows * parts.tile_tokens + row0 % parts.tile_rows / p.group >= part.tokens) return;
+    float m[kJoinRows], l[kJoinRows], total[kJoinRows][kMine] = {};
+#pragma unroll
+    for (int r = 0; r < kJoinRows; ++r) m[r] = -INFINITY, l[r] = 0.0f;
+    bool last = false;
+    int before = 0;
+    for (int base = blockIdx.x; base < static_cast<int>(gridDim.x) && !last; base += kWarpSize) {
+        int slot;
+        for (uint32_t set = join_slots(parts, blockIdx.x, base, lane, slot, last); set != 0; set &= set - 1, ++before) {
+            if (kSplit && before % kJoinWarps != warp) continue;
+            const int64_t at = static_cast<int64_t>(__shfl_sync(0xffffffffu, slot, __ffs(set) - 1)) * parts.slot_rows + row0;
+            const float2 own = lane < kJoinRows ? parts.stats[at + lane] : make_float2(0.0f, 0.0f);
+            float x[kJoinRows][kMine];
+#pragma unroll
+            for (int r = 0; r < kJoinRows; ++r) load_part(parts.sums + (at + r) * kDim + lane * kMine, x[r]);
+#pragma unroll
+            for (int r = 0; r < kJoinRows; ++r) {
+                const float there = __shfl_sync(0xffffffffu, own.x, r), top = fmaxf(m[r], there);
+                const float shift = top == -INFINITY ? 0.0f : top;
+                const float keep = exp2_approx(m[r] - shift), add = exp2_approx(there - shift);
+                m[r] = top;
+                l[r] = l[r] * keep + __shfl_sync(0xffffffffu, own.y, r) * add;
+#pragma unroll
+                for (int i = 0; i < kMine; ++i) total[r][i] = total[r][i] * keep + x[r][i] * add;
+            }
+        }
+    }
+    if constexpr (kSplit) {
+#pragma unroll
+        for (int r = 0; r < kJoinRows; ++r) {
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) sums[warp][r][lane * kMine + i] = total[r][i];
+            if (lane == 0) stats[warp][r] = make_float2(m[r], l[r]);
+        }
+        __syncthreads();
+        // A row a warp.
+        float top = -INFINITY, weight = 0.0f, sum[kMine] = {};
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, stats[w][warp].x);
+        const float shift = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) {
+            const float f = exp2_approx(stats[w][warp].x - shift);
+            weight += f * stats[w][warp].y;
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) sum[i] += f * sums[w][warp][lane * kMine + i];
+        }
+        uint16_t* out = join_output(p, parts, part, row0 + warp);
+        if (out != nullptr && lane * kMine < p.dim) write_joined(out + lane * kMine, weight, sum);
+        return;
+    }
+    if (lane * kMine >= p.dim) return;
+#pragma unroll
+    for (int r = 0; r < kJoinRows; ++r) {
+        uint16_t* out = join_output(p, parts, part, row0 + r);
+        if (out != nullptr) write_joined(out + lane * kMine, l[r], total[r]);
+    }
+}
+
+// Few rows in many parts (the shared kernel's): block (c, y) takes two rows, 8 warps share a row's parts.
+constexpr int kJoinSplit = 8;
+
+template <int kDim>
+__global__ void __launch_bounds__(2 * kJoinSplit * kWarpSize) attention_join_parts_kernel(const AttentionParams p, const AttentionParts parts) {
+    constexpr int kMine = kDim / kWarpSize;
+    __shared__ float sums[2 * kJoinSplit][kDim];
+    __shared__ float2 stats[2 * kJoinSplit];
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const AttentionPart part = parts.parts[2 * blockIdx.x + 1];
+    if (2 * static_cast<int>(blockIdx.y) >= part.tokens * p.group) return;
+    const int warp = threadIdx.x / kWarpSize, lane = threadIdx.x % kWarpSize;
+    const int row = 2 * blockIdx.y + warp / kJoinSplit, turn = warp % kJoinSplit;
     float m = -INFINITY, l = 0.0f, total[kMine] = {};
-    // The slots, 32 CTAs at a time, one a lane: those that hold something, up to the last part.
-    for (int base = blockIdx.x; base < ctas; base += kWarpSize) {
-        const int slot = base + lane == static_cast<int>(blockIdx.x) ? first : 2 * (base + lane);
-        const bool there = base + lane < ctas && parts.parts[slot].tokens != 0;
-        const uint32_t ends = __ballot_sync(0xffffffffu, there && parts.parts[slot].last != 0);
-        const bool mine = there && (ends == 0 || lane < __ffs(ends)) && lane % kSplit == turn;
+    bool last = false;
+    for (int base = blockIdx.x; base < static_cast<int>(gridDim.x) && !last; base += kWarpSize) {
+        int slot;
+        const uint32_t set = join_slots(parts, blockIdx.x, base, lane, slot, last);
+        const bool mine = (set >> lane & 1u) != 0 && lane % kJoinSplit == turn;
         const int64_t at = static_cast<int64_t>(slot) * parts.slot_rows + row;
         const float2 own = mine ? parts.stats[at] : make_float2(-INFINITY, 0.0f);
         const float top = fmaxf(m, warp_max(own.x)), shift = top == -INFINITY ? 0.0f : top;
@@ -140,49 +253,35 @@ __global__ void __launch_bounds__(kRows * kSplit * kWarpSize) attention_join_ker
         m = top;
 #pragma unroll
         for (int i = 0; i < kMine; ++i) total[i] *= keep;
-        const uint32_t set = __ballot_sync(0xffffffffu, mine);
 #pragma unroll
-        for (int j = 0; j < kWarpSize / kSplit; ++j) {
-            const int from = j * kSplit + turn;
+        for (int j = 0; j < kWarpSize / kJoinSplit; ++j) {
+            const int from = j * kJoinSplit + turn;
             const float f = __shfl_sync(0xffffffffu, add, from);
-            const int64_t there_at = __shfl_sync(0xffffffffu, at, from);
+            const int64_t there = __shfl_sync(0xffffffffu, at, from);
             if (!(set >> from & 1u)) continue;
-            const float* x = parts.sums + there_at * kDim + lane * kMine;
-            if constexpr (kMine == 4) {
-                const float4 y = *reinterpret_cast<const float4*>(x);
-                total[0] += y.x * f, total[1] += y.y * f, total[2] += y.z * f, total[3] += y.w * f;
-            } else {
-                const float2 y = *reinterpret_cast<const float2*>(x);
-                total[0] += y.x * f, total[1] += y.y * f;
-            }
-        }
-        if (ends != 0) break;
-    }
-    if constexpr (kSplit > 1) {
+            float x[kMine];
+            load_part(parts.sums + there * kDim + lane * kMine, x);
 #pragma unroll
-        for (int i = 0; i < kMine; ++i) sums[warp][lane * kMine + i] = total[i];
-        if (lane == 0) stats[warp] = make_float2(m, l);
-        __syncthreads();
-        if (turn != 0) return;
-#pragma unroll
-        for (int w = 1; w < kSplit; ++w) {
-            const float2 other = stats[warp + w];
-            const float top = fmaxf(m, other.x), shift = top == -INFINITY ? 0.0f : top;
-            const float keep = exp2_approx(m - shift), add = exp2_approx(other.x - shift);
-            l = l * keep + other.y * add;
-            m = top;
-#pragma unroll
-            for (int i = 0; i < kMine; ++i) total[i] = total[i] * keep + sums[warp + w][lane * kMine + i] * add;
+            for (int i = 0; i < kMine; ++i) total[i] += x[i] * f;
         }
     }
-    const int in_tile = row % parts.tile_rows, token_in_tile = in_tile / p.group;
-    const int token = row / parts.tile_rows * parts.tile_tokens + token_in_tile, d = lane * kMine;
-    if (token_in_tile >= parts.tile_tokens || token >= part.tokens || d >= p.dim) return;
-    const float inverse = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    const int head = part.kv_head * p.group + in_tile - token_in_tile * p.group;
-    uint16_t* out = p.out + static_cast<int64_t>(part.token + token) * p.out_token + head * p.out_head + d;
 #pragma unroll
-    for (int i = 0; i < kMine; i += 2) *reinterpret_cast<uint32_t*>(out + i) = pack_bf16x2(total[i] * inverse, total[i + 1] * inverse);
+    for (int i = 0; i < kMine; ++i) sums[warp][lane * kMine + i] = total[i];
+    if (lane == 0) stats[warp] = make_float2(m, l);
+    __syncthreads();
+    if (turn != 0) return;
+#pragma unroll
+    for (int w = 1; w < kJoinSplit; ++w) {
+        const float2 other = stats[warp + w];
+        const float top = fmaxf(m, other.x), shift = top == -INFINITY ? 0.0f : top;
+        const float keep = exp2_approx(m - shift), add = exp2_approx(other.x - shift);
+        l = l * keep + other.y * add;
+        m = top;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) total[i] = total[i] * keep + sums[warp + w][lane * kMine + i] * add;
+    }
+    uint16_t* out = join_output(p, parts, part, row);
+    if (out != nullptr && lane * kMine < p.dim) write_joined(out + lane * kMine, l, total);
 }
 
 // ---- everything else --------------------------------------------------------------------------------

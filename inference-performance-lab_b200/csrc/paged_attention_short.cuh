@@ -13,7 +13,7 @@
 // * attention_short_kernel: a cluster of 1 to 16 CTAs for each sequence, key head and tile of rows, joined through
 //   distributed shared memory: one launch, no workspace, for small calls;
 // * attention_shared_kernel: CTAs that fill the GPU once take equal stretches of all the blocks, laid end to end;
-//   rows that a border cuts leave parts for attention_join_kernel. No last wave, whatever the lengths.
+//   rows that a border cuts leave parts for attention_join_parts_kernel. No last wave, whatever the lengths.
 #pragma once
 
 #include "paged_attention.cuh"

@@ -11,7 +11,7 @@
 //   warp 9           loads Q, and K and V page by page (TMA), into a ring of shared-memory stages;
 //   warp 10          hands out the work.
 // A CTA on every SM takes an equal share of the steps of all pairs of tiles and key heads, laid end to end;
-// a pair that a share's border cuts leaves parts in the workspace, which attention_join_kernel adds.
+// a pair that a share's border cuts leaves parts in the workspace, which attention_join_rows_kernel adds.
 // Against a CTA for each pair, that evens out the last wave (57 pairs x 4 heads on 148 SMs are 1.54 waves)
 // and hides each pair's first loads behind the pair before.
 // P overwrites the first half of its S; the products are issued in the order P_t V (step j), Q_t K^T (step
@@ -47,6 +47,7 @@ struct TileParams {
     int group_reciprocal;  // 65536 / group + 1: row / group of a row below 128 is the product's high half
     int box_keys;     // keys a TMA box: the largest power of two up to 128 that divides the page size
     int units;        // upper bound of the tile pairs of all sequences
+    int wide_out;     // rows of output are whole 32-byte sectors
     AttentionParts parts;  // of pairs that several CTAs share
 };
 
@@ -99,27 +100,6 @@ __device__ __forceinline__ uint32_t bits_below(int n) { return n >= 32 ? ~0u : n
 __device__ __forceinline__ uint32_t seen_bits(int c, int begin, int end, uint32_t blocks) {
     const uint32_t there = (blocks >> (2 * c) & 1u ? 0x0000ffffu : 0u) | (blocks >> (2 * c) & 2u ? 0xffff0000u : 0u);
     return __brev(there & bits_below(end - 32 * c) & ~bits_below(begin - 32 * c));
-}
-
-// Eight threads of adjacent rows hold eight chunks of 16 bytes of their rows each; afterwards thread j holds chunk
-// j of row k in v[4 k] and on, so that a store of the warp writes 128 bytes of each of four rows. (Every thread
-// storing its own row, 16 or 32 bytes a row and instruction, took 4000-6000 cycles a tile of 128 x 128.)
-__device__ __forceinline__ void transpose_chunks(uint32_t (&v)[32], int lane) {
-#pragma unroll
-    for (int s = 4; s > 0; s /= 2) {
-        const bool upper = lane & s;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (i & s) continue;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                uint32_t &low = v[4 * i + w], &high = v[4 * (i + s) + w];
-                const uint32_t got = __shfl_xor_sync(0xffffffffu, upper ? low : high, s);
-                low = upper ? got : low;
-                high = upper ? high : got;
-            }
-        }
-    }
 }
 
 // The largest of three, NaN if one is.
@@ -289,8 +269,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
         sum_through(own + more, head_weight);
     }
     const int64_t all_weight = static_cast<int64_t>(head_weight) * a.kv_heads;
-    const int64_t share = divide(all_weight + gridDim.x - 1, gridDim.x);
-    const int64_t share_begin = min(share * blockIdx.x, all_weight), share_end = min(share_begin + share, all_weight);
+    const int64_t share_begin = divide(all_weight * blockIdx.x, gridDim.x), share_end = divide(all_weight * (blockIdx.x + 1), gridDim.x);
     const int begin_head = head_weight > 0 ? static_cast<int>(divide(share_begin, head_weight)) : 0;
     int begin_weight = static_cast<int>(share_begin - static_cast<int64_t>(begin_head) * head_weight);
     for (int base = 0, before = 0; share_begin < share_end && base < p.units; base += kTileThreads) {
@@ -734,41 +713,40 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             const int slot = item.slot;
             const int64_t part = static_cast<int64_t>(slot) * (2 * kTileRows) + t * kTileRows + r;
             if (slot >= 0) p.parts.stats[part] = make_float2(top, sum);
-            // Byte offset of this thread's row (-1: padding), which the eight threads that share their rows' chunks need.
-            const int64_t mine = slot >= 0 ? part * (kDim * 4)
-                                 : !real   ? -1
-                                           : 2 * (static_cast<int64_t>(item.token + t * p.tile_tokens + in_tile) * a.out_token +
-                                                  (item.kv_head * a.group + r - in_tile * a.group) * a.out_head);
-            char* const to = (slot >= 0 ? reinterpret_cast<char*>(p.parts.sums) : reinterpret_cast<char*>(a.out)) + 16 * (lane & 7);
-            const int columns = slot >= 0 ? 32 : 64, width = 128 / columns;  // of a pass: 128 bytes a row
-            if (item.steps == 0 && real) {  // rows that see nothing
-                for (int d = 0; d < a.dim; d += 8) st_v4(reinterpret_cast<char*>(a.out) + mine + 2 * d, U32x4{});
-            }
-            for (int c = 0; c < kDim && item.steps > 0; c += columns) {
-                uint32_t v[32];
-                tmem_load_32(o_tmem + c, reinterpret_cast<float(&)[32]>(v));
-                tmem_wait_loads();
-                if (slot < 0) {
+            uint16_t* out = a.out + static_cast<int64_t>(item.token + t * p.tile_tokens + in_tile) * a.out_token +
+                            (item.kv_head * a.group + r - in_tile * a.group) * a.out_head;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        v[i] = pack_bf16x2(__uint_as_float(v[2 * i]) * inverse, __uint_as_float(v[2 * i + 1]) * inverse);
-                    }
-                    uint32_t high[32];
-                    tmem_load_32(o_tmem + c + 32, reinterpret_cast<float(&)[32]>(high));
+            for (int c = 0; c < kDim / 32; ++c) {
+                float o[32] = {};
+                if (item.steps > 0) {
+                    tmem_load_32(o_tmem + 32 * c, o);
                     tmem_wait_loads();
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        v[16 + i] = pack_bf16x2(__uint_as_float(high[2 * i]) * inverse, __uint_as_float(high[2 * i + 1]) * inverse);
-                    }
                 }
-                transpose_chunks(v, lane);
-                const int64_t outside = slot >= 0 || c + 8 * (lane & 7) < a.dim ? 0 : -1;
+                if (!real) continue;
+                // 32 bytes a store, whole sectors. (Chunks exchanged between threads, so that a store of the warp
+                // wrote 128 bytes a row, took as long: the instructions count here, not the sectors.)
+                if (slot >= 0) {
+                    float* to = p.parts.sums + part * kDim + 32 * c;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const int from = (lane & 24) + k;
-                    const int64_t at = __shfl_sync(0xffffffffu, mine, from);
-                    if ((at | outside) >= 0) {
-                        st_v4(to + at + width * c, U32x4{v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]});
+                    for (int i = 0; i < 4; ++i) {
+                        U32x8 v;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) v.v[j] = __float_as_uint(o[8 * i + j]);
+                        st_v8(to + 8 * i, v);
+                    }
+                    continue;
+                }
+                U32x8 v[2];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[i / 8].v[i % 8] = pack_bf16x2(o[2 * i] * inverse, o[2 * i + 1] * inverse);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    uint16_t* to = out + 32 * c + 16 * i;
+                    if (p.wide_out) {
+                        if (32 * c + 16 * i < a.dim) st_v8(to, v[i]);
+                    } else {
+                        if (32 * c + 16 * i < a.dim) st_v4(to, U32x4{v[i].v[0], v[i].v[1], v[i].v[2], v[i].v[3]});
+                        if (32 * c + 16 * i + 8 < a.dim) st_v4(to + 8, U32x4{v[i].v[4], v[i].v[5], v[i].v[6], v[i].v[7]});
                     }
                 }
             }
