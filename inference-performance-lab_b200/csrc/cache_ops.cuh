@@ -80,6 +80,10 @@ template <bool kAppend>
 ipl_status run_rotary(const ipl_rotary_args* a, cudaStream_t stream) {
     const ipl_status st = check_rotary_args(a, kAppend);
     if (st != IPL_SUCCESS || a->num_tokens == 0) return st;
+    int device = 0;
+    DeviceInfo* info = nullptr;
+    const ipl_status found = current_device(&device, &info);
+    if (found != IPL_SUCCESS) return found;
     const bool vector = rotary_vectorises(*a, kAppend);
     RotaryParams p = {};
     p.positions = a->positions;
@@ -117,15 +121,19 @@ ipl_status run_rotary(const ipl_rotary_args* a, cudaStream_t stream) {
         p.items += p.passed_items + kv_heads * static_cast<uint32_t>(v_chunks);
     }
     p.items_div = make_fast_div32(p.items);
-    p.tokens_per_cta = p.items < kRotaryThreads ? kRotaryThreads / p.items : 1;
+    // CTAs of 128 threads once the items are more than about four times the threads the GPU holds.
+    const bool large = a->num_tokens * p.items > 4 * int64_t{kThreadsPerSm} * info->sm_count.load(std::memory_order_relaxed);
+    uint32_t threads = large ? 128 : 256;
+    if (!large && p.items > threads) threads = p.items < kRotaryMaxThreads ? (p.items + 31) / 32 * 32 : kRotaryMaxThreads;
+    p.tokens_per_cta = p.items < threads ? threads / p.items : 1;
     const unsigned grid = (p.tokens + p.tokens_per_cta - 1) / p.tokens_per_cta;
     cudaError_t err;
     if (vector) {
-        err = a->is_neox ? launch(rotary_kernel<true, true, kAppend>, grid, kRotaryThreads, 0, stream, p)
-                         : launch(rotary_kernel<true, false, kAppend>, grid, kRotaryThreads, 0, stream, p);
+        err = a->is_neox ? launch(rotary_kernel<true, true, kAppend>, grid, threads, 0, stream, p)
+                         : launch(rotary_kernel<true, false, kAppend>, grid, threads, 0, stream, p);
     } else {
-        err = a->is_neox ? launch(rotary_kernel<false, true, kAppend>, grid, kRotaryThreads, 0, stream, p)
-                         : launch(rotary_kernel<false, false, kAppend>, grid, kRotaryThreads, 0, stream, p);
+        err = a->is_neox ? launch(rotary_kernel<false, true, kAppend>, grid, threads, 0, stream, p)
+                         : launch(rotary_kernel<false, false, kAppend>, grid, threads, 0, stream, p);
     }
     return launch_status(err, "rotary embedding");
 }

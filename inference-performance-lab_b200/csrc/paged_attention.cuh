@@ -157,7 +157,7 @@ __device__ __forceinline__ void write_joined(uint16_t* out, float weight, const 
 constexpr int kJoinRows = 8, kJoinWarps = 8;
 
 template <int kDim, bool kSplit>
-__global__ void __launch_bounds__(kJoinWarps * kWarpSize) attention_join_rows_kernel(const AttentionParams p, const AttentionParts parts) {
+__global__ void __launch_bounds__(kJoinWarps * kWarpSize, 2) attention_join_rows_kernel(const AttentionParams p, const AttentionParts parts) {
     grid_dependency_wait();
     grid_launch_dependents();
     constexpr int kMine = kDim / kWarpSize;
