@@ -539,6 +539,12 @@ PageState page_state(const ipl_page_pool& pool) {
     return s;
 }
 
+PageLayout page_layout(const ipl_page_caches& c) {
+    PageLayout page = {c.page_stride_bytes, c.page_bytes, (c.page_stride_bytes | c.page_bytes) % 32 == 0};
+    for (int64_t i = 0; i < c.num_caches; ++i) page.wide = page.wide && aligned(c.caches[i], 32);
+    return page;
+}
+
 // The caches from number `from` on, as many as one launch takes.
 int cache_list(const ipl_page_caches& c, int64_t from, CacheList* list) {
     int n = 0;
@@ -637,13 +643,13 @@ ipl_status ipl_copy_pages(const ipl_page_caches* caches, int64_t num_pages, cons
     if (pairs == nullptr || !aligned(pairs, 4)) {
         return fail(IPL_ERROR_INVALID_VALUE, "pairs must be non-null and 4-byte aligned");
     }
+    const PageLayout layout = page_layout(*caches);
     for (int64_t from = 0; from < caches->num_caches; from += kMaxCachesPerLaunch) {
         CopyPagesParams p = {};
         p.num_caches = cache_list(*caches, from, &p.caches);
         p.pairs = pairs;
         p.num_pages = static_cast<int>(num_pages);
-        p.page_stride = caches->page_stride_bytes;
-        p.page_bytes = caches->page_bytes;
+        p.page = layout;
         const unsigned grid = static_cast<unsigned>(count * p.num_caches);
         st = launch_status(launch(page_copy_kernel, grid, kPageCopyThreads, 0, static_cast<cudaStream_t>(stream), p), "page copy");
         if (st != IPL_SUCCESS) return st;
@@ -670,6 +676,7 @@ ipl_status ipl_fork_sequences(const ipl_page_caches* caches, const ipl_page_pool
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     st = launch_claim<true>(claim, s);
     if (st != IPL_SUCCESS || count == 0) return st;
+    const PageLayout layout = page_layout(*caches);
     int64_t from = 0;
     do {
         ForkParams p = {};
@@ -679,12 +686,8 @@ ipl_status ipl_fork_sequences(const ipl_page_caches* caches, const ipl_page_pool
         p.parents = parents;
         p.children = children;
         p.status = status;
-        p.page_stride = caches->page_stride_bytes;
-        p.page_bytes = caches->page_bytes;
-        if (p.num_caches == 0) {  // tables alone
-            p.num_caches = 1;
-            p.page_bytes = 0;
-        }
+        p.page = layout;
+        if (p.num_caches == 0) p.num_caches = 1, p.page.bytes = 0;  // tables alone
         const unsigned grid = static_cast<unsigned>(count * p.num_caches);
         st = launch_status(launch(page_fork_kernel, grid, kPageCopyThreads, 0, s, p), "page fork");
         if (st != IPL_SUCCESS) return st;
@@ -743,6 +746,7 @@ ipl_status ipl_compact_pages(const ipl_page_caches* caches, const ipl_page_pool*
     plan.moves = plan.movers + pool->num_pages;
     st = launch_status(launch(page_compact_plan_kernel, 1, kPlanThreads, 0, s, plan), "page compaction plan");
     if (st != IPL_SUCCESS) return st;
+    const PageLayout layout = page_layout(*caches);
     int64_t from = 0;
     do {
         CompactMoveParams p = {};
@@ -757,16 +761,15 @@ ipl_status ipl_compact_pages(const ipl_page_caches* caches, const ipl_page_pool*
         p.map = plan.map;
         p.holes = plan.holes;
         p.movers = plan.movers;
-        p.page_stride = caches->page_stride_bytes;
-        p.page_bytes = caches->page_bytes;
+        p.page = layout;
         // At most half the pages move; the kernel's loop covers what the grid does not.
         const int64_t most = pool->num_pages / 2 * p.num_caches;
-        const int64_t entries = (pool->num_rows * pool->width + kPageCopyThreads - 1) / kPageCopyThreads;
+        const int64_t entries = (pool->num_rows * pool->width + kPageMoveThreads - 1) / kPageMoveThreads;
         const int64_t cap = static_cast<int64_t>(info->sm_count.load(std::memory_order_relaxed)) * 8;
         int64_t grid = most > entries ? most : entries;
         grid = grid < 1 ? 1 : grid > cap ? cap : grid;
-        if (p.num_caches == 0) p.num_caches = 1, p.page_bytes = 0;
-        st = launch_status(launch(page_compact_move_kernel, static_cast<unsigned>(grid), kPageCopyThreads, 0, s, p),
+        if (p.num_caches == 0) p.num_caches = 1, p.page.bytes = 0;
+        st = launch_status(launch(page_compact_move_kernel, static_cast<unsigned>(grid), kPageMoveThreads, 0, s, p),
                            "page compaction");
         if (st != IPL_SUCCESS) return st;
         from += kMaxCachesPerLaunch;

@@ -12,7 +12,8 @@ namespace ipl {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / kWarpSize;
-constexpr int kPageCopyThreads = 256;
+constexpr int kPageCopyThreads = 128;  // a CTA a page
+constexpr int kPageMoveThreads = 256;  // CTAs that take pages in turn (377 MB moved: 130 us, with 128 threads 139)
 constexpr int kReleaseThreads = 128;
 constexpr int kMaxCachesPerLaunch = 128;
 
@@ -188,21 +189,39 @@ __global__ void __launch_bounds__(kPlanThreads) page_claim_kernel(const ClaimPar
 
 // ---- copying pages -----------------------------------------------------------------------------
 
-// `bytes` (a multiple of 16) from one page to another of one cache.
-__device__ __forceinline__ void copy_page(char* cache, int64_t page_stride, int from, int to, int64_t bytes) {
-    const char* src = cache + from * page_stride;
-    char* dst = cache + to * page_stride;
-    constexpr int kUnroll = 4;
-    constexpr int64_t kStep = int64_t{kPageCopyThreads} * 16;
-    int64_t at = int64_t{threadIdx.x} * 16;
-    for (; at + (kUnroll - 1) * kStep < bytes; at += kUnroll * kStep) {
-        U32x4 v[kUnroll];
+// `bytes` from one page to another of one cache, by the whole CTA: HBM-bound. Two 32-byte accesses a thread in flight
+// where pages allow them (`wide`), else four of 16 bytes. At 96 pages of 64 KB in 56 caches (704 MB read and written)
+// CTAs of 128 threads a page took 114 us, 6.2 TB/s; with 16-byte accesses 126, with four 32-byte ones 117.
+template <typename Vec, int kUnroll>
+__device__ __forceinline__ void copy_vectors(const char* src, char* dst, int64_t bytes) {
+    const int64_t step = static_cast<int64_t>(blockDim.x) * sizeof(Vec);
+    const auto load = [](const char* p) {
+        if constexpr (sizeof(Vec) == 32) return ld_v8(p);
+        else return ld_v4(p);
+    };
+    const auto store = [](char* p, const Vec& v) {
+        if constexpr (sizeof(Vec) == 32) st_v8(p, v);
+        else st_v4(p, v);
+    };
+    int64_t at = threadIdx.x * sizeof(Vec);
+    for (; at + (kUnroll - 1) * step < bytes; at += kUnroll * step) {
+        Vec v[kUnroll];
 #pragma unroll
-        for (int i = 0; i < kUnroll; ++i) v[i] = ld_v4(src + at + i * kStep);
+        for (int i = 0; i < kUnroll; ++i) v[i] = load(src + at + i * step);
 #pragma unroll
-        for (int i = 0; i < kUnroll; ++i) st_v4(dst + at + i * kStep, v[i]);
+        for (int i = 0; i < kUnroll; ++i) store(dst + at + i * step, v[i]);
     }
-    for (; at < bytes; at += kStep) st_v4(dst + at, ld_v4(src + at));
+    for (; at < bytes; at += step) store(dst + at, load(src + at));
+}
+struct PageLayout {
+    int64_t stride, bytes;  // multiples of 16
+    bool wide;              // and of 32, with bases alike
+};
+__device__ __forceinline__ void copy_page(char* cache, const PageLayout& page, int from, int to) {
+    const char* src = cache + from * page.stride;
+    char* dst = cache + to * page.stride;
+    if (page.wide) copy_vectors<U32x8, 2>(src, dst, page.bytes);
+    else copy_vectors<U32x4, 4>(src, dst, page.bytes);
 }
 
 struct CopyPagesParams {
@@ -210,7 +229,7 @@ struct CopyPagesParams {
     int num_caches;
     const int32_t* pairs;  // [count, 2]: source, target
     int num_pages;
-    int64_t page_stride, page_bytes;
+    PageLayout page;
 };
 
 // A CTA for each pair and cache.
@@ -224,7 +243,7 @@ __global__ void __launch_bounds__(kPageCopyThreads) page_copy_kernel(const __gri
         if (threadIdx.x == 0) atomicOr(&g_fault_word, kFaultIndexOutOfRange);
         return;
     }
-    copy_page(p.caches.cache[cache], p.page_stride, from, to, p.page_bytes);
+    copy_page(p.caches.cache[cache], p.page, from, to);
 }
 
 struct ForkParams {
@@ -235,7 +254,7 @@ struct ForkParams {
     const int32_t* parents;
     const int32_t* children;
     const int32_t* status;
-    int64_t page_stride, page_bytes;
+    PageLayout page;
 };
 
 // A CTA for each child and cache: the child takes the parent's whole pages (one more reference each)
@@ -264,7 +283,7 @@ __global__ void __launch_bounds__(kPageCopyThreads) page_fork_kernel(const __gri
         if (threadIdx.x == 0) atomicOr(&g_fault_word, kFaultIndexOutOfRange);
         return;
     }
-    copy_page(p.caches.cache[cache], p.page_stride, last, to[whole], p.page_bytes);
+    copy_page(p.caches.cache[cache], p.page, last, to[whole]);
 }
 
 // ---- releasing ---------------------------------------------------------------------------------
@@ -356,17 +375,17 @@ struct CompactMoveParams {
     const int32_t* map;
     const int32_t* holes;
     const int32_t* movers;
-    int64_t page_stride, page_bytes;
+    PageLayout page;
 };
 
 // Renumbers the tables and moves the pages, a CTA for each page and cache in turn.
-__global__ void __launch_bounds__(kPageCopyThreads) page_compact_move_kernel(const __grid_constant__ CompactMoveParams p) {
+__global__ void __launch_bounds__(kPageMoveThreads) page_compact_move_kernel(const __grid_constant__ CompactMoveParams p) {
     grid_dependency_wait();
     grid_launch_dependents();
     if (p.tables != nullptr) {
         const int64_t entries = static_cast<int64_t>(p.num_rows) * p.width;
-        for (int64_t e = int64_t{blockIdx.x} * kPageCopyThreads + threadIdx.x; e < entries;
-             e += int64_t{gridDim.x} * kPageCopyThreads) {
+        for (int64_t e = int64_t{blockIdx.x} * kPageMoveThreads + threadIdx.x; e < entries;
+             e += int64_t{gridDim.x} * kPageMoveThreads) {
             const int64_t row = e / p.width, column = e - row * p.width;
             const int page = p.tables[row * p.table_row + column];
             const bool known = page >= 0 && page < p.num_pages;
@@ -376,7 +395,7 @@ __global__ void __launch_bounds__(kPageCopyThreads) page_compact_move_kernel(con
     const int64_t units = static_cast<int64_t>(*p.moves) * p.num_caches;
     for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
         const int64_t move = u / p.num_caches;
-        copy_page(p.caches.cache[u - move * p.num_caches], p.page_stride, p.movers[move], p.holes[move], p.page_bytes);
+        copy_page(p.caches.cache[u - move * p.num_caches], p.page, p.movers[move], p.holes[move]);
     }
 }
 

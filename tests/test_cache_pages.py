@@ -184,6 +184,20 @@ def test_copy_pages(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dim", [8, 24, 1000])
+def test_copy_pages_off_32_bytes(dim):
+    """Pages whose size or base is a multiple of 16 bytes but not of 32; nothing beside them is written."""
+    require_cuda()
+    flat = torch.randint(0, 127, (2 * 9 * dim + 64,), device="cuda", dtype=torch.int32).to(torch.bfloat16)
+    store = flat[8 : 8 + 2 * 9 * dim].view(2, 9, 1, dim)
+    before = flat.clone()
+    extension.copy_pages(list(store.unbind(0)), torch.tensor([[0, 3], [1, 8]], dtype=torch.int32, device="cuda"))
+    expected = before[8 : 8 + 2 * 9 * dim].view(2, 9, 1, dim)
+    expected[:, 3], expected[:, 8] = expected[:, 0], expected[:, 1]
+    assert torch.equal(flat, before)
+
+
+@gpu
 def test_interleaved_caches_and_long_offsets():
     """Layers interleaved page by page in one buffer of more than 2^32 bytes."""
     require_cuda()
