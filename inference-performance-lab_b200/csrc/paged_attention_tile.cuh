@@ -8,7 +8,7 @@
 // with the scores of one tile in the softmax while the tensor core works on the other. Roles:
 //   warps 0-3, 4-7   softmax of tile 0 and 1, a row a thread (a lane of tensor memory): no shuffles;
 //   warp 8           issues the products;
-//   warp 9           loads Q, and K and V page by page (TMA), into a ring of shared-memory stages;
+//   warps 9, 11      load Q and K, and V, page by page (TMA), into a ring of shared-memory stages;
 //   warp 10          hands out the work.
 // A CTA on every SM takes an equal share of the steps of all pairs of tiles and key heads, laid end to end;
 // a pair that a share's border cuts leaves parts in the workspace, which attention_join_rows_kernel adds.
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
         }
         for (int i = 0; i < kTileItems; ++i) {
             mbar_init(item_full + 8 * i, 1);
-            mbar_init(item_empty + 8 * i, 10);
+            mbar_init(item_empty + 8 * i, 11);
         }
         mbar_init(q_empty, 1);
         mbar_init(drain, 1);
@@ -381,13 +381,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
         }
         item.work = 0;
         if (ok) put(item);
-      } else if (warp == 9) {
-        // Producer. Lane l loads box l % boxes, half l / boxes of a stage.
+      } else if (warp == 9 || warp == 11) {
+        // Producers of K (and Q) and of V. Lane l loads box l % boxes, half l / boxes of a stage.
+        const bool keys = warp == 9;
+        const CUtensorMap* const map = keys ? &k_map : &v_map;
         const int boxes = kTileKeys / p.box_keys;
         const uint32_t box_bytes = static_cast<uint32_t>(p.box_keys) * 128u;
         const uint32_t q_bytes = L::kHalves * static_cast<uint32_t>(p.tile_tokens) * a.group * 128u;
         bool ok = true;
-        int loads = 0, q_loads = 0, tile_loads[2] = {0, 0};
+        int loads = keys ? 0 : 1, q_loads = 0, tile_loads[2] = {0, 0};  // the next load: K's are the even ones
         const auto load_q = [&](const volatile TileItem& item) {
             bool free = mbar_poll_bounded(q_empty, (q_loads & 1) ^ 1, abort, kFaultEmptyBarrierTimeout);
             free = __all_sync(0xffffffffu, free);
@@ -416,8 +418,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             if (!ok || item.work == 0) break;
             const int32_t* table = a.tables + item.seq * a.table_row;
             const int len = item.len, first = item.first, steps = item.steps, kv_head = item.kv_head;
-            if (n == 0 && steps > 0) ok = load_q(item);
-            for (int step = 0; step < steps && ok; ++step) {
+            if (keys && n == 0 && steps > 0) ok = load_q(item);
+            for (int step = 0; step < steps && ok; ++step, loads += 2) {
                 const int key0 = item.key0 + step * kTileKeys;
                 const int box = lane % boxes, half = lane / boxes;
                 const int key = key0 + box * p.box_keys;
@@ -436,27 +438,25 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 uint32_t mask = wanted && page < 0 ? ((1u << per_box) - 1u) << (box * per_box) : 0u;
                 mask = ~__reduce_or_sync(0xffffffffu, mask) & kAllBlocks;
                 const uint32_t count = __popc(__ballot_sync(0xffffffffu, page >= 0 && lane < boxes)) * L::kHalves;
-                if (lane == 0) block_masks[(loads / 2) % 8] = mask;
+                if (keys && lane == 0) block_masks[(loads / 2) % 8] = mask;
                 const int in_page = key - key_page * a.page_size;
-                for (int which = 0; which < 2; ++which, ++loads) {
-                    const int stage = loads % L::kStages;
-                    ok = mbar_poll_bounded(stage_empty + 8 * stage, ((loads / L::kStages) & 1) ^ 1, abort, kFaultEmptyBarrierTimeout);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    const uint32_t full = stage_full + 8 * stage;
-                    if (lane == 0) mbar_arrive_expect_tx(full, count * box_bytes);
-                    __syncwarp();
-                    if (page >= 0 && half < L::kHalves) {
-                        const uint32_t dst = smem + L::kStageBase + stage * L::kTileBytes + half * L::kHalfBytes + box * box_bytes;
-                        tma_load_4d(dst, which == 0 ? &k_map : &v_map, 64 * half, kv_head, in_page, page, full);
-                    }
-                    if (step == 0 && which == 0 && n > 0) {
-                        // Q behind the first keys: its place is free when the item before is done with its scores.
-                        ok = load_q(item);
-                        if (!ok) {
-                            ++loads;
-                            break;
-                        }
+                const int stage = loads % L::kStages;
+                ok = mbar_poll_bounded(stage_empty + 8 * stage, ((loads / L::kStages) & 1) ^ 1, abort, kFaultEmptyBarrierTimeout);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const uint32_t full = stage_full + 8 * stage;
+                if (lane == 0) mbar_arrive_expect_tx(full, count * box_bytes);
+                __syncwarp();
+                if (page >= 0 && half < L::kHalves) {
+                    const uint32_t dst = smem + L::kStageBase + stage * L::kTileBytes + half * L::kHalfBytes + box * box_bytes;
+                    tma_load_4d(dst, map, 64 * half, kv_head, in_page, page, full);
+                }
+                if (keys && step == 0 && n > 0) {
+                    // Q behind the first keys: its place is free when the item before is done with its scores.
+                    ok = load_q(item);
+                    if (!ok) {
+                        loads += 2;
+                        break;
                     }
                 }
             }
@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
         }
         if (*abort) {
             // Let every copy issued land before the CTA may leave.
-            for (int i = loads - L::kStages > 0 ? loads - L::kStages : 0; i < loads; ++i) {
+            for (int i = loads - 2; i >= 0 && i > loads - 2 - L::kStages; i -= 2) {
                 mbar_wait_timed(stage_full + 8 * (i % L::kStages), (i / L::kStages) & 1, kFaultCopyDrainTimeout);
             }
 #pragma unroll
