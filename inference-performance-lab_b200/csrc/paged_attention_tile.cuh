@@ -33,7 +33,7 @@ constexpr int kTileThreads = 384;  // three warpgroups, among which the register
 // softmax warpgroups take 208 and the third keeps 88 (64512 again).
 constexpr int kSoftmaxRegisters = 208, kOtherRegisters = 88;
 constexpr int kTileHeadKeys = 96;   // weights of a step handed over first, so that their product begins early
-constexpr int kTilePolynomial = 0;  // of 16 pairs of weights, by the polynomial
+constexpr int kTilePolynomial = 2;  // of 16 pairs of weights, by the polynomial (0: 1 % slower, 4: 2 %, 6: 4 %)
 constexpr int kTileBoxes = kTileKeys / kAttentionBlock;  // boxes of at least 16 keys a tile
 constexpr uint32_t kAllBlocks = (1u << kTileBoxes) - 1u;
 
@@ -193,6 +193,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     volatile int* const abort = reinterpret_cast<volatile int*>(at(tmem_slot + 4));
     // Blocks of 16 keys of a step whose page is in the cache, at its number % 8: the ring is shorter than that.
     volatile uint32_t* const block_masks = reinterpret_cast<volatile uint32_t*>(at(tmem_slot + 8));
+    volatile int* const issued = reinterpret_cast<volatile int*>(at(tmem_slot + 40));  // one past the last load of K and of V, loads of Q's tiles
     volatile TileItem* const items = reinterpret_cast<volatile TileItem*>(at(smem + L::kItemBase));
 
     const int warp = threadIdx.x / kWarpSize, lane = threadIdx.x % kWarpSize;
@@ -216,6 +217,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
         mbar_init(q_empty, 1);
         mbar_init(drain, 1);
         *abort = 0;
+        for (int i = 0; i < 4; ++i) issued[i] = 0;
         fence_mbar_init();
     }
     if (warp == 9 && lane == 0) {
@@ -389,7 +391,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
         const uint32_t box_bytes = static_cast<uint32_t>(p.box_keys) * 128u;
         const uint32_t q_bytes = L::kHalves * static_cast<uint32_t>(p.tile_tokens) * a.group * 128u;
         bool ok = true;
-        int loads = keys ? 0 : 1, q_loads = 0, tile_loads[2] = {0, 0};  // the next load: K's are the even ones
+        int loads = keys ? 0 : 1, q_loads = 0;  // the next load: K's are the even ones
         const auto load_q = [&](const volatile TileItem& item) {
             bool free = mbar_poll_bounded(q_empty, (q_loads & 1) ^ 1, abort, kFaultEmptyBarrierTimeout);
             free = __all_sync(0xffffffffu, free);
@@ -400,13 +402,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             for (int t = 0; t < 2; ++t) {
                 if (t >= tiles) break;
                 if (lane == 0) {
+                    issued[2 + t] = item.tile_items[t] + 1;
                     mbar_arrive_expect_tx(q_full + 8 * t, q_bytes);
                     for (int h = 0; h < L::kHalves; ++h) {
                         tma_load_3d(smem + t * L::kTileBytes + h * L::kHalfBytes, &q_map, 64 * h, head, token + t * p.tile_tokens,
                                     q_full + 8 * t);
                     }
                 }
-                ++tile_loads[t];
             }
             __syncwarp();
             return true;
@@ -440,12 +442,19 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 const uint32_t count = __popc(__ballot_sync(0xffffffffu, page >= 0 && lane < boxes)) * L::kHalves;
                 if (keys && lane == 0) block_masks[(loads / 2) % 8] = mask;
                 const int in_page = key - key_page * a.page_size;
+#ifdef IPL_TEST_TILE_SKIP_LOAD
+                // Test builds: CTA 0 never issues this load, so the waits for it run out.
+                if (blockIdx.x == 0 && loads == IPL_TEST_TILE_SKIP_LOAD) continue;
+#endif
                 const int stage = loads % L::kStages;
                 ok = mbar_poll_bounded(stage_empty + 8 * stage, ((loads / L::kStages) & 1) ^ 1, abort, kFaultEmptyBarrierTimeout);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 const uint32_t full = stage_full + 8 * stage;
-                if (lane == 0) mbar_arrive_expect_tx(full, count * box_bytes);
+                if (lane == 0) {
+                    issued[keys ? 0 : 1] = loads + 1;
+                    mbar_arrive_expect_tx(full, count * box_bytes);
+                }
                 __syncwarp();
                 if (page >= 0 && half < L::kHalves) {
                     const uint32_t dst = smem + L::kStageBase + stage * L::kTileBytes + half * L::kHalfBytes + box * box_bytes;
@@ -462,16 +471,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             }
             if (ok && lane == 0) mbar_arrive(item_empty + 8 * (n % kTileItems));
             __syncwarp();
-        }
-        if (*abort) {
-            // Let every copy issued land before the CTA may leave.
-            for (int i = loads - 2; i >= 0 && i > loads - 2 - L::kStages; i -= 2) {
-                mbar_wait_timed(stage_full + 8 * (i % L::kStages), (i / L::kStages) & 1, kFaultCopyDrainTimeout);
-            }
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                if (tile_loads[t] > 0) mbar_wait_timed(q_full + 8 * t, (tile_loads[t] - 1) & 1, kFaultCopyDrainTimeout);
-            }
         }
       } else if (warp == 8) {
         // Issuer: the whole warp walks, one elected lane issues.
@@ -572,6 +571,25 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
         // No product and no arrival outlives the CTA.
         commit(drain);
         mbar_wait_timed(drain, 0, kFaultCopyDrainTimeout);
+      }
+      __syncwarp();
+      // Once the issuer is through, every copy has landed, unless a wait ran out: then let those issued land before the
+      // CTA leaves, the last load of each stage, K's (even) or V's (odd), and Q's.
+      named_barrier_sync(1, 4 * kWarpSize);
+      if (*abort && threadIdx.x == 8 * kWarpSize) {
+        for (int stage = 0; stage < L::kStages; ++stage) {
+            int last = -1;
+            for (int i = stage; i < max(issued[0], issued[1]); i += L::kStages) {
+#ifdef IPL_TEST_TILE_SKIP_LOAD
+                if (blockIdx.x == 0 && i == IPL_TEST_TILE_SKIP_LOAD) continue;
+#endif
+                if (i < issued[i & 1]) last = i;
+            }
+            if (last >= 0) mbar_wait_timed(stage_full + 8 * stage, (last / L::kStages) & 1, kFaultCopyDrainTimeout);
+        }
+        for (int t = 0; t < 2; ++t) {
+            if (issued[2 + t] > 0) mbar_wait_timed(q_full + 8 * t, (issued[2 + t] - 1) & 1, kFaultCopyDrainTimeout);
+        }
       }
     } else {
       warpgroup_take_registers<kSoftmaxRegisters>();
