@@ -205,6 +205,8 @@ AttentionParams attention_params(const ipl_paged_attention_args& a) {
     p.value_page = a.value_cache_page_stride, p.value_token = a.value_cache_token_stride;
     p.value_head = a.value_cache_head_stride;
     p.scale_log2 = static_cast<float>(a.scale * 1.4426950408889634);
+    p.page_blocks = make_fast_div32(static_cast<uint32_t>(p.page_size >= kAttentionBlock ? p.page_size / kAttentionBlock : 1));
+    p.group_div = make_fast_div32(static_cast<uint32_t>(p.group));
     return p;
 }
 
@@ -290,7 +292,7 @@ int64_t key_turns(int64_t keys) { return (keys + kShortWarps * kAttentionBlock -
 // CTAs of the short kernel that the GPU holds in clusters of this size: a cluster stays within a part of the GPU,
 // which leaves some SMs out (72 clusters of 4 and 36 of 8 took a second wave on 296 places, 116 of 2 did not).
 int64_t short_resident(int tiles, int sm_count, int cluster) {
-    const int64_t places = static_cast<int64_t>(sm_count) * short_ctas(tiles);
+    const int64_t places = static_cast<int64_t>(sm_count) * kShortCtas;
     return cluster == 1 ? places : cluster <= 4 ? places * 7 / 8 : places * 3 / 4;
 }
 
@@ -356,7 +358,7 @@ AttentionPlan plan_attention(const ipl_paged_attention_args& a, int sm_count) {
         // A cluster for each sequence, key head and row tile where the GPU holds all of them and no warp has more
         // than 16 blocks of keys; otherwise equal shares (row tiles: clusters all the same, they are not cut).
         const int64_t units = a.num_seqs * a.num_kv_heads * plan.row_tiles;
-        const int64_t resident = static_cast<int64_t>(sm_count) * short_ctas(plan.tiles);
+        const int64_t resident = static_cast<int64_t>(sm_count) * shared_ctas(plan.tiles);
         plan.cluster = short_cluster(units, keys, plan.tiles, sm_count);
         if (plan.row_tiles == 1 && (units * plan.cluster > resident || key_turns(keys) > 16 * plan.cluster)) {
             plan.cluster = 0;

@@ -11,6 +11,7 @@
 #pragma once
 
 #include "ipl_common.cuh"
+#include "silu_and_mul.cuh"
 
 namespace ipl {
 
@@ -33,6 +34,8 @@ struct AttentionParams {
     // Sequences of at most short_rows rows (new tokens x group) belong to the short kernels, the others
     // to the tile kernel.
     int short_rows;
+    FastDiv32 page_blocks;  // blocks of 16 keys a page (fast kernels)
+    FastDiv32 group_div;
     int row_tiles;  // row tiles of a sequence that the short kernel takes at the same time
 };
 

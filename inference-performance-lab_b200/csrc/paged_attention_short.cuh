@@ -76,8 +76,8 @@ struct ShortShared {
 
 // Rows row0 and on of a sequence against its blocks block_begin to block_end, each warp's maxima, sums of weights
 // and sums in shared memory. The whole CTA; ends with a barrier. kDim: the head size padded to 64 or 128; kTiles:
-// column tiles of 8 rows.
-template <int kDim, int kTiles>
+// column tiles of 8 rows; kBlocks: adjacent blocks a warp takes at once.
+template <int kDim, int kTiles, int kBlocks>
 __device__ __forceinline__ void short_rows(const AttentionParams& p, const ShortSequence& s, int seq, int kv_head, int row0,
                                            int block_begin, int block_end, ShortShared<kDim, kTiles>& shared) {
     constexpr int kRows = 8 * kTiles;
@@ -89,14 +89,14 @@ __device__ __forceinline__ void short_rows(const AttentionParams& p, const Short
     const int32_t* table = p.tables + seq * p.table_row;
     const uint16_t* key_base = p.key_cache + kv_head * p.key_head;
     const uint16_t* value_base = p.value_cache + kv_head * p.value_head;
-    const int blocks_per_page = p.page_size / kAttentionBlock;
 
     // Q: row row0 + 8 n + g.
     uint32_t q[kTiles][kChunks][4];
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
         const int row = row0 + 8 * n + g;
-        const int token = s.begin + row / p.group, head = kv_head * p.group + row % p.group;
+        const int in_seq = static_cast<int>(fast_div(static_cast<uint32_t>(row), p.group_div));
+        const int token = s.begin + in_seq, head = kv_head * p.group + row - in_seq * p.group;
         const uint16_t* src = p.q + token * p.q_token + head * p.q_head;
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
@@ -111,10 +111,10 @@ __device__ __forceinline__ void short_rows(const AttentionParams& p, const Short
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) position[n][j] = s.true_len - s.new_tokens + (row0 + 8 * n + 2 * t + j) / p.group;
+        for (int j = 0; j < 2; ++j) position[n][j] = s.true_len - s.new_tokens + static_cast<int>(fast_div(static_cast<uint32_t>(row0 + 8 * n + 2 * t + j), p.group_div));
     }
-    const int lowest = s.true_len - s.new_tokens + row0 / p.group;
-    const int highest = s.true_len - s.new_tokens + (row0 + kRows - 1) / p.group;
+    const int lowest = s.true_len - s.new_tokens + static_cast<int>(fast_div(static_cast<uint32_t>(row0), p.group_div));
+    const int highest = s.true_len - s.new_tokens + static_cast<int>(fast_div(static_cast<uint32_t>(row0 + kRows - 1), p.group_div));
 
     float o[kTiles][kMmas][4] = {};
     float top[kTiles][2], sum[kTiles][2];
@@ -122,140 +122,171 @@ __device__ __forceinline__ void short_rows(const AttentionParams& p, const Short
     for (int n = 0; n < kTiles; ++n) top[n][0] = top[n][1] = -INFINITY, sum[n][0] = sum[n][1] = 0.0f;
 
     // Page numbers of this warp's next 32 blocks, one a lane.
+    constexpr int kTurn = kShortWarps * kBlocks, kTurns = kWarpSize / kBlocks;
     int pages = -1;
     const auto fetch_pages = [&](int block) {
-        const int mine = block + lane * kShortWarps;
+        const int mine = block + lane / kBlocks * kTurn + lane % kBlocks;
         pages = -1;
         if (mine < block_end) {
-            pages = table[(s.first_block + mine) / blocks_per_page];
+            pages = table[fast_div(static_cast<uint32_t>(s.first_block + mine), p.page_blocks)];
             if (pages < 0 || pages >= p.num_pages) {
                 atomicOr(&g_fault_word, kFaultIndexOutOfRange);
                 pages = -1;
             }
         }
     };
-    uint32_t k[kChunks][2][4];  // chunk, key g or g + 8
-    U32x4 v[kPasses][4];        // half of the row, key 2t, 2t + 1, 2t + 8, 2t + 9
-    const auto load_keys = [&](int block, int page) {
-        const int key0 = (s.first_block + block) * kAttentionBlock;
-        const int64_t at = page * p.key_page + static_cast<int64_t>((s.first_block + block) % blocks_per_page * kAttentionBlock) * p.key_token;
+    const auto in_page = [&](int block) {  // the block's first token in its page
+        const uint32_t number = static_cast<uint32_t>(s.first_block + block);
+        return static_cast<int64_t>(number - fast_div(number, p.page_blocks) * p.page_blocks.divisor) * kAttentionBlock;
+    };
+    uint32_t k[kBlocks][kChunks][2][4];  // chunk, key g or g + 8
+    U32x4 v[kBlocks][kPasses][4];        // half of the row, key 2t, 2t + 1, 2t + 8, 2t + 9
+    const auto load_keys = [&](int block, const int (&page)[kBlocks]) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int key = g + 8 * r;
-            const bool there = page >= 0 && key0 + key < s.len;
-            const uint16_t* src = key_base + at + key * p.key_token;
+        for (int u = 0; u < kBlocks; ++u) {
+            const int key0 = (s.first_block + block + u) * kAttentionBlock;
+            const int64_t at = page[u] * p.key_page + in_page(block + u) * p.key_token;
 #pragma unroll
-            for (int c = 0; c < kChunks; ++c) {
-                const int d = 8 * (t + 4 * c);
-                const U32x4 x = ld_stream_v4_or_zero(src + d, there && d < p.dim);
+            for (int r = 0; r < 2; ++r) {
+                const int key = g + 8 * r;
+                const bool there = page[u] >= 0 && key0 + key < s.len;
+                const uint16_t* src = key_base + at + key * p.key_token;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) k[c][r][i] = x.v[i];
+                for (int c = 0; c < kChunks; ++c) {
+                    const int d = 8 * (t + 4 * c);
+                    const U32x4 x = ld_stream_v4_or_zero(src + d, there && d < p.dim);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) k[u][c][r][i] = x.v[i];
+                }
             }
         }
     };
-    const auto load_values = [&](int block, int page) {
-        const int key0 = (s.first_block + block) * kAttentionBlock;
-        const int64_t at = page * p.value_page + static_cast<int64_t>((s.first_block + block) % blocks_per_page * kAttentionBlock) * p.value_token;
+    const auto load_values = [&](int block, const int (&page)[kBlocks]) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int key = 2 * t + (r & 1) + 4 * (r & 2);
-            // Rows that no token sees may hold anything, NaN included: they count as zeros.
-            const bool there = page >= 0 && key0 + key < s.len && key0 + key >= s.first;
-            const uint16_t* src = value_base + at + key * p.value_token;
+        for (int u = 0; u < kBlocks; ++u) {
+            const int key0 = (s.first_block + block + u) * kAttentionBlock;
+            const int64_t at = page[u] * p.value_page + in_page(block + u) * p.value_token;
 #pragma unroll
-            for (int h = 0; h < kPasses; ++h) {
-                const int d = 64 * h + 8 * g;
-                v[h][r] = ld_stream_v4_or_zero(src + d, there && d < p.dim);
+            for (int r = 0; r < 4; ++r) {
+                const int key = 2 * t + (r & 1) + 4 * (r & 2);
+                // Rows that no token sees may hold anything, NaN included: they count as zeros.
+                const bool there = page[u] >= 0 && key0 + key < s.len && key0 + key >= s.first;
+                const uint16_t* src = value_base + at + key * p.value_token;
+#pragma unroll
+                for (int h = 0; h < kPasses; ++h) {
+                    const int d = 64 * h + 8 * g;
+                    v[u][h][r] = ld_stream_v4_or_zero(src + d, there && d < p.dim);
+                }
             }
         }
     };
 
-    int block = block_begin + warp;
-    int turn = 0;
+    int block = block_begin + warp * kBlocks;
+    int turn = 0, page[kBlocks], next_page[kBlocks];
+    const auto take_pages = [&](int (&to)[kBlocks]) {  // -1 past block_end
+#pragma unroll
+        for (int u = 0; u < kBlocks; ++u) to[u] = __shfl_sync(0xffffffffu, pages, turn * kBlocks + u);
+    };
     fetch_pages(block);
-    int page = __shfl_sync(0xffffffffu, pages, 0);
+    take_pages(page);
     if (block < block_end) {
         load_keys(block, page);
         load_values(block, page);
     }
-    for (; block < block_end; block += kShortWarps) {
-        const int next = block + kShortWarps;
-        turn = (turn + 1) & 31;
+    for (; block < block_end; block += kTurn) {
+        const int next = block + kTurn;
+        turn = (turn + 1) % kTurns;
         if (turn == 0) fetch_pages(next);
-        const int next_page = __shfl_sync(0xffffffffu, pages, turn);
+        take_pages(next_page);
 
-        float score[kTiles][4];
+        float score[kBlocks][kTiles][4];
 #pragma unroll
-        for (int n = 0; n < kTiles; ++n) {
-            float even[4] = {}, odd[4] = {};
+        for (int u = 0; u < kBlocks; ++u) {
 #pragma unroll
-            for (int c = 0; c < kChunks; ++c) {
-                const uint32_t a0[4] = {k[c][0][0], k[c][1][0], k[c][0][1], k[c][1][1]};
-                const uint32_t a1[4] = {k[c][0][2], k[c][1][2], k[c][0][3], k[c][1][3]};
-                mma_bf16(even, a0, q[n][c][0], q[n][c][1]);
-                mma_bf16(odd, a1, q[n][c][2], q[n][c][3]);
+            for (int n = 0; n < kTiles; ++n) {
+                float even[4] = {}, odd[4] = {};
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c) {
+                    const uint32_t a0[4] = {k[u][c][0][0], k[u][c][1][0], k[u][c][0][1], k[u][c][1][1]};
+                    const uint32_t a1[4] = {k[u][c][0][2], k[u][c][1][2], k[u][c][0][3], k[u][c][1][3]};
+                    mma_bf16(even, a0, q[n][c][0], q[n][c][1]);
+                    mma_bf16(odd, a1, q[n][c][2], q[n][c][3]);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) score[u][n][i] = (even[i] + odd[i]) * p.scale_log2;
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) score[n][i] = (even[i] + odd[i]) * p.scale_log2;
         }
         if (next < block_end) load_keys(next, next_page);
 
-        const int key0 = (s.first_block + block) * kAttentionBlock;
-        // score[n][2 r + j]: key g + 8 r, row 2t + j.
-        if (page < 0 || key0 + kAttentionBlock > min(lowest + 1, s.len) || highest - key0 >= p.window) {
+        // score[u][n][2 r + j]: key g + 8 r of block u, row 2t + j.
 #pragma unroll
-            for (int n = 0; n < kTiles; ++n) {
+        for (int u = 0; u < kBlocks; ++u) {
+            const int key0 = (s.first_block + block + u) * kAttentionBlock;
+            if (page[u] < 0 || key0 + kAttentionBlock > min(lowest + 1, s.len) || highest - key0 >= p.window) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int key = key0 + g + 4 * (i & 2), at = position[n][i & 1];
-                    if (page < 0 || key >= s.len || key > at || at - key >= p.window) score[n][i] = -INFINITY;
+                for (int n = 0; n < kTiles; ++n) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = key0 + g + 4 * (i & 2), at = position[n][i & 1];
+                        if (page[u] < 0 || key >= s.len || key > at || at - key >= p.window) score[u][n][i] = -INFINITY;
+                    }
                 }
             }
         }
-        uint32_t weights[kTiles][2];
+        uint32_t weights[kBlocks][kTiles][2];
 #pragma unroll
         for (int n = 0; n < kTiles; ++n) {
             float keep[2], shift[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                float m = fmaxf(score[n][j], score[n][2 + j]);
+                float m = top[n][j];
+#pragma unroll
+                for (int u = 0; u < kBlocks; ++u) m = fmaxf(m, fmaxf(score[u][n][j], score[u][n][2 + j]));
 #pragma unroll
                 for (int offset = 4; offset < kWarpSize; offset *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, offset));
-                m = fmaxf(m, top[n][j]);
                 shift[j] = m == -INFINITY ? 0.0f : m;
                 keep[j] = exp2_approx(top[n][j] - shift[j]);
                 top[n][j] = m;
+                sum[n][j] *= keep[j];
             }
-            float w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = exp2_approx(score[n][i] - shift[i & 1]);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) sum[n][j] = sum[n][j] * keep[j] + (w[j] + w[2 + j]);
 #pragma unroll
             for (int m = 0; m < kMmas; ++m) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[n][m][i] *= keep[i & 1];
             }
-            // The weights of 16 bits for the product; their sum above is of the unrounded ones.
-            weights[n][0] = transpose_8x8(pack_bf16x2(w[0], w[1]));
-            weights[n][1] = transpose_8x8(pack_bf16x2(w[2], w[3]));
+#pragma unroll
+            for (int u = 0; u < kBlocks; ++u) {
+                float w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    w[i] = exp2_approx(score[u][n][i] - shift[i & 1]);
+                    sum[n][i & 1] += w[i];
+                }
+                // The weights of 16 bits for the product; their sum above is of the unrounded ones.
+                weights[u][n][0] = transpose_8x8(pack_bf16x2(w[0], w[1]));
+                weights[u][n][1] = transpose_8x8(pack_bf16x2(w[2], w[3]));
+            }
         }
         // Product tile m: head elements 8g + m and 64 + 8g + m (kDim 128), 8g + 2m and 8g + 2m + 1 (64).
 #pragma unroll
-        for (int m = 0; m < kMmas; ++m) {
-            uint32_t a[4];
+        for (int u = 0; u < kBlocks; ++u) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int h = kPasses == 2 ? r : 0, e = kPasses == 2 ? m : 2 * m + r;
-                const uint32_t pick = e & 1 ? 0x7632u : 0x5410u;
-                a[r] = __byte_perm(v[h][0].v[e >> 1], v[h][1].v[e >> 1], pick);
-                a[2 + r] = __byte_perm(v[h][2].v[e >> 1], v[h][3].v[e >> 1], pick);
+            for (int m = 0; m < kMmas; ++m) {
+                uint32_t a[4];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const int h = kPasses == 2 ? r : 0, e = kPasses == 2 ? m : 2 * m + r;
+                    const uint32_t pick = e & 1 ? 0x7632u : 0x5410u;
+                    a[r] = __byte_perm(v[u][h][0].v[e >> 1], v[u][h][1].v[e >> 1], pick);
+                    a[2 + r] = __byte_perm(v[u][h][2].v[e >> 1], v[u][h][3].v[e >> 1], pick);
+                }
+#pragma unroll
+                for (int n = 0; n < kTiles; ++n) mma_bf16(o[n][m], a, weights[u][n][0], weights[u][n][1]);
             }
-#pragma unroll
-            for (int n = 0; n < kTiles; ++n) mma_bf16(o[n][m], a, weights[n][0], weights[n][1]);
         }
         if (next < block_end) load_values(next, next_page);
-        page = next_page;
+#pragma unroll
+        for (int u = 0; u < kBlocks; ++u) page[u] = next_page[u];
     }
 
     // Join the warps: sums over their maxima, then one rescaled sum.
@@ -303,17 +334,20 @@ __device__ __forceinline__ float4 join_warps(const ShortShared<kDim, kTiles>& sh
 __device__ __forceinline__ void write_short(const AttentionParams& p, const ShortSequence& s, int kv_head, int row, int d, float l,
                                             float4 total) {
     const float inverse = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    const int token = row / p.group, head = kv_head * p.group + row - token * p.group;
+    const int token = static_cast<int>(fast_div(static_cast<uint32_t>(row), p.group_div)), head = kv_head * p.group + row - token * p.group;
     st_v2(p.out + static_cast<int64_t>(s.begin + token) * p.out_token + head * p.out_head + d,
           pack_bf16x2(total.x * inverse, total.y * inverse), pack_bf16x2(total.z * inverse, total.w * inverse));
 }
 
 constexpr int kShortThreads = kShortWarps * kWarpSize;
-// CTAs an SM: 168 registers a thread for 8 rows, 255 for 16.
-constexpr int short_ctas(int tiles) { return tiles == 1 ? 3 : 2; }
+// Where a warp has few turns, latency counts: it takes two blocks a turn for 8 rows, of which two CTAs fit an SM (255
+// registers). Where the GPU is full three CTAs of one block a turn (168 registers) have as much in flight.
+constexpr int short_blocks(int tiles) { return tiles == 1 ? 2 : 1; }
+constexpr int kShortCtas = 2;
+constexpr int shared_ctas(int tiles) { return tiles == 1 ? 3 : 2; }
 
 template <int kDim, int kTiles>
-__global__ void __launch_bounds__(kShortThreads, short_ctas(kTiles)) attention_short_kernel(const AttentionParams p) {
+__global__ void __launch_bounds__(kShortThreads, kShortCtas) attention_short_kernel(const AttentionParams p) {
     constexpr int kRows = 8 * kTiles;
     __shared__ ShortShared<kDim, kTiles> shared;
     grid_dependency_wait();
@@ -326,7 +360,7 @@ __global__ void __launch_bounds__(kShortThreads, short_ctas(kTiles)) attention_s
     const int block_begin = static_cast<int>(static_cast<int64_t>(s.blocks) * rank / ctas);
     const int block_end = static_cast<int>(static_cast<int64_t>(s.blocks) * (rank + 1) / ctas);
     for (int row0 = (unit - pair * p.row_tiles) * kRows; row0 < s.rows; row0 += p.row_tiles * kRows) {
-        short_rows(p, s, seq, kv_head, row0, block_begin, block_end, shared);
+        short_rows<kDim, kTiles, short_blocks(kTiles)>(p, s, seq, kv_head, row0, block_begin, block_end, shared);
         for (int e = threadIdx.x; e < kRows * (kDim / 4); e += kShortThreads) {
             const int local = e / (kDim / 4), d = e % (kDim / 4) * 4;
             float m, l;
@@ -384,7 +418,7 @@ constexpr int kShortPairCost = 8;   // of a sequence and key head beside its blo
 constexpr int kShortLeast = 24;     // of a stretch, in blocks: shorter ones cost more parts than they save time
 
 template <int kDim, int kTiles>
-__global__ void __launch_bounds__(kShortThreads, short_ctas(kTiles)) attention_shared_kernel(const AttentionParams p,
+__global__ void __launch_bounds__(kShortThreads, shared_ctas(kTiles)) attention_shared_kernel(const AttentionParams p,
                                                                                           const AttentionParts parts) {
     constexpr int kRows = 8 * kTiles;
     __shared__ ShortShared<kDim, kTiles> shared;
@@ -462,7 +496,7 @@ __global__ void __launch_bounds__(kShortThreads, short_ctas(kTiles)) attention_s
         left -= take;
         skip = 0;
         for (int row0 = 0; work && row0 < s.rows; row0 += kRows) {
-            short_rows(p, s, seq, kv_head, row0, block_begin, block_end, shared);
+            short_rows<kDim, kTiles, 1>(p, s, seq, kv_head, row0, block_begin, block_end, shared);
             for (int e = threadIdx.x; e < kRows * (kDim / 4); e += kShortThreads) {
                 const int local = e / (kDim / 4), d = e % (kDim / 4) * 4;
                 float m, l;
