@@ -124,6 +124,14 @@ def silu_and_mul_packed(x: torch.Tensor) -> torch.Tensor:
 # ---- paged KV cache (not in the reference library) -----------------------------------------------
 
 
+@cache
+def _op(name: str):
+    """The op's overload, looked up once: in a decode step the calls' host time counts."""
+    load_extension()
+
+    return getattr(torch.ops.inference_performance_lab, name).default
+
+
 def rotary_embedding(
     positions: torch.Tensor,
     query: torch.Tensor,
@@ -138,9 +146,7 @@ def rotary_embedding(
     ``(x[i], x[i + R/2])`` with ``is_neox``, else ``(x[2i], x[2i+1])``. Any strides with a contiguous
     last dimension.
     """
-    load_extension()
-
-    torch.ops.inference_performance_lab.rotary_embedding(positions, query, key, cos_sin_cache, is_neox)
+    _op("rotary_embedding")(positions, query, key, cos_sin_cache, is_neox)
 
 
 def rotary_embedding_cache(
@@ -157,9 +163,7 @@ def rotary_embedding_cache(
     """Rotates ``query`` in place and writes rotated ``key`` and ``value`` to their slots of the caches
     ``[pages, page_size, kv_heads, D]``: slot ``s`` (int64, negative: none) is row ``s % page_size`` of
     page ``s // page_size``. ``key`` itself stays as it is."""
-    load_extension()
-
-    torch.ops.inference_performance_lab.rotary_embedding_cache(
+    _op("rotary_embedding_cache")(
         positions, query, key, value, cos_sin_cache, key_cache, value_cache, slot_mapping, is_neox
     )
 
@@ -183,10 +187,8 @@ def paged_attention(
     ``max_query_len`` and ``max_seq_len`` bound the lengths; ``window`` > 0 limits each token to the last
     ``window`` keys. A token that sees no key gives 0; rows of no sequence are left unwritten.
     """
-    load_extension()
-
     output = torch.empty_like(query, memory_format=torch.contiguous_format)
-    torch.ops.inference_performance_lab.paged_attention(
+    _op("paged_attention")(
         output, query, key_cache, value_cache, block_tables, query_start_loc, seq_lens, max_query_len, max_seq_len,
         scale, window
     )
@@ -196,9 +198,7 @@ def paged_attention(
 
 def copy_pages(caches: list[torch.Tensor], pairs: torch.Tensor) -> None:
     """Copies page ``pairs[i, 0]`` to page ``pairs[i, 1]`` (int32; negative: skipped) in every cache."""
-    load_extension()
-
-    torch.ops.inference_performance_lab.copy_pages(caches, pairs)
+    _op("copy_pages")(caches, pairs)
 
 
 def reserve_pages(
@@ -212,9 +212,7 @@ def reserve_pages(
     """Gives ``rows[i]`` pages for ``new_lens[i]`` tokens, in place. Returns an int32 ``[1]`` status on
     the device: 0, the number of free pages lacking, or -1 for an entry out of range; unless it is 0
     nothing has changed."""
-    load_extension()
-
-    return torch.ops.inference_performance_lab.reserve_pages(
+    return _op("reserve_pages")(
         block_tables, seq_lens, ref_counts, rows, new_lens, page_size
     )
 
@@ -230,9 +228,7 @@ def fork_sequences(
     """Makes the empty row ``children[i]`` a copy of row ``parents[i]``, in place: whole pages are
     shared, a partly filled last page is copied in every cache. Returns a status as
     :func:`reserve_pages` does."""
-    load_extension()
-
-    return torch.ops.inference_performance_lab.fork_sequences(
+    return _op("fork_sequences")(
         caches, block_tables, seq_lens, ref_counts, parents, children
     )
 
@@ -241,9 +237,7 @@ def release_sequences(
     block_tables: torch.Tensor, seq_lens: torch.Tensor, ref_counts: torch.Tensor, rows: torch.Tensor
 ) -> None:
     """Empties ``rows``, in place: each of their pages loses one reference."""
-    load_extension()
-
-    torch.ops.inference_performance_lab.release_sequences(block_tables, seq_lens, ref_counts, rows)
+    _op("release_sequences")(block_tables, seq_lens, ref_counts, rows)
 
 
 def compact_pages(
@@ -251,11 +245,9 @@ def compact_pages(
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Moves the pages in use to the lowest numbers. Returns the renumbered tables and counts and the
     number of pages in use (int32 ``[1]``); the old tables stay valid until moved pages are claimed."""
-    load_extension()
-
     new_tables = torch.empty_like(block_tables, memory_format=torch.contiguous_format)
     new_counts = torch.empty_like(ref_counts)
     live = ref_counts.new_empty(1)
-    torch.ops.inference_performance_lab.compact_pages(caches, block_tables, ref_counts, new_tables, new_counts, live)
+    _op("compact_pages")(caches, block_tables, ref_counts, new_tables, new_counts, live)
 
     return new_tables, new_counts, live

@@ -356,3 +356,31 @@ def test_no_tokens_needs_no_device():
     capi.paged_attention(attention_args(num_tokens=0))
     assert capi.paged_attention_plan(attention_args(num_tokens=0)) == "none"
     assert capi.paged_attention_workspace(attention_args(num_tokens=0)) == 0
+
+
+def test_plans():
+    """The kernels a call would run, on a B200's 148 SMs."""
+    plan = lambda **changes: capi.paged_attention_plan(attention_args(**changes))  # noqa: E731
+    # Few sequences: a cluster each; many, or long ones: equal shares.
+    assert plan() == "attention_short_kernel<1>"
+    assert plan(num_tokens=64, num_seqs=64, max_seq_len=8192) == "attention_shared_kernel<1> + attention_join_parts_kernel"
+    assert plan(max_seq_len=65536, table_width=4096) == "attention_shared_kernel<1> + attention_join_parts_kernel"
+    assert plan(num_heads=64, query_token_stride=8192, output_token_stride=8192) == "attention_short_kernel<2>"
+    # Chunks: the tile kernel, beside a short one where single tokens may be among them.
+    chunk = dict(num_tokens=2048, num_seqs=1, max_query_len=2048, max_seq_len=16384, table_width=1024)
+    assert plan(**chunk) == "attention_tile_kernel + attention_join_rows_kernel"
+    mixed = {**chunk, "num_tokens": 2050, "num_seqs": 3, "max_seq_len": 32768}
+    assert plan(**mixed) == ("attention_tile_kernel + attention_join_rows_kernel + attention_shared_kernel<1> + "
+                             "attention_join_parts_kernel")
+    # A few tokens stay with the short kernel, many sequences of a few with the tile kernel.
+    assert plan(num_tokens=4, num_seqs=1, max_query_len=4) == "attention_short_kernel<2>"
+    assert plan(num_tokens=256, num_seqs=64, max_query_len=4, max_seq_len=2000) == "attention_tile_kernel + attention_join_rows_kernel"
+    # Anything that does not lie in 16-byte chunks and blocks of 16 keys: a warp a row.
+    for odd in (dict(head_size=20), dict(page_size=24), dict(key_cache=0x7F0000000008), dict(query_head_stride=132),
+                dict(head_size=256), dict(value_cache_token_stride=516)):
+        assert plan(**odd) == "attention_row_kernel"
+    # Broadcast keys (a stride of 0) cannot be mapped: rows of any number through the short kernel.
+    assert plan(**chunk, key_cache_head_stride=0) == "attention_short_kernel<2>"
+    assert capi.paged_attention_workspace(attention_args()) == 0
+    parts = 2 * 148 * (256 * (128 * 4 + 8) + 16)
+    assert capi.paged_attention_workspace(attention_args(**chunk)) == parts
