@@ -182,7 +182,7 @@ IPL_API ipl_status ipl_rotary_embedding_cache_bf16(const ipl_rotary_args* args, 
  * 0..num_pages-1 contributes nothing and sets bit 3 of the fault word. Rows of query that belong to no
  * sequence are not written.
  *
- * Strides are in elements; the last dimension is contiguous. max_query_len and max_seq_len are upper
+ * Strides are in elements; the last dimension is contiguous; output overlaps none of the inputs. max_query_len and max_seq_len are upper
  * bounds of the lengths, known on the host: they choose the kernels and the split of long rows.
  * Sequences longer than the bounds are computed all the same, more slowly. The workspace
  * (ipl_paged_attention_workspace bytes, 16-byte aligned) holds the parts of split rows.

@@ -649,6 +649,7 @@ ipl_status ipl_copy_pages(const ipl_page_caches* caches, int64_t num_pages, cons
     for (int64_t from = 0; from < caches->num_caches; from += kMaxCachesPerLaunch) {
         CopyPagesParams p = {};
         p.num_caches = cache_list(*caches, from, &p.caches);
+        p.count = static_cast<int>(count);
         p.pairs = pairs;
         p.num_pages = static_cast<int>(num_pages);
         p.page = layout;
@@ -683,6 +684,7 @@ ipl_status ipl_fork_sequences(const ipl_page_caches* caches, const ipl_page_pool
     do {
         ForkParams p = {};
         p.num_caches = cache_list(*caches, from, &p.caches);
+        p.count = static_cast<int>(count);
         p.with_tables = from == 0;
         p.state = claim.state;
         p.parents = parents;

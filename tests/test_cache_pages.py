@@ -231,6 +231,39 @@ def test_graph_replay():
 
 
 @gpu
+def test_c_abi():
+    """The same calls through the C ABI, on raw pointers."""
+    require_cuda()
+    d = Device(4, 8, 20, 4)
+    stream = torch.cuda.current_stream().cuda_stream
+    state = capi.PagePool(d.tables.data_ptr(), d.lens.data_ptr(), d.refs.data_ptr(), 4, 8, 8, 20, 4)
+    bytes_per_page = d.caches[0][0].numel() * 2
+    store = capi.page_caches([c.data_ptr() for c in d.caches], bytes_per_page, bytes_per_page)
+    status, live = d.ints([7]), d.ints([0])
+    rows, lens, parents, children = d.ints([0, 2]), d.ints([9, 30]), d.ints([2]), d.ints([1])
+    capi.reserve_pages(state, rows.data_ptr(), lens.data_ptr(), 2, status.data_ptr(), stream)
+    assert status.tolist() == [d.pool.reserve([0, 2], [9, 30])]
+    before = d.view.clone()
+    capi.fork_sequences(store, state, parents.data_ptr(), children.data_ptr(), 1, status.data_ptr(), stream)
+    lacking, copies = d.pool.fork([2], [1])
+    assert status.tolist() == [lacking] and len(copies) == 1
+    assert torch.equal(d.view[:, copies[0][1]], before[:, copies[0][0]])
+    d.same()
+    capi.release_sequences(state, rows.data_ptr(), 1, stream)
+    d.pool.release([0])
+    d.same()
+    tables, refs = torch.empty_like(d.tables), torch.empty_like(d.refs)
+    size = capi.compact_pages_workspace(20)
+    workspace = torch.empty(size, dtype=torch.uint8, device="cuda")
+    capi.compact_pages(store, state, tables.data_ptr(), refs.data_ptr(), live.data_ptr(), workspace.data_ptr(), size, stream)
+    want_tables, want_refs, want_live, _ = d.pool.compact()
+    assert tables.tolist() == want_tables and refs.tolist() == want_refs and live.tolist() == [want_live]
+    pairs = d.ints([[0, 15]])
+    capi.copy_pages(store, 20, pairs.data_ptr(), 1, stream)
+    assert torch.equal(d.view[:, 15], d.view[:, 0])
+
+
+@gpu
 def test_refusals():
     require_cuda()
     d = Device(4, 8, 20, 4)

@@ -5,6 +5,8 @@ strides, long offsets, streams and graphs; and its refusals."""
 
 from __future__ import annotations
 
+import random
+
 import pytest
 import torch
 
@@ -222,6 +224,47 @@ def test_lengths_past_the_bounds_given():
     for most_new, most in ((1, 1), (1, 700), (60, 32), (2, 2), (4096, 100000)):
         got = extension.paged_attention(*inputs, most_new, most, 0.125)
         assert ((got.double() - expected).abs() <= attention_bound(expected, size)).all(), (most_new, most)
+
+
+@gpu
+def test_more_sequences_than_threads():
+    """Hundreds of ragged sequences: single tokens, chunks and both, with lengths of zero among them."""
+    require_cuda()
+    rng = random.Random(7)
+    for most_new, longest, count in ((1, 300, 700), (40, 250, 450), (9, 2000, 130)):
+        new = [rng.choice([0, 1, 1, rng.randint(1, most_new)]) for _ in range(count)]
+        total = [rng.randint(0, longest) for _ in range(count)]
+        inputs = make(new, total, heads=4, kv_heads=2, dim=64, seed=count)
+        check(inputs, new, total)
+
+
+@gpu
+def test_long_sequences_among_many_single_tokens_past_the_bounds():
+    """A call that plans equal shares of single tokens meets chunks that max_query_len denies."""
+    require_cuda()
+    new = [60 if s % 50 == 3 else 1 for s in range(240)]
+    total = [max(n, 200 + s) for s, n in enumerate(new)]
+    inputs = make(new, total, heads=14, kv_heads=2, dim=64)
+    expected, size = attention(*inputs, 0.125)
+    got = extension.paged_attention(*inputs, 1, max(total), 0.125)
+    assert ((got.double() - expected).abs() <= attention_bound(expected, size)).all()
+
+
+@gpu
+def test_groups_wider_than_a_tile():
+    require_cuda()
+    for new, total in (([1, 3], [300, 40]), ([50], [90])):
+        check(make(new, total, heads=200, kv_heads=1, dim=64), new, total)
+
+
+@gpu
+def test_broadcast_keys():
+    """One key head shown as four by a stride of 0: not mappable, computed all the same."""
+    require_cuda()
+    for new, total in (([1, 1], [300, 40]), ([150], [190])):
+        q, kc, vc, tables, starts, lens = make(new, total, heads=8, kv_heads=1, dim=64)
+        wide = [c.expand(-1, -1, 4, -1) for c in (kc, vc)]
+        check((q, *wide, tables, starts, lens), new, total)
 
 
 @gpu
