@@ -13,7 +13,7 @@ namespace ipl {
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / kWarpSize;
 constexpr int kPageCopyThreads = 128;  // a CTA a page
-constexpr int kPageMoveThreads = 256;  // CTAs that take pages in turn (377 MB moved: 130 us, with 128 threads 139)
+constexpr int kPageMoveThreads = 256;  // CTAs that take pages in turn (377 MB moved: 129 us, with 128 threads 134)
 constexpr int kReleaseThreads = 128;
 constexpr int kMaxCachesPerLaunch = 128;
 
@@ -191,7 +191,8 @@ __global__ void __launch_bounds__(kPlanThreads) page_claim_kernel(const ClaimPar
 
 // `bytes` from one page to another of one cache, by the whole CTA: HBM-bound. Two 32-byte accesses a thread in flight
 // where pages allow them (`wide`), else four of 16 bytes. 96 pages of 64 KB in 56 caches, 704 MB read and written:
-// 114 us with CTAs of 128 threads a page, 6.2 TB/s; 126 with 16-byte accesses, 117 with four 32-byte ones.
+// 111 us with CTAs of 128 threads a page, 6.3 TB/s; 115 with 16-byte accesses. Four 32-byte ones: 109, but then the
+// compaction, which shares this, takes 137 us for 411 moves in place of 129.
 template <typename Vec, int kUnroll>
 __device__ __forceinline__ void copy_vectors(const char* src, char* dst, int64_t bytes) {
     const int64_t step = static_cast<int64_t>(blockDim.x) * sizeof(Vec);
@@ -264,8 +265,9 @@ __global__ void __launch_bounds__(kPageCopyThreads) page_fork_kernel(const __gri
     grid_launch_dependents();
     if (*p.status != 0) return;
     const PageState& s = p.state;
-    // Cache after cache, so that a parent's page is read from HBM once for all of its children: 96 children of 16
-    // parents in 56 caches, 352 MB written and 59 MB read, take 76 us; child after child 110.
+    // Cache after cache, so that a parent's page is read from HBM once for all of its children. Release, fork and
+    // reserve of 96 children of 16 parents in 56 caches: 87 us, child after child 121. Where the 59 MB of parents'
+    // pages are in L2 already, the two orders are level (release and fork 77 and 78 us).
     const uint32_t cache = blockIdx.x / p.count, child = blockIdx.x - cache * p.count;
     const int row = p.children[child], len = s.lens[row];  // the parent's
     const int whole = len / s.page_size, used = len % s.page_size;

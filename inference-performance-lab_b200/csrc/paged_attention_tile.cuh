@@ -33,7 +33,7 @@ constexpr int kTileThreads = 384;  // three warpgroups, among which the register
 // softmax warpgroups take 208 and the third keeps 88 (64512 again).
 constexpr int kSoftmaxRegisters = 208, kOtherRegisters = 88;
 constexpr int kTileHeadKeys = 96;   // weights of a step handed over first, so that their product begins early
-constexpr int kTilePolynomial = 2;  // of 16 pairs of weights, by the polynomial (0: 1 % slower, 4: 2 %, 6: 4 %)
+constexpr int kTilePolynomial = 2;  // of 16 pairs of weights, by the polynomial (0: 1 % slower, 4: 2 to 5 %, 6: 4 to 6 %)
 constexpr int kTileBoxes = kTileKeys / kAttentionBlock;  // boxes of at least 16 keys a tile
 constexpr uint32_t kAllBlocks = (1u << kTileBoxes) - 1u;
 

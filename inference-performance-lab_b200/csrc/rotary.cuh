@@ -54,8 +54,8 @@ __device__ __forceinline__ void turn_pairs(float* a, float* b, const float* c, c
 // interleaved); otherwise one pair (or one element to copy) an item. Bound by HBM in large launches, by the chain of
 // loads (position, then its row of the table) in small ones: the elements are loaded ahead of the position. Small
 // launches give a token's items a thread each in one CTA; large ones use CTAs of 128 threads, which retire more
-// evenly (8192 tokens of 28 + 4 heads of 128, written to pages: 29.5 us, 0.80 of the copy peak, with 256 threads 33.6;
-// 64 tokens: 2.3 us, with 128 threads 3.3). Four heads a thread, sharing cosines and sines, measured the same.
+// evenly (8192 tokens of 28 + 4 heads of 128, written to pages: 27.3 to 28.0 us, 0.84 to 0.86 of the copy peak, with 256 threads
+// 31.7; 64 tokens: 1.9 us, with 128 threads 2.65). Four heads a thread, sharing cosines and sines, measured the same.
 template <bool kVector, bool kHalf, bool kAppend>
 __global__ void __launch_bounds__(kRotaryMaxThreads) rotary_kernel(const RotaryParams p) {
     constexpr int kChunk = kVector ? 8 : 1;
