@@ -189,10 +189,13 @@ __global__ void __launch_bounds__(kPlanThreads) page_claim_kernel(const ClaimPar
 
 // ---- copying pages -----------------------------------------------------------------------------
 
-// `bytes` from one page to another of one cache, by the whole CTA: HBM-bound. Two 32-byte accesses a thread in flight
-// where pages allow them (`wide`), else four of 16 bytes. 96 pages of 64 KB in 56 caches, 704 MB read and written:
-// 111 us with CTAs of 128 threads a page, 6.3 TB/s; 115 with 16-byte accesses. Four 32-byte ones: 109, but then the
-// compaction, which shares this, takes 137 us for 411 moves in place of 129.
+// `bytes` from one page to another of one cache, by the whole CTA: HBM-bound. 32-byte accesses where pages allow them
+// (`wide`), four a thread in flight in copies and forks, two in the compaction; else four of 16 bytes. 96 pages of
+// 64 KB in 56 caches, 704 MB read and written: 109 us with CTAs of 128 threads a page, 6.4 TB/s; 111 with two in
+// flight, 115 with 16-byte accesses. A compaction of 411 moves in its CTAs of 256 threads: 129 us with two, 137 with
+// four.
+constexpr int kCopyUnroll = 4, kMoveUnroll = 2;
+
 template <typename Vec, int kUnroll>
 __device__ __forceinline__ void copy_vectors(const char* src, char* dst, int64_t bytes) {
     const int64_t step = static_cast<int64_t>(blockDim.x) * sizeof(Vec);
@@ -218,10 +221,11 @@ struct PageLayout {
     int64_t stride, bytes;  // multiples of 16
     bool wide;              // and of 32, with bases alike
 };
+template <int kWideUnroll>
 __device__ __forceinline__ void copy_page(char* cache, const PageLayout& page, int from, int to) {
     const char* src = cache + from * page.stride;
     char* dst = cache + to * page.stride;
-    if (page.wide) copy_vectors<U32x8, 2>(src, dst, page.bytes);
+    if (page.wide) copy_vectors<U32x8, kWideUnroll>(src, dst, page.bytes);
     else copy_vectors<U32x4, 4>(src, dst, page.bytes);
 }
 
@@ -244,7 +248,7 @@ __global__ void __launch_bounds__(kPageCopyThreads) page_copy_kernel(const __gri
         if (threadIdx.x == 0) atomicOr(&g_fault_word, kFaultIndexOutOfRange);
         return;
     }
-    copy_page(p.caches.cache[cache], p.page, from, to);
+    copy_page<kCopyUnroll>(p.caches.cache[cache], p.page, from, to);
 }
 
 struct ForkParams {
@@ -266,7 +270,8 @@ __global__ void __launch_bounds__(kPageCopyThreads) page_fork_kernel(const __gri
     if (*p.status != 0) return;
     const PageState& s = p.state;
     // Cache after cache, so that a parent's page is read from HBM once for all of its children. Release, fork and
-    // reserve of 96 children of 16 parents in 56 caches: 87 us, child after child 121. Where the 59 MB of parents'
+    // reserve of 96 children of 16 parents in 56 caches: 87 us, child after child 121 (with two
+    // accesses in flight; with four, cache after cache is still 87). Where the 59 MB of parents'
     // pages are in L2 already, the two orders are level (release and fork 77 and 78 us).
     const uint32_t cache = blockIdx.x / p.count, child = blockIdx.x - cache * p.count;
     const int row = p.children[child], len = s.lens[row];  // the parent's
@@ -287,7 +292,7 @@ __global__ void __launch_bounds__(kPageCopyThreads) page_fork_kernel(const __gri
         if (threadIdx.x == 0) atomicOr(&g_fault_word, kFaultIndexOutOfRange);
         return;
     }
-    copy_page(p.caches.cache[cache], p.page, last, to[whole]);
+    copy_page<kCopyUnroll>(p.caches.cache[cache], p.page, last, to[whole]);
 }
 
 // ---- releasing ---------------------------------------------------------------------------------
@@ -399,7 +404,7 @@ __global__ void __launch_bounds__(kPageMoveThreads) page_compact_move_kernel(con
     const int64_t units = static_cast<int64_t>(*p.moves) * p.num_caches;
     for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
         const int64_t move = u / p.num_caches;
-        copy_page(p.caches.cache[u - move * p.num_caches], p.page, p.movers[move], p.holes[move]);
+        copy_page<kMoveUnroll>(p.caches.cache[u - move * p.num_caches], p.page, p.movers[move], p.holes[move]);
     }
 }
 
