@@ -277,8 +277,11 @@ size_t parts_bytes(int64_t ctas, int64_t slot_rows, int64_t dim) {
 }
 AttentionParts attention_parts(void* workspace, int64_t ctas, int slot_rows, int64_t dim, int tile_rows, int tile_tokens) {
     AttentionParts parts;
-    parts.sums = static_cast<float*>(workspace);
-    parts.stats = reinterpret_cast<float2*>(parts.sums + 2 * ctas * slot_rows * dim);
+    float* const base = static_cast<float*>(workspace);
+    // The tile kernel stores sums 32 bytes at once, a workspace lies on 16: the sums begin at the next 32 bytes. They
+    // end 16 bytes late then, in the last slot's, which nothing is written to: no CTA comes after the last one.
+    parts.sums = aligned(base, 32) ? base : base + 4;
+    parts.stats = reinterpret_cast<float2*>(base + 2 * ctas * slot_rows * dim);
     parts.parts = reinterpret_cast<AttentionPart*>(parts.stats + 2 * ctas * slot_rows);
     parts.slot_rows = slot_rows;
     parts.tile_rows = tile_rows;

@@ -427,3 +427,33 @@ def test_plans():
     assert capi.paged_attention_workspace(attention_args()) == 0
     parts = 2 * 148 * (256 * (128 * 4 + 8) + 16)
     assert capi.paged_attention_workspace(attention_args(**chunk)) == parts
+
+
+@gpu
+@pytest.mark.parametrize("new, total", [([1200], [2400]), ([1] * 64, [3000] * 64), ([1] * 8 + [500], [3000] * 9)])
+def test_workspace_at_any_16_bytes(new, total):
+    """Parts of cut rows in a workspace whose base is a multiple of 16 bytes and not of 32, as in one that is."""
+    require_cuda()
+    q, kc, vc, tables, starts, lens = make(new, total)
+    outs = [torch.empty_like(q) for _ in range(2)]
+    for out, offset in zip(outs, (0, 16)):
+        a = capi.PagedAttentionArgs(
+            output=out.data_ptr(), query=q.data_ptr(), key_cache=kc.data_ptr(), value_cache=vc.data_ptr(),
+            block_tables=tables.data_ptr(), query_start_loc=starts.data_ptr(), seq_lens=lens.data_ptr(), num_tokens=q.shape[0],
+            num_seqs=len(new), num_heads=28, num_kv_heads=4, head_size=128, num_pages=kc.shape[0], page_size=16,
+            table_width=tables.shape[1], table_stride=tables.stride(0), output_token_stride=out.stride(0),
+            output_head_stride=out.stride(1), query_token_stride=q.stride(0), query_head_stride=q.stride(1),
+            key_cache_page_stride=kc.stride(0), key_cache_token_stride=kc.stride(1), key_cache_head_stride=kc.stride(2),
+            value_cache_page_stride=vc.stride(0), value_cache_token_stride=vc.stride(1), value_cache_head_stride=vc.stride(2),
+            max_query_len=max(new), max_seq_len=max(total), window=0, scale=128**-0.5)
+        size = capi.paged_attention_workspace(a)
+        assert size > 0
+        workspace = torch.empty(size + 48, dtype=torch.uint8, device="cuda")
+        at = -workspace.data_ptr() % 32 + offset
+        workspace[at + size :] = 77
+        a.workspace, a.workspace_bytes = workspace.data_ptr() + at, size
+        capi.paged_attention(a, torch.cuda.current_stream().cuda_stream)
+        assert (workspace[at + size :] == 77).all()
+    assert torch.equal(*outs)
+    expected, size = attention(q, kc, vc, tables, starts, lens, 128**-0.5)
+    assert ((outs[0].double() - expected).abs() <= attention_bound(expected, size)).all()
