@@ -335,10 +335,11 @@ __global__ void __launch_bounds__(kAttentionRowWarps * kWarpSize) attention_row_
                 score = dot * p.scale_log2;
             }
         }
-        const float new_top = fmaxf(top, warp_max(score));
-        if (new_top == -INFINITY) continue;
-        const float weight = exp2f(score - new_top);
-        const float keep = exp2f(top - new_top);
+        if (!__any_sync(0xffffffffu, page >= 0)) continue;
+        // The maximum passes over NaN scores; their weights do not.
+        const float new_top = fmaxf(top, warp_max(score)), shift = new_top == -INFINITY ? 0.0f : new_top;
+        const float weight = exp2f(score - shift);
+        const float keep = exp2f(top - shift);
         sum = sum * keep + warp_sum(weight);
         top = new_top;
 #pragma unroll
@@ -356,7 +357,7 @@ __global__ void __launch_bounds__(kAttentionRowWarps * kWarpSize) attention_row_
             }
         }
     }
-    const float inverse = sum > 0.0f ? 1.0f / sum : 0.0f;
+    const float inverse = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
 #pragma unroll
     for (int i = 0; i < kSlots; ++i) {
         const int d = lane + i * kWarpSize;

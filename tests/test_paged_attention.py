@@ -457,3 +457,43 @@ def test_workspace_at_any_16_bytes(new, total):
     assert torch.equal(*outs)
     expected, size = attention(q, kc, vc, tables, starts, lens, 128**-0.5)
     assert ((outs[0].double() - expected).abs() <= attention_bound(expected, size)).all()
+
+
+def check_not_finite(inputs, new, total):
+    """As the formula in 64 bits, NaN and infinities included."""
+    got, scale = call(inputs, new, total)
+    expected, size = attention(*inputs, scale)
+    finite = expected.isfinite()
+    assert torch.equal(got.isnan(), expected.isnan())
+    assert ((got.double() - expected).abs() <= attention_bound(expected, size))[finite].all()
+
+
+EVERY_KERNEL = [
+    # heads, kv_heads, dim, page: the vector path, then a warp a row for its head size and its page size
+    (28, 4, 128, 16), (32, 8, 64, 32), (6, 3, 256, 16), (8, 2, 64, 24),
+]
+
+
+@gpu
+@pytest.mark.parametrize("heads, kv_heads, dim, page", EVERY_KERNEL)
+@pytest.mark.parametrize("new, total", [([1, 1], [70, 200]), ([1, 1], [1, 33]), ([1] * 40, [4000] * 40), ([150, 9], [190, 9])])
+def test_nan_and_infinite_inputs_reach_the_rows_that_see_them(heads, kv_heads, dim, page, new, total):
+    require_cuda()
+    group = heads // kv_heads
+    inputs = make(new, total, heads, kv_heads, dim, page)
+    q, kc, vc, tables, starts, lens = inputs
+    # One head of the last token.
+    q[-1, 1, dim // 2] = float("nan")
+    check_not_finite(inputs, new, total)
+    q[-1, 1, dim // 2] = 0.5
+    # Every visible key of a first block of 32, of one head of the first sequence.
+    for bad in (float("nan"), float("inf"), float("-inf")):
+        kept = [kc[int(tables[0, t // page]), t % page, 1].clone() for t in range(min(32, total[0]))]
+        for t in range(len(kept)):
+            kc[int(tables[0, t // page]), t % page, 1, 3] = bad
+        if bad == bad and total[0] <= 32:  # its one score may be -inf, of which the formula has no value
+            q[0, group : 2 * group, 3] = 1.0 if bad > 0 else -1.0
+        check_not_finite(inputs, new, total)
+        for t, row in enumerate(kept):
+            kc[int(tables[0, t // page]), t % page, 1] = row
+    assert capi.device_fault_flags(0) == 0
