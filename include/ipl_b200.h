@@ -174,16 +174,18 @@ IPL_API ipl_status ipl_rotary_embedding_cache_bf16(const ipl_rotary_args* args, 
  *   output = sum_t w_t v_t / sum_t w_t,   w_t = exp(scale q.k_t - max_t scale q.k_t)
  *
  * with fp32 scores, statistics and sums, rounded to bf16 once; the weights enter the product with the
- * values rounded to bf16 (their fp32 sum is the denominator). A token that sees no key gives 0. Query
- * head h reads key head h / (num_heads / num_kv_heads). Key t lies in page block_tables[s][t /
- * page_size], row t % page_size; table entries past a sequence's pages are never read, rows past its
- * length never matter, whatever they hold. Keys at masked positions never matter either; values that
- * one token of a sequence sees must be finite for its other tokens to be. A page number outside
- * 0..num_pages-1 contributes nothing and sets bit 3 of the fault word. Rows of query that belong to no
- * sequence are not written.
+ * values rounded to bf16 (their fp32 sum is the denominator). A token that sees no key gives 0, and so
+ * does one all of whose scores are -infinity; NaN and +infinity among its scores give NaN. Query head h
+ * reads key head h / (num_heads / num_kv_heads). Key t lies in page block_tables[s][t / page_size], row
+ * t % page_size; table entries past a sequence's pages are never read, rows past its length never
+ * matter, whatever they hold. Keys at masked positions never matter either; values that one token of a
+ * sequence sees must be finite for its other tokens to be. A page number outside 0..num_pages-1
+ * contributes nothing and sets bit 3 of the fault word. Rows of query that belong to no sequence are
+ * not written.
  *
- * Strides are in elements; the last dimension is contiguous; output overlaps none of the inputs. max_query_len and max_seq_len are upper
- * bounds of the lengths, known on the host: they choose the kernels and the split of long rows.
+ * Strides are in elements; the last dimension is contiguous; output overlaps none of the inputs.
+ * max_query_len and max_seq_len are upper bounds of the lengths, known on the host: they choose the
+ * kernels and the split of long rows.
  * Sequences longer than the bounds are computed all the same, more slowly. The workspace
  * (ipl_paged_attention_workspace bytes, 16-byte aligned) holds the parts of split rows.
  *

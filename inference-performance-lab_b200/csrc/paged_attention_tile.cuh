@@ -70,7 +70,8 @@ struct TileLayout {
 // step have scores for each of their cycles, so a part of the pairs is computed on the FMA pipes:
 // 2^x = 2^n 2^r, n = x rounded (by adding 1.5 2^23, which leaves n in the low bits), r in [-1/2, 1/2],
 // with the polynomial of degree 3 of least relative error for 2^r (7.5e-5 by the Remez exchange, a fiftieth
-// of the rounding of a weight to bf16). x is held above -126, so a vanishing weight is 2^-126, not 0.
+// of the rounding of a weight to bf16). x is held above -126, so a vanishing weight is 2^-126, not 0, and so is that of
+// NaN: a row whose maximum is not finite is seen to at its end.
 __device__ __forceinline__ F32x2 exp2_pair_units(F32x2 x) {
     float a, b;
     f32x2_split(x, a, b);
@@ -725,6 +726,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 tcgen05_fence_after();
             }
             if (!ok) break;
+            // The polynomial gives 2^-126 for -inf and NaN. A maximum of -inf: no weight. Of +inf or NaN: NaN.
+            sum = top == -INFINITY ? 0.0f : sum + (top - top);
             const float inverse = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
             const int r = row(), in_tile = row_token(r);
             const bool real = in_tile < p.tile_tokens && t * p.tile_tokens + in_tile < item.tokens;

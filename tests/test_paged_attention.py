@@ -497,3 +497,36 @@ def test_nan_and_infinite_inputs_reach_the_rows_that_see_them(heads, kv_heads, d
         for t, row in enumerate(kept):
             kc[int(tables[0, t // page]), t % page, 1] = row
     assert capi.device_fault_flags(0) == 0
+
+
+@gpu
+@pytest.mark.parametrize("dim", [64, 128])
+def test_an_infinite_score_anywhere_in_a_step_gives_nan(dim):
+    """Each key of a block of 32 that every row sees, in pairs of tiles that one CTA has whole (1200 of them)."""
+    require_cuda()
+    new, total = [60] * 150, [500] * 150
+    inputs = make(new, total, 16, 8, dim)
+    q, kc, _, tables = inputs[:4]
+    q.abs_()
+    for key in range(256, 288):
+        pages, row = tables[:, key // 16].long(), key % 16
+        kept = kc[pages, row]
+        kc[pages, row, 1::2, 0] = float("inf")
+        got, _ = call(inputs, new, total)
+        wide = got.view(-1, 8, 2, dim)
+        assert wide[:, 1::2].isnan().all(), key
+        assert wide[:, 0::2].isfinite().all()
+        kc[pages, row] = kept
+
+
+@gpu
+@pytest.mark.parametrize("heads, kv_heads, dim, page", EVERY_KERNEL)
+def test_scores_of_minus_infinity_alone_give_zero(heads, kv_heads, dim, page):
+    """As no score at all: such keys are as good as masked."""
+    require_cuda()
+    for new, total in (([1, 1], [70, 1]), ([1] * 40, [4000] * 40), ([150], [700]), ([60] * 150, [500] * 150)):
+        q, kc, vc, tables, starts, lens = make(new, total, heads, kv_heads, dim, page)
+        q.abs_()
+        kc[..., 0] = float("-inf")
+        got, _ = call((q, kc, vc, tables, starts, lens), new, total)
+        assert (got == 0).all(), (new, total)
