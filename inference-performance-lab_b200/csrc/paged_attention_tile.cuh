@@ -664,10 +664,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 const bool move = top < INFINITY && !(m <= top + 8.0f);
                 if (__any_sync(0xffffffffu, move)) {
                     const float keep = move ? exp2_approx(top - m) : 1.0f;
-                    if (move) {
-                        sum *= keep;
-                        top = m;
-                    }
+                    sum *= keep;
+                    top = move ? m : top;
+                    __syncwarp();
                     if (step > 0) {
 #pragma unroll
                         for (int c = 0; c < kDim / 16; ++c) {
@@ -698,6 +697,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                         }
                     }
                     fence_async_shared();
+                    __syncwarp();
                 }
                 const F32x2 scale = f32x2_make(a.scale_log2, a.scale_log2), minus_shift = f32x2_make(-shift, -shift);
                 F32x2 sums[2] = {0ull, 0ull};
@@ -713,6 +713,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                         tcgen05_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(p_ready + 16 * t + 8 * (c - (kTileHeadKeys / 32 - 1)));
+                        __syncwarp();
                     }
                 }
                 float parts[4];
@@ -739,6 +740,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
 #pragma unroll
             for (int c = 0; c < kDim / 32; ++c) {
                 float o[32] = {};
+                __syncwarp();  // the rows' stores part the warp, tensor memory is read by all of it
                 if (item.steps > 0) {
                     tmem_load_32(o_tmem + 32 * c, o);
                     tmem_wait_loads();

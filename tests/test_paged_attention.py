@@ -530,3 +530,16 @@ def test_scores_of_minus_infinity_alone_give_zero(heads, kv_heads, dim, page):
         kc[..., 0] = float("-inf")
         got, _ = call((q, kc, vc, tables, starts, lens), new, total)
         assert (got == 0).all(), (new, total)
+
+
+@gpu
+@pytest.mark.parametrize("heads, kv_heads, dim", [(28, 4, 128), (11, 1, 64), (40, 8, 80), (127, 1, 128)])
+def test_warps_whose_rows_differ(heads, kv_heads, dim):
+    """Warps of the tile kernel with padding, tokens past the chunk's end and maxima that move in some rows only, over
+    first steps that a window cuts: each of them parts a warp ahead of work that all of it does together."""
+    require_cuda()
+    for new, total, window in (([70], [1500], 600), ([301, 33] * 20, [301, 700] * 20, 190)):
+        inputs = make(new, total, heads, kv_heads, dim)
+        q = inputs[0]
+        q[::3] *= 6.0  # scores of these rows spread over many times 2^8
+        check(inputs, new, total, window)
