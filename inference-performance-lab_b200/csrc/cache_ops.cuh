@@ -324,11 +324,13 @@ AttentionPlan plan_attention(const ipl_paged_attention_args& a, int sm_count) {
     plan.vector = true;
     plan.dim = a.head_size <= 64 ? 64 : 128;
     const int64_t group = a.num_heads / a.num_kv_heads;
-    const int64_t rows = a.max_query_len * group;
+    // The bounds may be any numbers; beyond the tokens there are, and for a window beyond the keys, they bound nothing.
+    const int64_t most_new = a.max_query_len < a.num_tokens ? a.max_query_len : a.num_tokens;
+    const int64_t rows = most_new * group;
     plan.tiles = rows <= 8 ? 1 : 2;
     plan.short_rows = INT_MAX;
     int64_t keys = a.max_seq_len > 1 ? a.max_seq_len : 1;
-    if (a.window > 0 && a.window + a.max_query_len < keys) keys = a.window + a.max_query_len;
+    if (a.window > 0 && a.window < keys && a.window + most_new < keys) keys = a.window + most_new;
     // TMA takes strides of up to 2^40 bytes and no zero ones.
     const int64_t strides[] = {a.query_token_stride, a.query_head_stride, a.key_cache_page_stride, a.key_cache_token_stride,
                                a.key_cache_head_stride, a.value_cache_page_stride, a.value_cache_token_stride, a.value_cache_head_stride};
@@ -344,7 +346,7 @@ AttentionPlan plan_attention(const ipl_paged_attention_args& a, int sm_count) {
             plan.tiles = group <= 8 ? 1 : 2;
             plan.short_rows = plan.tiles * 8;
             // Sequences of one length have no short one among them.
-            if (group > 16 || a.num_tokens == a.max_query_len * a.num_seqs) {
+            if (group > 16 || a.num_tokens == most_new * a.num_seqs) {
                 plan.tiles = 0;
                 plan.short_rows = 0;
             }

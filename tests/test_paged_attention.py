@@ -543,3 +543,19 @@ def test_warps_whose_rows_differ(heads, kv_heads, dim):
         q = inputs[0]
         q[::3] *= 6.0  # scores of these rows spread over many times 2^8
         check(inputs, new, total, window)
+
+
+def test_plans_of_bounds_without_limit():
+    """Bounds past the tokens there are, and a window past the keys, plan as the ones that fit."""
+    plan = lambda **changes: capi.paged_attention_plan(attention_args(**changes))  # noqa: E731
+    chunk = dict(num_tokens=2048, num_seqs=1, max_query_len=2048, max_seq_len=16384, table_width=1024)
+    few = dict(num_tokens=4, num_seqs=1, max_query_len=4)
+    batch = dict(num_tokens=64, num_seqs=64, max_seq_len=8192)
+    for call in (chunk, few, batch, {}):
+        for most in (dict(window=2**63 - 1), dict(window=2**62), dict(window=2**31)):
+            assert plan(**call, **most) == plan(**call)
+            assert capi.paged_attention_workspace(attention_args(**call, **most)) == capi.paged_attention_workspace(attention_args(**call))
+    for call in (chunk, few):
+        for most in (2**63 - 1, 2**62, 2**33):
+            assert plan(**{**call, "max_query_len": most}) == plan(**call)
+            assert plan(**{**call, "max_query_len": most, "window": 2**63 - 1}) == plan(**call)
