@@ -318,6 +318,8 @@ int64_t tile_time(int64_t pairs, int64_t keys, int sm_count) {
     return 16000 + 1900 * (pairs * (keys / kTileKeys + 2) / sm_count);
 }
 
+constexpr int kMostRowTiles = 4096;
+
 AttentionPlan plan_attention(const ipl_paged_attention_args& a, int sm_count) {
     AttentionPlan plan;
     if (!attention_vectorises(a)) return plan;
@@ -351,9 +353,11 @@ AttentionPlan plan_attention(const ipl_paged_attention_args& a, int sm_count) {
                 plan.short_rows = 0;
             }
         } else {
-            plan.row_tiles = static_cast<int>(most < 4096 ? most : 4096);
+            plan.row_tiles = static_cast<int>(most < kMostRowTiles ? most : kMostRowTiles);
         }
     }
+    // The short kernels count a sequence's rows, and a turn of its row tiles past them, in 32 bits.
+    if (!plan.tile && a.num_tokens * group > INT_MAX - 16 * kMostRowTiles) return AttentionPlan{};
     if (plan.tile) {
         plan.tile_ctas = sm_count;
         plan.tile_workspace = parts_bytes(plan.tile_ctas, 2 * kTileRows, plan.dim);

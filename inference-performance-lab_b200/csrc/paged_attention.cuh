@@ -32,7 +32,7 @@ struct AttentionParams {
     int64_t key_page, key_token, key_head, value_page, value_token, value_head;
     float scale_log2;  // scale * log2(e): the exponentials are powers of two
     // Sequences of at most short_rows rows (new tokens x group) belong to the short kernels, the others
-    // to the tile kernel.
+    // to the tile kernel. The short kernels count rows in 32 bits, the tile kernel only those of a tile.
     int short_rows;
     FastDiv32 page_blocks;  // blocks of 16 keys a page (fast kernels)
     FastDiv32 group_div;

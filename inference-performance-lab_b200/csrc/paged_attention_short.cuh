@@ -55,8 +55,9 @@ struct ShortSequence {
 __device__ __forceinline__ bool short_sequence(const AttentionParams& p, int seq, ShortSequence& s) {
     s.begin = p.starts[seq];
     s.new_tokens = min(p.starts[seq + 1], p.num_tokens) - s.begin;
-    s.rows = s.new_tokens * p.group;
-    if (s.begin < 0 || s.new_tokens <= 0 || s.rows > p.short_rows) return false;
+    const int64_t rows = static_cast<int64_t>(s.new_tokens) * p.group;
+    if (s.begin < 0 || s.new_tokens <= 0 || rows > p.short_rows) return false;
+    s.rows = static_cast<int>(rows);
     s.true_len = p.lens[seq];
     s.len = table_bounded_length(p, seq);
     const KeyRange range = visible_keys(p, s.true_len, s.new_tokens);

@@ -164,7 +164,7 @@ __device__ __forceinline__ bool tile_pair(const TileParams& p, int u, TilePair& 
     }
     const int begin = a.starts[lo], new_tokens = min(a.starts[lo + 1], a.num_tokens) - begin;
     const int token0 = (u - (static_cast<int>(fast_div(static_cast<uint32_t>(max(begin, 0)), p.pair_tokens)) + lo)) * pair_tokens;
-    if (u >= p.units || begin < 0 || token0 < 0 || token0 >= new_tokens || new_tokens * a.group <= a.short_rows) return false;
+    if (u >= p.units || begin < 0 || token0 < 0 || token0 >= new_tokens || static_cast<int64_t>(new_tokens) * a.group <= a.short_rows) return false;
     pair.seq = lo;
     pair.token = begin + token0;
     pair.tokens = min(pair_tokens, new_tokens - token0);

@@ -559,3 +559,31 @@ def test_plans_of_bounds_without_limit():
         for most in (2**63 - 1, 2**62, 2**33):
             assert plan(**{**call, "max_query_len": most}) == plan(**call)
             assert plan(**{**call, "max_query_len": most, "window": 2**63 - 1}) == plan(**call)
+
+
+@gpu
+def test_more_rows_of_a_group_than_31_bits_count():
+    """2^24 + 1 tokens of 128 heads that share a key head: 2^31 + 128 rows, all but the last 100 tokens before
+    position 0. The query's rows overlap, so that it takes little memory."""
+    require_cuda()
+    tokens = 2**24 + 1
+    small, kc, vc, tables, starts, lens = make([100], [100], 128, 1, 8)
+    flat = torch.randn(8 * (tokens + 127), device="cuda").to(torch.bfloat16)
+    q = flat.as_strided((tokens, 128, 8), (8, 8, 1))
+    starts[1] = tokens
+    out = torch.full((tokens, 128, 8), 7.0, dtype=torch.bfloat16, device="cuda")
+    torch.ops.inference_performance_lab.paged_attention(out, q, kc, vc, tables, starts, lens, tokens, 100, 0.35, 0)
+    assert all(bool((part == 0).all()) for part in out[:-100].split(2**20))
+    expected, size = attention(q[-100:], kc, vc, tables, torch.tensor([0, 100]), lens, 0.35)
+    assert ((out[-100:].double() - expected).abs() <= attention_bound(expected, size)).all()
+    assert capi.device_fault_flags(0) == 0
+    del out
+    torch.cuda.empty_cache()
+
+
+def test_plan_of_more_rows_than_31_bits_count():
+    """Without the tile kernel (broadcast keys), the rows of a group are counted by the kernel of a warp a row."""
+    changes = dict(num_tokens=2**24 + 1, num_seqs=1, num_heads=128, num_kv_heads=1, head_size=8, max_query_len=2**24 + 1,
+                   max_seq_len=100, key_cache_token_stride=0)
+    assert capi.paged_attention_plan(attention_args(**changes)) == "attention_row_kernel"
+    assert capi.paged_attention_plan(attention_args(**{**changes, "num_tokens": 2**24 - 1024})) == "attention_short_kernel<2>"
