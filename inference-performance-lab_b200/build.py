@@ -28,9 +28,11 @@ NATIVE = PACKAGE_ROOT / "inference_performance_lab" / "_native"
 
 LIB_NAME = "libipl_b200.so"
 TORCH_OPS_NAME = "inference_performance_lab_cuda.so"
-# Test-only variant of LIB_NAME (never loaded by the package): see build_wait_test().
+# Test-only variants of LIB_NAME (never loaded by the package): see build_wait_test() and build_weight_test().
 WAIT_TEST_NAME = "test/libipl_b200_waittest.so"
 WAIT_TEST_DEFINES = ["-DIPL_WAIT_LIMIT_NS=1000000ull", "-DIPL_TEST_STAGED_SKIP_ROW=0", "-DIPL_TEST_TILE_SKIP_LOAD=2"]
+WEIGHT_TEST_NAME = "test/libipl_b200_weighttest.so"
+WEIGHT_TEST_DEFINES = ["-DIPL_TEST_TILE_PAIR_COST=16777216"]
 
 # Stable ABI target: torch 2.10 (the oldest version that has every call the shim uses).
 TORCH_TARGET_VERSION = "0x020a000000000000"
@@ -130,10 +132,20 @@ def build_wait_test(verbose: bool = False) -> Path:
     instead of 2 s, CTA 0 of the staged kernel never issues its row 0, and CTA 0 of the attention tile
     kernel never its second load of keys, so what waits for them runs out of time. Tests load it
     (ctypes) to check that the kernels then return, record the fault bit and leave the context usable."""
-    output = NATIVE / WAIT_TEST_NAME
+    return _build_test_variant(WAIT_TEST_NAME, WAIT_TEST_DEFINES, verbose)
+
+
+def build_weight_test(verbose: bool = False) -> Path:
+    """The same kernels and C ABI with pairs of tiles that weigh 2^24 steps more than they have, so that
+    the shares of a small call are cut from sums that a call of a million tokens reaches."""
+    return _build_test_variant(WEIGHT_TEST_NAME, WEIGHT_TEST_DEFINES, verbose)
+
+
+def _build_test_variant(name: str, defines: list[str], verbose: bool) -> Path:
+    output = NATIVE / name
     output.parent.mkdir(parents=True, exist_ok=True)
     sources = sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + [INCLUDE / "ipl_b200.h"]
-    flags = [*NVCC_FLAGS, *WAIT_TEST_DEFINES, f"-I{INCLUDE}", f"-I{CSRC}"]
+    flags = [*NVCC_FLAGS, *defines, f"-I{INCLUDE}", f"-I{CSRC}"]
     stamp = _stamp(sources, flags)
     if _up_to_date(output, stamp):
         return output
@@ -183,8 +195,8 @@ def build_torch_ops(verbose: bool = False) -> Path:
 
 
 def build(verbose: bool = False, tests: bool = False) -> None:
-    """Build both libraries (and, with ``tests``, the test-only wait-limit variant); concurrent
-    callers (e.g. several ranks) serialise on a lock file."""
+    """Build both libraries (and, with ``tests``, the test-only variants); concurrent callers (e.g. several
+    ranks) serialise on a lock file."""
     import fcntl
 
     NATIVE.mkdir(parents=True, exist_ok=True)
@@ -195,6 +207,7 @@ def build(verbose: bool = False, tests: bool = False) -> None:
             build_torch_ops(verbose)
             if tests:
                 build_wait_test(verbose)
+                build_weight_test(verbose)
         finally:
             fcntl.flock(lock, fcntl.LOCK_UN)
 

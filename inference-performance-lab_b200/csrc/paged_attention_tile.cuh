@@ -37,7 +37,10 @@ constexpr int kTilePolynomial = 2;  // of 16 pairs of weights, by the polynomial
 constexpr int kTileBoxes = kTileKeys / kAttentionBlock;  // boxes of at least 16 keys a tile
 constexpr uint32_t kAllBlocks = (1u << kTileBoxes) - 1u;
 
-constexpr int kTilePairCost = 2;  // of a pair beside its steps (first scores, output), in steps
+#ifndef IPL_TEST_TILE_PAIR_COST
+#define IPL_TEST_TILE_PAIR_COST 2  // test builds: a cost at which few pairs weigh more than 2^31
+#endif
+constexpr int kTilePairCost = IPL_TEST_TILE_PAIR_COST;  // of a pair beside its steps (first scores, output), in steps
 constexpr int kTileItems = 4;     // ring of work items
 
 struct TileParams {
@@ -231,9 +234,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     grid_launch_dependents();
 
     // This CTA's share of the steps: of the pairs of one key head in their order, then of the next head. The
-    // items' memory serves the sums. Pair u weighs its steps and kTilePairCost.
-    int* const scratch = reinterpret_cast<int*>(at(smem + L::kItemBase));
-    int* const found = scratch + kTileThreads / kWarpSize;  // the pair the share begins in, and its weight before it
+    // items' memory serves the sums. Pair u weighs its steps and kTilePairCost, all pairs more than 31 bits hold.
+    int64_t* const scratch = reinterpret_cast<int64_t*>(at(smem + L::kItemBase));
+    int* const found = reinterpret_cast<int*>(scratch + kTileThreads / kWarpSize);  // the pair the share begins in, and its weight before it
     if (threadIdx.x < a.num_seqs) {
         // The searches below go through these one load after the other: bring them near at once.
         asm volatile("prefetch.global.L1 [%0];" ::"l"(a.starts + threadIdx.x));
@@ -241,11 +244,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     }
     const auto weight = [&](int u, TilePair& pair) { return u < p.units && tile_pair(p, u, pair) ? pair.steps + kTilePairCost : 0; };
     // Sum over the CTA up to and with this thread; `total` gets all of it.
-    const auto sum_through = [&](int value, int& total) {
-        int through = value;
+    const auto sum_through = [&](int64_t value, int64_t& total) {
+        int64_t through = value;
 #pragma unroll
         for (int offset = 1; offset < kWarpSize; offset *= 2) {
-            const int below = __shfl_up_sync(0xffffffffu, through, offset);
+            const int64_t below = __shfl_up_sync(0xffffffffu, through, offset);
             if (lane >= offset) through += below;
         }
         __syncthreads();
@@ -260,30 +263,32 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     };
     // In the common case every thread has one pair, whose weight serves both sums.
     TilePair pair = {};
-    int own = weight(threadIdx.x, pair), more = 0;
+    int own = weight(threadIdx.x, pair);
+    int64_t more = 0;
     for (int u = threadIdx.x + kTileThreads; u < p.units; u += kTileThreads) {
         TilePair other;
         more += weight(u, other);
     }
-    int through, head_weight;
+    int64_t through, head_weight;
     if (p.units <= kTileThreads) {
         through = sum_through(own, head_weight);
     } else {
         sum_through(own + more, head_weight);
     }
-    const int64_t all_weight = static_cast<int64_t>(head_weight) * a.kv_heads;
+    const int64_t all_weight = head_weight * a.kv_heads;
     const int64_t share_begin = divide(all_weight * blockIdx.x, gridDim.x), share_end = divide(all_weight * (blockIdx.x + 1), gridDim.x);
     const int begin_head = head_weight > 0 ? static_cast<int>(divide(share_begin, head_weight)) : 0;
-    int begin_weight = static_cast<int>(share_begin - static_cast<int64_t>(begin_head) * head_weight);
-    for (int base = 0, before = 0; share_begin < share_end && base < p.units; base += kTileThreads) {
-        int total = 0;
+    const int64_t begin_weight = share_begin - begin_head * head_weight;
+    int64_t before = 0;
+    for (int base = 0; share_begin < share_end && base < p.units; base += kTileThreads) {
+        int64_t total = 0;
         if (p.units > kTileThreads) {
             own = weight(base + threadIdx.x, pair);
             through = before + sum_through(own, total);
         }
         if (begin_weight < through && begin_weight >= through - own) {
             found[0] = base + threadIdx.x;
-            found[1] = begin_weight - (through - own);
+            found[1] = static_cast<int>(begin_weight - (through - own));
         }
         before += total;
         if (begin_weight < before) break;
@@ -291,8 +296,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     // The pairs from there on, for the warp that hands out the work: in the last stage, which is loaded into later.
     TilePair* const first_pairs = reinterpret_cast<TilePair*>(at(smem + L::kStageBase + (L::kStages - 1) * L::kTileBytes));
     __syncthreads();
-    const int begin_unit = found[0];
-    begin_weight = found[1];
+    const int begin_unit = found[0], begin_skip = found[1];
     if (p.units <= kTileThreads && share_begin < share_end) {
         const int place = static_cast<int>(threadIdx.x) - begin_unit;
         if (place >= 0 && place < kWarpSize) {
@@ -329,7 +333,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             return ok;
         };
         int64_t left = share_end - share_begin;
-        int skip = begin_weight, head = begin_head;
+        int skip = begin_skip, head = begin_head;
         TileItem item = {};
         bool ok = true;
         for (int base = begin_unit; left > 0 && ok; base += kWarpSize) {
