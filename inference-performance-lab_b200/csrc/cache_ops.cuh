@@ -365,11 +365,14 @@ AttentionPlan plan_attention(const ipl_paged_attention_args& a, int sm_count) {
     }
     if (plan.tiles > 0) {
         // A cluster for each sequence, key head and row tile where the GPU holds all of them and no warp has more
-        // than 16 blocks of keys; otherwise equal shares (row tiles: clusters all the same, they are not cut).
+        // than 16 blocks of keys; otherwise equal shares (row tiles: clusters all the same, they are not cut). Those
+        // are cut from a sum of blocks in 32 bits, which the tables' width bounds.
+        const int64_t longest = a.table_width < INT_MAX / a.page_size ? a.table_width * a.page_size : INT_MAX;
+        const bool countable = a.num_seqs <= INT_MAX / (longest / kAttentionBlock + 1 + kShortPairCost);
         const int64_t units = a.num_seqs * a.num_kv_heads * plan.row_tiles;
         const int64_t resident = static_cast<int64_t>(sm_count) * shared_ctas(plan.tiles);
         plan.cluster = short_cluster(units, keys, plan.tiles, sm_count);
-        if (plan.row_tiles == 1 && (units * plan.cluster > resident || key_turns(keys) > 16 * plan.cluster)) {
+        if (plan.row_tiles == 1 && countable && (units * plan.cluster > resident || key_turns(keys) > 16 * plan.cluster)) {
             plan.cluster = 0;
             plan.shared_ctas = static_cast<int>(resident);
             plan.workspace += parts_bytes(plan.shared_ctas, 8 * plan.tiles, plan.dim);

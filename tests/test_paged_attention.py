@@ -587,3 +587,13 @@ def test_plan_of_more_rows_than_31_bits_count():
                    max_seq_len=100, key_cache_token_stride=0)
     assert capi.paged_attention_plan(attention_args(**changes)) == "attention_row_kernel"
     assert capi.paged_attention_plan(attention_args(**{**changes, "num_tokens": 2**24 - 1024})) == "attention_short_kernel<2>"
+
+
+def test_plan_of_more_blocks_than_31_bits_count():
+    """Equal shares are cut from a sum of all blocks of 16 keys; where the tables could hold 2^31 of them, clusters."""
+    batch = dict(num_tokens=64, num_seqs=64, max_seq_len=8192)
+    shares = "attention_shared_kernel<1> + attention_join_parts_kernel"
+    assert capi.paged_attention_plan(attention_args(**batch, table_width=2**20)) == shares
+    assert capi.paged_attention_plan(attention_args(**batch, table_width=2**25)) == "attention_short_kernel<1>"
+    assert capi.paged_attention_plan(attention_args(**batch, table_width=2**31 - 1, page_size=2**20)) == "attention_short_kernel<1>"
+    assert capi.paged_attention_workspace(attention_args(**batch, table_width=2**25)) == 0
