@@ -35,7 +35,12 @@ struct CacheList {
     char* cache[kMaxCachesPerLaunch];
 };
 
-// Exclusive prefix sum over the CTA; `total` gets the sum. `warp_sums`: kPlanWarps ints of shared
+// a + b of non-negative numbers, INT32_MAX where the sum is past it.
+__device__ __forceinline__ int saturating_add(int a, int b) {
+    return static_cast<int>(min(static_cast<unsigned>(a) + static_cast<unsigned>(b), static_cast<unsigned>(INT32_MAX)));
+}
+
+// Exclusive prefix sum of non-negative numbers over the CTA, saturating; `total` gets the sum. `warp_sums`: kPlanWarps ints of shared
 // memory, free for reuse after the call's own barriers.
 __device__ __forceinline__ int block_exclusive_sum(int value, int* warp_sums, int* total) {
     const int lane = threadIdx.x % kWarpSize, warp = threadIdx.x / kWarpSize;
@@ -43,7 +48,7 @@ __device__ __forceinline__ int block_exclusive_sum(int value, int* warp_sums, in
 #pragma unroll
     for (int offset = 1; offset < kWarpSize; offset *= 2) {
         const int below = __shfl_up_sync(0xffffffffu, inclusive, offset);
-        if (lane >= offset) inclusive += below;
+        if (lane >= offset) inclusive = saturating_add(inclusive, below);
     }
     if (lane == kWarpSize - 1) warp_sums[warp] = inclusive;
     __syncthreads();
@@ -52,7 +57,7 @@ __device__ __forceinline__ int block_exclusive_sum(int value, int* warp_sums, in
 #pragma unroll
         for (int offset = 1; offset < kWarpSize; offset *= 2) {
             const int below = __shfl_up_sync(0xffffffffu, sum, offset);
-            if (lane >= offset) sum += below;
+            if (lane >= offset) sum = saturating_add(sum, below);
         }
         if (lane < kPlanWarps) warp_sums[lane] = sum;
     }
@@ -60,7 +65,7 @@ __device__ __forceinline__ int block_exclusive_sum(int value, int* warp_sums, in
     const int before = warp == 0 ? 0 : warp_sums[warp - 1];
     *total = warp_sums[kPlanWarps - 1];
     __syncthreads();
-    return before + inclusive - value;
+    return saturating_add(before, inclusive - value);
 }
 
 // ---- claiming pages ----------------------------------------------------------------------------
@@ -131,8 +136,8 @@ __global__ void __launch_bounds__(kPlanThreads) page_claim_kernel(const ClaimPar
         }
         int total = 0;
         const int before = block_exclusive_sum(need, warp_sums, &total);
-        if (i < p.count) first[i] = marked ? needed + before : -1;
-        needed = total > INT32_MAX - needed ? INT32_MAX : needed + total;
+        if (i < p.count) first[i] = marked ? saturating_add(needed, before) : -1;
+        needed = saturating_add(needed, total);
     }
 
     int found = 0;

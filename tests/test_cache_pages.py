@@ -331,3 +331,20 @@ def test_workspace_and_empty_calls():
     assert capi.compact_pages_workspace(100) >= 4 * 300
     capi.copy_pages(caches(), 20, 0, 0)
     capi.release_sequences(pool(), 0, 0)
+
+
+@gpu
+@pytest.mark.parametrize("rows, width", [(1024, 2**21), (1024, 2**21 + 8), (16384, 140000)])
+def test_needs_past_31_bits_change_nothing(rows, width):
+    """A round of 1024 rows, or the rounds before one, that lack 2^31 pages and more (a little less in the first case).
+    The rows of the tables are one row shown many times, which a call that changes nothing does not write."""
+    require_cuda()
+    table = torch.full((width,), -1, dtype=torch.int32, device="cuda")
+    lens = torch.arange(rows, dtype=torch.int32, device="cuda") % 7
+    refs = torch.zeros(100, dtype=torch.int32, device="cuda")
+    index = torch.arange(rows, dtype=torch.int32, device="cuda")
+    expected = lens.clone()
+    status = extension.reserve_pages(table.expand(rows, -1), lens, refs, index, torch.full_like(index, width), 1)
+    lacking = min(rows * width - int(expected.sum()), 2**31 - 1) - 100
+    assert status.tolist() == [lacking]
+    assert torch.equal(lens, expected) and not refs.any() and (table == -1).all()
