@@ -26,7 +26,10 @@ def rotary_frequencies(
       linear mix by ``original / wavelength`` between them;
     * ``yarn``: a pair that turns ``beta_fast`` times or more over the original context kept, one that
       turns ``beta_slow`` times or less divided by ``factor``, a linear ramp over the pair's number
-      between them; cosines and sines times ``attention_factor`` (default ``0.1 ln(factor) + 1``).
+      between them, its ends rounded outwards to whole pairs unless ``truncate`` is false; cosines and
+      sines times ``attention_factor``, by default ``m(mscale) / m(mscale_all_dim)`` where the configuration
+      has both and ``m(1)`` where it has neither, ``m(s) = 0.1 s ln(factor) + 1``. One of the two
+      alone, and ``attn_factor`` and ``extrapolation_factor`` other than 1, are refused.
     """
     if rotary_dim < 2 or rotary_dim % 2 != 0:
         raise ValueError("rotary dimension must be even and positive")
@@ -60,10 +63,24 @@ def rotary_frequencies(
         """The (fractional) number of the pair that turns so often over the original context."""
         return rotary_dim * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-    low, high = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), rotary_dim - 1)
+    for other in ("attn_factor", "extrapolation_factor"):
+        if scaling.get(other) not in (None, 1):
+            raise ValueError(f"unsupported key of a yarn rope scaling: {other}")
+    low, high = pair_of(fast), pair_of(slow)
+    if scaling.get("truncate", True):
+        low, high = math.floor(low), math.ceil(high)
+    low, high = max(low, 0), min(high, rotary_dim - 1)
     ramp = ((pair / 2 - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
     attention = scaling.get("attention_factor")
-    attention = float(attention) if attention is not None else 0.1 * math.log(factor) + 1.0
+    if attention is not None:
+        attention = float(attention)
+    else:
+        attention = 0.1 * math.log(factor) + 1.0
+        mscale, mscale_all = scaling.get("mscale"), scaling.get("mscale_all_dim")
+        if (mscale is None) != (mscale_all is None):
+            raise ValueError("mscale and mscale_all_dim of a yarn rope scaling must be given together")
+        if mscale is not None:
+            attention = (0.1 * float(mscale) * math.log(factor) + 1.0) / (0.1 * float(mscale_all) * math.log(factor) + 1.0)
     return frequencies * ((1.0 - ramp) + ramp / factor), attention
 
 

@@ -275,3 +275,47 @@ def test_scaled_frequencies():
 def test_table_refusals(args, kwargs, message):
     with pytest.raises(ValueError, match=message):
         rotary_frequencies(*args, **kwargs)
+
+
+def test_yarn_factor_from_two_scales():
+    """The factor on cosines and sines that m(s) = 0.1 s ln(factor) + 1 gives, and its precedence."""
+    yarn = dict(rope_type="yarn", factor=40.0, original_max_position_embeddings=4096)
+    log = math.log(40.0)
+    for more, want in (
+        (dict(), 0.1 * log + 1),
+        (dict(mscale=1.0, mscale_all_dim=1.0), 1.0),
+        (dict(mscale=0.707, mscale_all_dim=0.707), 1.0),
+        (dict(mscale=1.0, mscale_all_dim=0.0), 0.1 * log + 1),
+        (dict(mscale=1, mscale_all_dim=0.5), (0.1 * log + 1) / (0.05 * log + 1)),
+        (dict(mscale=1.0, mscale_all_dim=1.0, attention_factor=1.25), 1.25),
+        (dict(mscale=0.5, attention_factor=1.25), 1.25),
+        (dict(mscale=None, mscale_all_dim=None, attn_factor=1, extrapolation_factor=1.0), 0.1 * log + 1),
+    ):
+        frequencies, factor = rotary_frequencies(64, 10000.0, {**yarn, **more})
+        assert factor == pytest.approx(want, rel=1e-15)
+        assert torch.equal(frequencies, rotary_frequencies(64, 10000.0, yarn)[0])
+
+
+def test_yarn_ramp_without_rounding():
+    """truncate=False: the ramp begins and ends where a pair would turn beta_fast and beta_slow times."""
+    dim, base, original, by = 64, 150000.0, 4096, 32.0
+    yarn = dict(rope_type="yarn", factor=by, original_max_position_embeddings=original, beta_fast=32.0, beta_slow=1.0)
+    plain, _ = rotary_frequencies(dim, base)
+    scaled, _ = rotary_frequencies(dim, base, {**yarn, "truncate": False})
+    # Pair i turns original / (2 pi base^(2 i / dim)) times: i as a function of the turns.
+    at = [math.log(original / (2 * math.pi * turns), base) * dim / 2 for turns in (32.0, 1.0)]
+    for i in range(dim // 2):
+        kept = 1 - min(max((i - at[0]) / (at[1] - at[0]), 0.0), 1.0)
+        assert scaled[i].item() == pytest.approx(plain[i].item() * (kept + (1 - kept) / by), rel=1e-12)
+    rounded, _ = rotary_frequencies(dim, base, yarn)
+    assert torch.equal(rounded, rotary_frequencies(dim, base, {**yarn, "truncate": True})[0])
+    assert not torch.equal(rounded, scaled)
+
+
+@pytest.mark.parametrize("more, message", [
+    (dict(mscale=1.0), "given together"), (dict(mscale_all_dim=1.0), "given together"),
+    (dict(attn_factor=1.2), "attn_factor"), (dict(extrapolation_factor=0.5), "extrapolation_factor"),
+])
+def test_yarn_refusals(more, message):
+    with pytest.raises(ValueError, match=message):
+        rotary_frequencies(64, 10000.0, dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=4096, **more))
