@@ -180,8 +180,8 @@ IPL_API ipl_status ipl_rotary_embedding_cache_bf16(const ipl_rotary_args* args, 
  * t % page_size; table entries past a sequence's pages are never read, rows past its length never
  * matter, whatever they hold. Keys at masked positions never matter either; values that one token of a
  * sequence sees must be finite for its other tokens to be. A page number outside 0..num_pages-1
- * contributes nothing and sets bit 3 of the fault word. Rows of query that belong to no sequence are
- * not written.
+ * contributes nothing and sets bit 3 of the fault word; so do keys past the table's row or past 2^31 -
+ * 256. Rows of query that belong to no sequence are not written.
  *
  * Strides are in elements; the last dimension is contiguous; output overlaps none of the inputs.
  * max_query_len and max_seq_len are upper bounds of the lengths, known on the host: they choose the

@@ -88,9 +88,12 @@ __device__ __forceinline__ int sequence_of_token(const int32_t* starts, int num_
     return lo;
 }
 
-// A sequence's length as far as its row of the block table reaches.
+// The longest sequence whose keys, and those of a block or tile that begins below its end, 32 bits count.
+constexpr int kMostKeys = INT32_MAX - 255;
+
+// A sequence's length as far as its row of the block table and the count of keys reach.
 __device__ __forceinline__ int table_bounded_length(const AttentionParams& p, int seq) {
-    const int64_t most = static_cast<int64_t>(p.table_width) * p.page_size;
+    const int64_t most = min(static_cast<int64_t>(p.table_width) * p.page_size, static_cast<int64_t>(kMostKeys));
     const int len = p.lens[seq];
     if (len > most) {
         atomicOr(&g_fault_word, kFaultIndexOutOfRange);

@@ -597,3 +597,32 @@ def test_plan_of_more_blocks_than_31_bits_count():
     assert capi.paged_attention_plan(attention_args(**batch, table_width=2**25)) == "attention_short_kernel<1>"
     assert capi.paged_attention_plan(attention_args(**batch, table_width=2**31 - 1, page_size=2**20)) == "attention_short_kernel<1>"
     assert capi.paged_attention_workspace(attention_args(**batch, table_width=2**25)) == 0
+
+
+@gpu
+@pytest.mark.parametrize("heads, kv_heads, dim, new", [(28, 4, 128, 1), (28, 4, 128, 300), (32, 8, 64, 3), (6, 3, 256, 2)])
+def test_lengths_at_the_end_of_32_bits(heads, kv_heads, dim, new):
+    """A window at the end of the longest sequence there can be, and of a longer one, whose keys past it are left out.
+    All of its pages are the same few."""
+    require_cuda()
+    capi.clear_device_fault_flags(0)
+    page, window, pages = 16, 500, 48
+    q, kc, vc, _, starts, _ = make([new], [pages * page], heads, kv_heads, dim, spare=0)
+    width = 2**31 // page
+    tables = (torch.arange(width, device="cuda", dtype=torch.int32) % pages)[None]
+    for total in (2**31 - 256, 2**31 - 1):
+        lens = torch.tensor([total], dtype=torch.int32, device="cuda")
+        got = extension.paged_attention(q, kc, vc, tables, starts, lens, new, 2**30 - 1, dim**-0.5, window)
+        assert capi.device_fault_flags(0) == (0 if total == 2**31 - 256 else 8)
+        capi.clear_device_fault_flags(0)
+        # The formula over the last 2048 places, those past the limit left out.
+        place = torch.arange(2**31 - 2048, min(total, 2**31 - 256), device="cuda", dtype=torch.int64)
+        keys, values = (c[(place // page % pages), place % page].double() for c in (kc, vc))
+        position = total - new + torch.arange(new, device="cuda", dtype=torch.int64)
+        seen = (place[None] <= position[:, None]) & (place[None] > position[:, None] - window)
+        for h in range(heads):
+            g = h // (heads // kv_heads)
+            logits = (q[:, h].double() @ keys[:, g].T * dim**-0.5).masked_fill(~seen, -torch.inf)
+            w = torch.softmax(logits, -1)
+            want, size = w @ values[:, g], w @ values[:, g].abs()
+            assert ((got[:, h].double() - want).abs() <= attention_bound(want, size)).all()
