@@ -74,7 +74,7 @@ struct TileLayout {
 // 2^x = 2^n 2^r, n = x rounded (by adding 1.5 2^23, which leaves n in the low bits), r in [-1/2, 1/2],
 // with the polynomial of degree 3 of least relative error for 2^r (7.5e-5 by the Remez exchange, a fiftieth
 // of the rounding of a weight to bf16). x is held above -126, so a vanishing weight is 2^-126, not 0, and so is that of
-// NaN: a row whose maximum is not finite is seen to at its end.
+// NaN: rows whose maximum is not finite are seen to where it is taken and at their end.
 __device__ __forceinline__ F32x2 exp2_pair_units(F32x2 x) {
     float a, b;
     f32x2_split(x, a, b);
@@ -243,17 +243,19 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
         asm volatile("prefetch.global.L1 [%0];" ::"l"(a.lens + threadIdx.x));
     }
     const auto weight = [&](int u, TilePair& pair) { return u < p.units && tile_pair(p, u, pair) ? pair.steps + kTilePairCost : 0; };
-    // Sum over the CTA up to and with this thread; `total` gets all of it.
-    const auto sum_through = [&](int64_t value, int64_t& total) {
-        int64_t through = value;
+    // Sum over the CTA up to and with this thread; `total` gets all of it. Over a warp in the value's type: 32 bits
+    // hold the weights of 32 pairs.
+    const auto sum_through = [&](auto value, int64_t& total) -> int64_t {
+        auto in_warp = value;
 #pragma unroll
         for (int offset = 1; offset < kWarpSize; offset *= 2) {
-            const int64_t below = __shfl_up_sync(0xffffffffu, through, offset);
-            if (lane >= offset) through += below;
+            const auto below = __shfl_up_sync(0xffffffffu, in_warp, offset);
+            if (lane >= offset) in_warp += below;
         }
         __syncthreads();
-        if (lane == kWarpSize - 1) scratch[warp] = through;
+        if (lane == kWarpSize - 1) scratch[warp] = in_warp;
         __syncthreads();
+        int64_t through = in_warp;
         total = 0;
         for (int i = 0; i < kTileThreads / kWarpSize; ++i) {
             if (i == warp) through += total;
@@ -668,7 +670,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 const bool move = top < INFINITY && !(m <= top + 8.0f);
                 if (__any_sync(0xffffffffu, move)) {
                     const float keep = move ? exp2_approx(top - m) : 1.0f;
-                    sum *= keep;
+                    sum = sum * keep + (move ? m - m : 0.0f);  // the polynomial hides +inf and NaN, this does not
                     top = move ? m : top;
                     __syncwarp();
                     if (step > 0) {
@@ -731,9 +733,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 tcgen05_fence_after();
             }
             if (!ok) break;
-            // The polynomial gives 2^-126 for -inf and NaN. A maximum of -inf: no weight. Of +inf or NaN: NaN.
-            sum = top == -INFINITY ? 0.0f : sum + (top - top);
-            const float inverse = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+            // At least 1 where a score was above -inf; what the polynomial adds for -inf alone stays below 2^-64.
+            const float inverse = sum > 0x1p-64f || sum != sum ? 1.0f / sum : 0.0f;
             const int r = row(), in_tile = row_token(r);
             const bool real = in_tile < p.tile_tokens && t * p.tile_tokens + in_tile < item.tokens;
             const int slot = item.slot;

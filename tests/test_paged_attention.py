@@ -572,6 +572,7 @@ def test_more_rows_of_a_group_than_31_bits_count():
     q = flat.as_strided((tokens, 128, 8), (8, 8, 1))
     starts[1] = tokens
     out = torch.full((tokens, 128, 8), 7.0, dtype=torch.bfloat16, device="cuda")
+    extension.load_extension()
     torch.ops.inference_performance_lab.paged_attention(out, q, kc, vc, tables, starts, lens, tokens, 100, 0.35, 0)
     assert all(bool((part == 0).all()) for part in out[:-100].split(2**20))
     expected, size = attention(q[-100:], kc, vc, tables, torch.tensor([0, 100]), lens, 0.35)
