@@ -294,24 +294,24 @@ int64_t key_turns(int64_t keys) { return (keys + kShortWarps * kAttentionBlock -
 
 // CTAs of the short kernel that the GPU holds in clusters of this size: a cluster stays within a part of the GPU,
 // which leaves some SMs out (72 clusters of 4 and 36 of 8 took a second wave on 296 places, 116 of 2 did not).
-int64_t short_resident(int tiles, int sm_count, int cluster) {
+int64_t short_resident(int sm_count, int cluster) {
     const int64_t places = static_cast<int64_t>(sm_count) * kShortCtas;
     return cluster == 1 ? places : cluster <= 4 ? places * 7 / 8 : places * 3 / 4;
 }
 
 // CTAs a cluster: as many as the GPU holds of all of them, up to one for each turn.
-int short_cluster(int64_t units, int64_t keys, int tiles, int sm_count) {
+int short_cluster(int64_t units, int64_t keys, int sm_count) {
     int cluster = 1;
-    while (cluster < kShortCluster && cluster < key_turns(keys) && units * cluster * 2 <= short_resident(tiles, sm_count, cluster * 2)) {
+    while (cluster < kShortCluster && cluster < key_turns(keys) && units * cluster * 2 <= short_resident(sm_count, cluster * 2)) {
         cluster *= 2;
     }
     return cluster;
 }
 
 // Estimates of the two kernels' times in ns, within a fifth of those measured at 1-256 tokens a sequence, 1-148
-// sequences and 36-8192 keys (28 and 4 heads of 128).
-int64_t short_time(int64_t units, int64_t keys, int tiles, int sm_count, int cluster) {
-    const int64_t held = short_resident(tiles, sm_count, cluster), waves = (units * cluster + held - 1) / held;
+// sequences and 36-8192 keys, all of one layout: 28 and 4 heads of 128. Others go by the same constants.
+int64_t short_time(int64_t units, int64_t keys, int sm_count, int cluster) {
+    const int64_t held = short_resident(sm_count, cluster), waves = (units * cluster + held - 1) / held;
     return 3000 + waves * (2500 + 1300 * ((key_turns(keys) + cluster - 1) / cluster));
 }
 int64_t tile_time(int64_t pairs, int64_t keys, int sm_count) {
@@ -343,7 +343,7 @@ AttentionPlan plan_attention(const ipl_paged_attention_args& a, int sm_count) {
         const int64_t most = (rows + 15) / 16, tiles = a.num_tokens * group / 16 + a.num_seqs;
         const int64_t units = (tiles < most * a.num_seqs ? tiles : most * a.num_seqs) * a.num_kv_heads;
         const int64_t pairs = (a.num_tokens * group / (2 * kTileRows) + a.num_seqs) * a.num_kv_heads;
-        if (group <= kTileRows && mappable && short_time(units, keys, 2, sm_count, short_cluster(units, keys, 2, sm_count)) > tile_time(pairs, keys, sm_count)) {
+        if (group <= kTileRows && mappable && short_time(units, keys, sm_count, short_cluster(units, keys, sm_count)) > tile_time(pairs, keys, sm_count)) {
             plan.tile = true;
             plan.tiles = group <= 8 ? 1 : 2;
             plan.short_rows = plan.tiles * 8;
@@ -371,7 +371,7 @@ AttentionPlan plan_attention(const ipl_paged_attention_args& a, int sm_count) {
         const bool countable = a.num_seqs <= INT_MAX / (longest / kAttentionBlock + 1 + kShortPairCost);
         const int64_t units = a.num_seqs * a.num_kv_heads * plan.row_tiles;
         const int64_t resident = static_cast<int64_t>(sm_count) * shared_ctas(plan.tiles);
-        plan.cluster = short_cluster(units, keys, plan.tiles, sm_count);
+        plan.cluster = short_cluster(units, keys, sm_count);
         if (plan.row_tiles == 1 && countable && (units * plan.cluster > resident || key_turns(keys) > 16 * plan.cluster)) {
             plan.cluster = 0;
             plan.shared_ctas = static_cast<int>(resident);
