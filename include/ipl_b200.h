@@ -174,7 +174,9 @@ IPL_API ipl_status ipl_rotary_embedding_cache_bf16(const ipl_rotary_args* args, 
  *   output = sum_t w_t v_t / sum_t w_t,   w_t = exp(scale q.k_t - max_t scale q.k_t)
  *
  * with fp32 scores, statistics and sums, rounded to bf16 once; the weights enter the product with the
- * values rounded to bf16 (their fp32 sum is the denominator). A token that sees no key gives 0, and so
+ * values rounded to bf16 (their fp32 sum is the denominator), and are off by up to 1e-4 of themselves
+ * before that (approximate exponentials). Equal calls give equal bits; which keys are summed together
+ * depends on all sequences of a call, so in another call a sequence's last bits may differ. A token that sees no key gives 0, and so
  * does one all of whose scores are -infinity; NaN and +infinity among its scores give NaN. Query head h
  * reads key head h / (num_heads / num_kv_heads). Key t lies in page block_tables[s][t / page_size], row
  * t % page_size; table entries past a sequence's pages are never read, rows past its length never
@@ -227,7 +229,8 @@ IPL_API const char* ipl_paged_attention_plan(const ipl_paged_attention_args* arg
  *
  * status receives 0, or the number of free pages lacking, or -1 for an entry out of range (a row, a
  * length, a row given twice, a child that holds tokens); unless it is 0 nothing has changed. A call
- * takes up to 16384 rows.
+ * takes up to 16384 rows. Lengths and tables change through these calls alone: a claim writes the
+ * entries past a row's length, and a page that still stood there keeps its reference for good.
  *
  * ipl_copy_pages: page pairs[2 i] to page pairs[2 i + 1] in every cache; negative entries are skipped.
  *   No target may be the source or target of another pair.

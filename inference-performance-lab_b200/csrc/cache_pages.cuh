@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(kPageCopyThreads) page_fork_kernel(const __gri
     // Cache after cache, so that a parent's page is read from HBM once for all of its children. Release, fork and
     // reserve of 96 children of 16 parents in 56 caches: 87 us, child after child 121 (with two
     // accesses in flight; with four, cache after cache is still 87). Where the 59 MB of parents'
-    // pages are in L2 already, the two orders are level (release and fork 77 and 78 us).
+    // pages are in L2 already, the two orders are level (release and fork 77 and 78 us, 76 since).
     const uint32_t cache = blockIdx.x / p.count, child = blockIdx.x - cache * p.count;
     const int row = p.children[child], len = s.lens[row];  // the parent's
     const int whole = len / s.page_size, used = len % s.page_size;

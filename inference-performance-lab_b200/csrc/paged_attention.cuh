@@ -159,7 +159,7 @@ __device__ __forceinline__ void write_joined(uint16_t* out, float weight, const 
 // The tile kernel's parts, kDim / 32 elements a lane. Many pairs in few parts each (kSplit false): block (c, y) takes 64
 // rows, a warp 8 of them at once; with a row a warp the blocks were four waves of start-up latency (19 us after 147
 // cut pairs). Few pairs in many parts: block (c, y) takes 8 rows, its warps share the parts (18
-// tokens on 8192 keys, the whole call: 22.7 us, one after the other 35.1).
+// tokens on 8192 keys, the whole call: 22.7 us, one after the other 35.1; 23.1 since).
 constexpr int kJoinRows = 8, kJoinWarps = 8;
 
 template <int kDim, bool kSplit>

@@ -185,7 +185,9 @@ def paged_attention(
     Sequence ``s`` owns rows ``query_start_loc[s]:query_start_loc[s + 1]`` of ``query`` and has
     ``seq_lens[s]`` tokens in the cache, those included; its pages are ``block_tables[s]`` (all int32).
     ``max_query_len`` and ``max_seq_len`` bound the lengths; ``window`` > 0 limits each token to the last
-    ``window`` keys. A token that sees no key gives 0; rows of no sequence are left unwritten.
+    ``window`` keys. A token that sees no key gives 0, and so does one all of whose scores are -infinity;
+    rows of no sequence are left unwritten. Head sizes that are multiples of 8 up to 128 over pages of a
+    multiple of 16 tokens are the fast ones; others, up to 256, are slower than plain torch operations.
     """
     output = torch.empty_like(query, memory_format=torch.contiguous_format)
     _op("paged_attention")(
@@ -211,7 +213,7 @@ def reserve_pages(
 ) -> torch.Tensor:
     """Gives ``rows[i]`` pages for ``new_lens[i]`` tokens, in place. Returns an int32 ``[1]`` status on
     the device: 0, the number of free pages lacking, or -1 for an entry out of range; unless it is 0
-    nothing has changed."""
+    nothing has changed. A length lowered by hand loses the pages past it once the row grows again."""
     return _op("reserve_pages")(
         block_tables, seq_lens, ref_counts, rows, new_lens, page_size
     )
